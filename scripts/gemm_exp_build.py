@@ -95,6 +95,6 @@ open(src, "w").write(s.replace('#include "common.h"', '#include "../nlp-cube_amd
 sys.path.insert(0, ROOT)
 import __graft_entry__ as g  # noqa: E402
 others = [os.path.join(CSRC, f) for f in g.SOURCES if f != "gemm.hip"]
-subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-w", "-o",
+subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-std=c++17", "-fPIC", "-shared", "-w", "-o",
                        os.path.join(ROOT, "ab_tmp/lib_%s.so" % name), src] + others)
 print("built", name)

@@ -30,7 +30,7 @@ src = os.path.join(CSRC, "_lstm_exp_%s.hip" % name)
 open(src, "w").write(s)
 out = os.path.join(ROOT, "ab_tmp", "lib_lstm_%s.so" % name)
 try:
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-o", out, src,
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-std=c++17", "-fPIC", "-shared", "-o", out, src,
                     os.path.join(CSRC, "rowops.hip")], check=True, cwd=CSRC)
 finally:
     os.remove(src)

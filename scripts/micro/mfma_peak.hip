@@ -1,6 +1,6 @@
 // Sustained matrix-core rate of one MI355X for the two instructions the hot kernels use, nothing but MFMAs in the loop
 // (operands stay in registers): what the chip holds under its power limit, to read roofline fractions against.
-//   hipcc --offload-arch=gfx950 -O3 -o ab_tmp/mfma_peak scripts/micro/mfma_peak.hip && ./ab_tmp/mfma_peak
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o ab_tmp/mfma_peak scripts/micro/mfma_peak.hip && ./ab_tmp/mfma_peak
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #ifndef RANDOM_DATA

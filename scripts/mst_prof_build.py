@@ -52,6 +52,6 @@ extern "C" int cube_mst_prof(long long* out) { return hipMemcpyFromSymbol(out, H
 s = s.replace('#include "common.h"', '#include "../nlp-cube_amd/csrc/common.h"').replace('#include "../../include/cube_hip.h"', '#include "../include/cube_hip.h"')
 os.makedirs(os.path.join(ROOT, "ab_tmp"), exist_ok=True)
 open(os.path.join(ROOT, "ab_tmp/mst_prof.hip"), "w").write(s)
-subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-w", "-o",
+subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-std=c++17", "-fPIC", "-shared", "-w", "-o",
                        os.path.join(ROOT, "ab_tmp/mst_prof.so"), os.path.join(ROOT, "ab_tmp/mst_prof.hip"),
                        os.path.join(ROOT, "nlp-cube_amd/csrc/rowops.hip")])
