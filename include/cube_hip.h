@@ -30,6 +30,9 @@
  *                           (cube/networks/lemmatizer.py:160-167), Attention.forward
  *                           (modules.py:145-169), context bmm (lemmatizer.py:144-145)
  *   cube_lstm_cell          one time step of the decoder nn.LSTM cell (lemmatizer.py:152-154)
+ *
+ * Without a counterpart in the reference: 8-bit floating-point Linear layers (the cube_*_fp8 entries) and sampling from logits
+ * (cube_sample_rows).
  */
 #ifndef CUBE_HIP_H
 #define CUBE_HIP_H
@@ -399,6 +402,57 @@ int cube_packfile_entry(const cube_packfile* f, int i, cube_pack_entry* out);
 int cube_packfile_find(const cube_packfile* f, const char* name, cube_pack_entry* out);
 int cube_packfile_int(const cube_packfile* f, const char* name, long long* value);
 void cube_packfile_close(cube_packfile* f);
+
+/* ---- 8-bit floating-point Linear layers with a scale for each block of 128 columns ------------------------------------
+ * A precision tier beside bf16 / bf16x3 / int8x2 for nn.Linear (cube/networks/modules.py:28-52) and for the Linear layers of
+ * an LM encoder (cube/networks/lm.py:178-179 calls one); there is no counterpart in the reference.
+ * Quantised rows (activations and weights alike): e4m3 bytes q [rows, ld_q], ld_q >= 128 * KB, KB = ceil(K / 128), zeros
+ * behind column K; scales as 32-bit words s [ceil(KB / 4), ld_s], ld_s >= rows: byte j of s[i, row] is the E8M0 exponent byte
+ * (the scale is 2^(byte - 127)) of columns 128 * (4i + j) ... of that row.                                              */
+enum { CUBE_T_F32 = 0, CUBE_T_BF16 = 1, CUBE_T_F16 = 2, CUBE_T_E4M3 = 3 };
+enum { CUBE_FP8_NONE = 0, CUBE_FP8_TANH = 1, CUBE_FP8_RELU = 2 };
+
+/* x [M, ld_x] (f32, bf16 or f16) -> q, scale.  Per row and block: e = the smallest integer >= -127 with max|x| <= 448 * 2^e over
+ * the finite values, q = e4m3(x * 2^-e), nearest, ties to even; an infinity or NaN becomes e4m3's NaN.  q: 16-byte aligned rows;
+ * K <= 2^24.                                                                                                             */
+int cube_quant_fp8(const void* x, int x_type, long long ld_x, int M, int K, void* q, long long ld_q, uint32_t* scale, int ld_s,
+                   void* stream);
+
+/* out[m, n] = act(bias[n] + sum_k a[m, k] * w[n, k]), rounded once to out_type; sums in fp32.  Leading dimensions in elements;
+ * bias may be NULL; out may be any 4- or 2-byte aligned matrix.  Rows and columns that 2^(ea + ew) times a sum takes out of
+ * fp32's range become infinities, as in fp32 arithmetic.  Calls on one stream need no synchronisation between them.        */
+typedef struct cube_fp8_args {
+  const void* A; int a_type; long long lda; const uint32_t* A_scale; int lds_a; int M;
+  const void* W; long long ldw; const uint32_t* W_scale; int lds_w; int N; int K;
+  const float* bias; int act;
+  void* out; int out_type; long long ldo;
+} cube_fp8_args;
+/* A: quantised rows (a_type CUBE_T_E4M3, lda and ldw multiples of 16, 16-byte aligned).                                  */
+int cube_gemm_fp8(const cube_fp8_args* args, void* stream);
+/* A: plain rows (f32, bf16, f16), quantised on the way as cube_quant_fp8 does; A_scale and lds_a are not read.  ws: device memory
+ * of cube_linear_fp8_workspace_bytes(M, N, K) bytes, 16-byte aligned, the call's own until it has run on the stream.       */
+size_t cube_linear_fp8_workspace_bytes(int M, int N, int K);
+int cube_linear_fp8(const cube_fp8_args* args, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- sampling ---------------------------------------------------------------------------------------------------------
+ * One token a row from logits [M, ld] (V columns), beside the arg-max of a greedy decoder (cube/networks/lemmatizer.py:160-167).
+ * Candidates are the logits above -inf, in order of falling logit, ties lowest index first; w = exp((z - max) / temperature).
+ * Kept: the first top_k (<= 0 or >= V: all), of these the shortest prefix whose w add up to top_p times their sum (>= 1: all; <= 0:
+ * the first), of these the ones with w >= min_p (<= 0: all; >= 1: those equal to the largest).  token = index of the first
+ * kept candidate at which the running sum of w exceeds u times the kept sum (u in [0, 1), one per row, clamped to it);
+ * prob (may be NULL) = its w over that sum.  temperature <= 0 or NaN: the arg-max, prob 1.  A row without candidates: token
+ * -1, prob 0.  NaN logits are no candidates; +inf logits share the whole weight.
+ * temperature / top_k / top_p / min_p: device arrays of M, or NULL for the scalar beside each.  Weights are added in 64-bit
+ * fixed point: the token does not depend on how the row is split.                                                         */
+#define CUBE_SAMPLE_MAX_V (1 << 22)
+typedef struct cube_sample_args {
+  const void* logits; int type; long long ld; int M; int V;
+  const double* u;
+  const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;
+  float temperature0; int top_k0; float top_p0; float min_p0;
+  int32_t* token; float* prob;
+} cube_sample_args;
+int cube_sample_rows(const cube_sample_args* args, void* stream);
 
 #ifdef __cplusplus
 }

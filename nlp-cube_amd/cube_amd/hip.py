@@ -10,7 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libcubehip.so")
 
 EPI_F32, EPI_BF16, EPI_BF16_TANH, EPI_BF16_RELU, EPI_GATE, EPI_LSTM = 0, 1, 2, 3, 4, 5
-ABI_VERSION = 19  # include/cube_hip.h; a stale libcubehip.so is refused
+ABI_VERSION = 20  # include/cube_hip.h; a stale libcubehip.so is refused
 
 c_int, c_void_p, c_size_t = ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
 
@@ -76,6 +76,23 @@ class LemmaAttendArgs(ctypes.Structure):
         ("out_char", c_void_p), ("out_case", c_void_p), ("ld_out", c_int),
         ("eol", c_int), ("done", c_void_p), ("n_done", c_void_p),
     ]
+
+
+class Fp8Args(ctypes.Structure):
+    """cube_fp8_args (include/cube_hip.h)."""
+    _fields_ = [("A", c_void_p), ("a_type", c_int), ("lda", ctypes.c_longlong), ("A_scale", c_void_p), ("lds_a", c_int), ("M", c_int),
+                ("W", c_void_p), ("ldw", ctypes.c_longlong), ("W_scale", c_void_p), ("lds_w", c_int), ("N", c_int), ("K", c_int),
+                ("bias", c_void_p), ("act", c_int),
+                ("out", c_void_p), ("out_type", c_int), ("ldo", ctypes.c_longlong)]
+
+
+class SampleArgs(ctypes.Structure):
+    """cube_sample_args (include/cube_hip.h)."""
+    _fields_ = [("logits", c_void_p), ("type", c_int), ("ld", ctypes.c_longlong), ("M", c_int), ("V", c_int),
+                ("u", c_void_p),
+                ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("min_p", c_void_p),
+                ("temperature0", ctypes.c_float), ("top_k0", c_int), ("top_p0", ctypes.c_float), ("min_p0", ctypes.c_float),
+                ("token", c_void_p), ("prob", c_void_p)]
 
 
 class Pair:
@@ -151,6 +168,11 @@ SIGNATURES = {
     "cube_lemma_attend": (c_int, [ctypes.POINTER(LemmaAttendArgs), c_void_p]),
     "cube_lstm_cell": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p,
                                c_void_p, c_int, c_void_p]),
+    "cube_quant_fp8": (c_int, [c_void_p, c_int, ctypes.c_longlong, c_int, c_int, c_void_p, ctypes.c_longlong, c_void_p, c_int, c_void_p]),
+    "cube_gemm_fp8": (c_int, [ctypes.POINTER(Fp8Args), c_void_p]),
+    "cube_linear_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "cube_linear_fp8": (c_int, [ctypes.POINTER(Fp8Args), c_void_p, c_size_t, c_void_p]),
+    "cube_sample_rows": (c_int, [ctypes.POINTER(SampleArgs), c_void_p]),
 }
 
 _lib = None
@@ -286,3 +308,202 @@ def masked_mean(layers, weights, ld_x, word_len, N, W, C, out, ld_out, word_rows
     check(fn(his, los, ws, n, ld_x, word_len.data_ptr(), N, W, C, out.hi.data_ptr(), ptr(out.lo),
              ld_out, ptr(word_rows), stream if stream is not None else stream_handle()),
           "cube_masked_mean")
+
+
+# ---- 8-bit floating-point Linear layers and sampling: calls on tensors ------------------------------------------------------
+# These take whole tensors, check them, and launch on the current stream of the tensors' own device.  Workspaces come from torch's
+# caching allocator per call: stream-ordered, and inside a graph capture from the graph's own pool.
+
+FP8_BLOCK = 128  # columns that share one scale
+FP8_ACTS = {None: 0, "none": 0, "tanh": 1, "relu": 2}
+_T = None
+
+
+def _type_code(dtype):
+    global _T
+    if _T is None:
+        import torch
+        _T = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return _T.get(dtype)
+
+
+class _on:
+    """The tensor's device as the current one (cheap when it already is)."""
+    __slots__ = ("want", "was")
+
+    def __init__(self, t):
+        self.want = t.device.index
+
+    def __enter__(self):
+        import torch
+        self.was = torch._C._cuda_getDevice()
+        if self.was != self.want:
+            torch._C._cuda_setDevice(self.want)
+        return torch._C._cuda_getCurrentRawStream(self.want)
+
+    def __exit__(self, *a):
+        if self.was != self.want:
+            import torch
+            torch._C._cuda_setDevice(self.was)
+
+
+def _matrix(who, name, t):
+    """A 2-D f32 / bf16 / f16 tensor on a GPU with neighbouring columns -> (type code, row stride)."""
+    code = _type_code(t.dtype)
+    if code is None or t.dim() != 2:
+        raise ValueError("%s: %s must be a 2-D float32, bfloat16 or float16 tensor, got %s %s" % (who, name, t.dtype, tuple(t.shape)))
+    if t.device.type != "cuda":
+        raise CubeHipError("%s: %s is on %s; it must be on an MI355X (there is no CPU fallback)" % (who, name, t.device))
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("%s: the columns of %s must be neighbours (stride 1), got stride %d" % (who, name, t.stride(1)))
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise ValueError("%s: the rows of %s overlap (row stride %d, %d columns)" % (who, name, ld, t.shape[1]))
+    return code, ld
+
+
+def _vector(who, name, t, n, dtype, device):
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+        raise ValueError("%s: %s must be a contiguous %s tensor of %d values on %s, got %s %s on %s"
+                         % (who, name, dtype, n, device, t.dtype, tuple(t.shape), t.device))
+    return t.data_ptr()
+
+
+def _no_grad(who, *tensors):
+    import torch
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
+
+
+class Fp8Rows:
+    """Quantised rows: q uint8 [rows, 128 * KB] (e4m3), scale int32 [ceil(KB / 4), rows] (four E8M0 bytes a word), KB =
+    ceil(columns / 128): the layout of cube_quant_fp8 (include/cube_hip.h)."""
+    __slots__ = ("q", "scale", "columns")
+
+    def __init__(self, q, scale, columns):
+        import torch
+        kb = -(-columns // FP8_BLOCK)
+        if columns < 1 or q.dtype != torch.uint8 or q.dim() != 2 or q.shape[1] != kb * FP8_BLOCK or not q.is_contiguous():
+            raise ValueError("Fp8Rows: q must be a contiguous uint8 [rows, %d] tensor for %d columns, got %s %s"
+                             % (kb * FP8_BLOCK, columns, q.dtype, tuple(q.shape)))
+        if scale.dtype != torch.int32 or tuple(scale.shape) != (-(-kb // 4), q.shape[0]) or not scale.is_contiguous() or \
+                scale.device != q.device:
+            raise ValueError("Fp8Rows: scale must be a contiguous int32 %s tensor beside q, got %s %s on %s"
+                             % ((-(-kb // 4), q.shape[0]), scale.dtype, tuple(scale.shape), scale.device))
+        self.q, self.scale, self.columns = q, scale, columns
+
+    @property
+    def rows(self):
+        return self.q.shape[0]
+
+    def to(self, device):
+        return Fp8Rows(self.q.to(device), self.scale.to(device), self.columns)
+
+    def float(self):
+        """The values the rows stand for, f32 [rows, columns]."""
+        import torch
+        kb = self.q.shape[1] // FP8_BLOCK
+        e = self.scale.t().contiguous().view(torch.uint8)[:, :kb].to(torch.int32) - 127
+        v = self.q.view(torch.float8_e4m3fn).float().reshape(self.rows, kb, FP8_BLOCK)
+        return torch.ldexp(v, e[:, :, None]).reshape(self.rows, -1)[:, :self.columns]
+
+
+def quant_fp8(x):
+    """x [M, K] (f32, bf16, f16) -> Fp8Rows (cube_quant_fp8)."""
+    import torch
+    code, ld = _matrix("quant_fp8", "x", x)
+    _no_grad("quant_fp8", x)
+    M, K = x.shape
+    kb = -(-K // FP8_BLOCK)
+    with _on(x) as stream:
+        q = torch.empty((M, kb * FP8_BLOCK), dtype=torch.uint8, device=x.device)
+        scale = torch.empty((-(-kb // 4), M), dtype=torch.int32, device=x.device)
+        check(load().cube_quant_fp8(x.data_ptr(), code, ld, M, K, q.data_ptr(), kb * FP8_BLOCK, scale.data_ptr(), M, stream), "cube_quant_fp8")
+    return Fp8Rows(q, scale, K)
+
+
+def _fp8_call(who, a, K, w, bias, act, out, out_dtype):
+    """What gemm_fp8 and linear_fp8 check alike -> (output, its Fp8Args fields behind the activations')."""
+    import torch
+    device = a.device
+    if w.columns != K:
+        raise ValueError("%s: the weight has %d columns, the input %d" % (who, w.columns, K))
+    if w.q.device != device:
+        raise ValueError("%s: the weight is on %s, the input on %s" % (who, w.q.device, device))
+    if act not in FP8_ACTS:
+        raise ValueError("%s: act must be None, 'none', 'tanh' or 'relu', got %r" % (who, act))
+    M, N = a.shape[0], w.rows
+    _no_grad(who, a, bias)
+    if out is None:
+        if _type_code(out_dtype) is None:
+            raise ValueError("%s: the output must be float32, bfloat16 or float16, got %s" % (who, out_dtype))
+        out = torch.empty((M, N), dtype=out_dtype, device=device)
+    elif tuple(out.shape) != (M, N) or out.device != device or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("%s: out must be a %s tensor of type %s on %s, got %s %s on %s"
+                         % (who, (M, N), out_dtype, device, tuple(out.shape), out.dtype, out.device))
+    code, ldo = _matrix(who, "out", out)
+    return out, (w.q.data_ptr(), w.q.shape[1], w.scale.data_ptr(), w.scale.shape[1], N, K,
+                 None if bias is None else _vector(who, "bias", bias, N, torch.float32, device), FP8_ACTS[act],
+                 out.data_ptr(), code, ldo)
+
+
+def gemm_fp8(a, w, bias=None, act=None, out=None, out_dtype=None):
+    """act(a @ w.T + bias) of two Fp8Rows (cube_gemm_fp8): a [M, K], w [N, K] -> [M, N] of out_dtype (bfloat16 unless given).
+    bias: f32 [N]; act: None, 'tanh', 'relu'; out: where to (rows may be strided)."""
+    import torch
+    if a.q.device.type != "cuda":
+        raise CubeHipError("gemm_fp8: the rows are on %s; they must be on an MI355X (there is no CPU fallback)" % a.q.device)
+    if out is None and out_dtype is None:
+        out_dtype = torch.bfloat16
+    with _on(a.q) as stream:
+        out, rest = _fp8_call("gemm_fp8", a.q, a.columns, w, bias, act, out, out_dtype)
+        args = Fp8Args(a.q.data_ptr(), 3, a.q.shape[1], a.scale.data_ptr(), a.scale.shape[1], a.rows, *rest)
+        check(load().cube_gemm_fp8(ctypes.byref(args), stream), "cube_gemm_fp8")
+    return out
+
+
+def linear_fp8(x, w, bias=None, act=None, out=None, out_dtype=None):
+    """act(quant_fp8(x) @ w.T + bias) in one call (cube_linear_fp8): x [M, K] f32 / bf16 / f16, w Fp8Rows [N, K] -> [M, N] of
+    out_dtype (x's type unless given)."""
+    import torch
+    code, ld = _matrix("linear_fp8", "x", x)
+    if out is None and out_dtype is None:
+        out_dtype = x.dtype
+    with _on(x) as stream:
+        out, rest = _fp8_call("linear_fp8", x, x.shape[1], w, bias, act, out, out_dtype)
+        M, N, K = x.shape[0], w.rows, x.shape[1]
+        lib = load()
+        n = lib.cube_linear_fp8_workspace_bytes(M, N, K)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+        args = Fp8Args(x.data_ptr(), code, ld, None, 0, M, *rest)
+        check(lib.cube_linear_fp8(ctypes.byref(args), ptr(ws), n, stream), "cube_linear_fp8")
+    return out
+
+
+def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token a row (cube_sample_rows): logits [M, V] f32 / bf16 / f16, u float64 [M] in [0, 1) -> (token int32 [M], prob
+    f32 [M]).  Each setting is a number or a tensor of M (top_k int32, the others float32).  temperature 0: the arg-max;
+    top_k 0, top_p 1, min_p 0: no such filter.  A row of -inf (or NaN) gives token -1, prob 0."""
+    import torch
+    code, ld = _matrix("sample_rows", "logits", logits)
+    _no_grad("sample_rows", logits)
+    M, V = logits.shape
+    dev = logits.device
+    ptrs, scalars = [], []
+    for name, x, dtype, low in (("temperature", temperature, torch.float32, 0.0), ("top_k", top_k, torch.int32, 0),
+                                ("top_p", top_p, torch.float32, 0.0), ("min_p", min_p, torch.float32, 0.0)):
+        if isinstance(x, torch.Tensor):
+            ptrs.append(_vector("sample_rows", name, x, M, dtype, dev))
+            scalars.append(0)
+        else:
+            if not x >= low or (name != "top_k" and name != "temperature" and x > 1.0) or (name == "top_k" and int(x) != x):
+                raise ValueError("sample_rows: %s=%r" % (name, x))
+            ptrs.append(None)
+            scalars.append(min(int(x), 0x7fffffff) if name == "top_k" else x)
+    up = _vector("sample_rows", "u", u, M, torch.float64, dev)
+    with _on(logits) as stream:
+        token = torch.empty(M, dtype=torch.int32, device=dev)
+        prob = torch.empty(M, dtype=torch.float32, device=dev)
+        args = SampleArgs(logits.data_ptr(), code, ld, M, V, up, *ptrs, *scalars, token.data_ptr(), prob.data_ptr())
+        check(load().cube_sample_rows(ctypes.byref(args), stream), "cube_sample_rows")
+    return token, prob
