@@ -172,7 +172,8 @@ SIGNATURES = {
     "cube_gemm_fp8": (c_int, [ctypes.POINTER(Fp8Args), c_void_p]),
     "cube_linear_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "cube_linear_fp8": (c_int, [ctypes.POINTER(Fp8Args), c_void_p, c_size_t, c_void_p]),
-    "cube_sample_rows": (c_int, [ctypes.POINTER(SampleArgs), c_void_p]),
+    "cube_sample_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "cube_sample_rows": (c_int, [ctypes.POINTER(SampleArgs), c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None
@@ -505,5 +506,8 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         token = torch.empty(M, dtype=torch.int32, device=dev)
         prob = torch.empty(M, dtype=torch.float32, device=dev)
         args = SampleArgs(logits.data_ptr(), code, ld, M, V, up, *ptrs, *scalars, token.data_ptr(), prob.data_ptr())
-        check(load().cube_sample_rows(ctypes.byref(args), stream), "cube_sample_rows")
+        lib = load()
+        n = lib.cube_sample_workspace_bytes(M, V) if M and V else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        check(lib.cube_sample_rows(ctypes.byref(args), ptr(ws), n, stream), "cube_sample_rows")
     return token, prob

@@ -55,7 +55,7 @@ def logits(M, V, t, dev, seed=0, scale=2.5, pad=0, col=0):
 
 
 SIZES = [(5, 1), (9, 2), (40, 63), (40, 64), (40, 65), (70, 102), (20, 255), (20, 256), (20, 257), (20, 511), (20, 513), (8, 1000), (6, 4097), (5, 9000),
-         (3, 32003), (2, 100000)]
+         (4, 4096), (3, 32003), (2, 32768), (2, 32769), (2, 100000), (1, 250002), (300, 33000)]
 SETTINGS = [dict(), dict(T=0.7), dict(k=1), dict(k=5), dict(k=50), dict(p=0.9), dict(p=0.3, T=1.5), dict(m=0.05), dict(T=0.8, k=40, p=0.95, m=0.02),
             dict(k=1500, p=0.99), dict(T=0.0), dict(p=0.0), dict(m=1.0), dict(T=50.0, p=0.99)]
 
@@ -81,7 +81,7 @@ def test_every_row_its_own_settings(dev, V, t):
     check(z, u, T, k, p, m)
 
 
-@pytest.mark.parametrize("V", [3, 100, 300, 5000])
+@pytest.mark.parametrize("V", [3, 100, 300, 5000, 60000])
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 def test_masked_rows(dev, V, t):
     """-inf, NaN and the type's lowest value among the logits; rows of which nothing, one candidate, or only ties are left."""
@@ -104,7 +104,7 @@ def test_masked_rows(dev, V, t):
         assert tok[0] == -1 and tok[1] == -1 and tok[2] == V - 1 and tok[5] == 0 and tok[7] == 1
 
 
-@pytest.mark.parametrize("V", [5, 100, 400, 7000])
+@pytest.mark.parametrize("V", [5, 100, 400, 7000, 60001])
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 def test_infinite_and_huge_logits(dev, V, t):
     """+inf takes all the weight, several share it; finite logits as far apart as the type goes do not overflow."""
@@ -124,7 +124,7 @@ def test_infinite_and_huge_logits(dev, V, t):
     assert tok[0] == 2 and tok[1] == 4 and prob[1] == 0.5
 
 
-@pytest.mark.parametrize("V", [7, 200, 300, 2000, 30000])
+@pytest.mark.parametrize("V", [7, 200, 300, 2000, 30000, 60000])
 def test_ties_go_to_the_lowest_index(dev, V):
     """All logits equal (and a mix of -0 and +0): top-k keeps the first k, the running sum is the index."""
     z = torch.zeros(5, V, device=dev)
@@ -141,9 +141,10 @@ def test_ties_go_to_the_lowest_index(dev, V):
         check(few.bfloat16(), u, **s)
 
 
-def test_values_next_to_each_other(dev):
+@pytest.mark.parametrize("V", [200, 3000, 50000])
+def test_values_next_to_each_other(dev, V):
     """f32 logits that differ in the last bits only, and rows that differ from one another beyond bf16's precision."""
-    base = torch.full((4, 3000), 5.0)
+    base = torch.full((4, V), 5.0)
     base += torch.randint(0, 8, base.shape, generator=torch.Generator().manual_seed(0)) * 2.0 ** -21
     _, u = logits(4, 10, "f32", dev, seed=1)
     for s in (dict(), dict(k=100), dict(p=0.5), dict(k=700, p=0.6)):
@@ -151,7 +152,7 @@ def test_values_next_to_each_other(dev):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("V,col,pad", [(102, 3, 5), (1001, 1, 2), (5000, 7, 1), (20001, 0, 3)])
+@pytest.mark.parametrize("V,col,pad", [(102, 3, 5), (1001, 1, 2), (5000, 7, 1), (20001, 0, 3), (70001, 1, 2)])
 def test_strided_and_unaligned_rows(dev, V, col, pad, t):
     z, u = logits(7, V, t, dev, seed=2, col=col, pad=pad)
     for s in (dict(), dict(k=20, p=0.9), dict(p=0.8), dict(m=0.1)):

@@ -69,14 +69,24 @@ def test_sample_rows_refuses(bad):
     a = hip.SampleArgs(P, 0, 100, 8, 100, P, None, None, None, None, 1.0, 0, 1.0, 0.0, P, P)
     for k, v in bad.items():
         setattr(a, k, v)
-    _err(hip.load().cube_sample_rows(ctypes.byref(a), None))
+    _err(hip.load().cube_sample_rows(ctypes.byref(a), None, 0, None))
+
+
+def test_sample_rows_refuses_a_workspace_that_is_short():
+    lib = hip.load()
+    V = 1 << 20
+    a = hip.SampleArgs(P, 0, V, 8, V, P, None, None, None, None, 1.0, 0, 1.0, 0.0, P, P)
+    need = lib.cube_sample_workspace_bytes(8, V)
+    assert need > 0 and lib.cube_sample_workspace_bytes(8, 200) == 0
+    for ws, n in ((None, need), (P, need - 1), (P + 8, need)):
+        _err(lib.cube_sample_rows(ctypes.byref(a), ws, n, None))
 
 
 def test_null_structures_are_refused():
     lib = hip.load()
     _err(lib.cube_gemm_fp8(None, None))
     _err(lib.cube_linear_fp8(None, None, 0, None))
-    _err(lib.cube_sample_rows(None, None))
+    _err(lib.cube_sample_rows(None, None, 0, None))
 
 
 def test_empty_batches_do_nothing():
@@ -86,7 +96,7 @@ def test_empty_batches_do_nothing():
     assert lib.cube_linear_fp8(ctypes.byref(_fp8(a_type=0, M=0, A=None)), None, 0, None) == 0
     assert lib.cube_quant_fp8(None, 0, 200, 0, 200, None, 256, None, 0, None) == 0
     a = hip.SampleArgs(None, 0, 100, 0, 100, None, None, None, None, None, 1.0, 0, 1.0, 0.0, None, None)
-    assert lib.cube_sample_rows(ctypes.byref(a), None) == 0
+    assert lib.cube_sample_rows(ctypes.byref(a), None, 0, None) == 0
 
 
 def test_calls_on_tensors_refuse():
