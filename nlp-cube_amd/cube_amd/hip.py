@@ -315,51 +315,35 @@ def masked_mean(layers, weights, ld_x, word_len, N, W, C, out, ld_out, word_rows
 # These take whole tensors, check them, and launch on the current stream of the tensors' own device.  Workspaces come from torch's
 # caching allocator per call: stream-ordered, and inside a graph capture from the graph's own pool.
 
+# (A call on a few rows is mostly host time: the checks below are attribute reads, and outputs come from empty_strided.)
+
 FP8_BLOCK = 128  # columns that share one scale
 FP8_ACTS = {None: 0, "none": 0, "tanh": 1, "relu": 2}
-_T = None
+_T = {}          # torch dtype -> CUBE_T_*, filled when torch is there
 
 
-def _type_code(dtype):
-    global _T
-    if _T is None:
+def _types():
+    if not _T:
         import torch
-        _T = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    return _T.get(dtype)
-
-
-class _on:
-    """The tensor's device as the current one (cheap when it already is)."""
-    __slots__ = ("want", "was")
-
-    def __init__(self, t):
-        self.want = t.device.index
-
-    def __enter__(self):
-        import torch
-        self.was = torch._C._cuda_getDevice()
-        if self.was != self.want:
-            torch._C._cuda_setDevice(self.want)
-        return torch._C._cuda_getCurrentRawStream(self.want)
-
-    def __exit__(self, *a):
-        if self.was != self.want:
-            import torch
-            torch._C._cuda_setDevice(self.was)
+        _T.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    return _T
 
 
 def _matrix(who, name, t):
     """A 2-D f32 / bf16 / f16 tensor on a GPU with neighbouring columns -> (type code, row stride)."""
-    code = _type_code(t.dtype)
+    code = (_T or _types()).get(t.dtype)
     if code is None or t.dim() != 2:
         raise ValueError("%s: %s must be a 2-D float32, bfloat16 or float16 tensor, got %s %s" % (who, name, t.dtype, tuple(t.shape)))
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise CubeHipError("%s: %s is on %s; it must be on an MI355X (there is no CPU fallback)" % (who, name, t.device))
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError("%s: the columns of %s must be neighbours (stride 1), got stride %d" % (who, name, t.stride(1)))
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        raise ValueError("%s: the rows of %s overlap (row stride %d, %d columns)" % (who, name, ld, t.shape[1]))
+    rows, cols = t.shape
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError("%s: the columns of %s must be neighbours (stride 1), got stride %d" % (who, name, one))
+    if rows <= 1:
+        return code, cols
+    if ld < cols:
+        raise ValueError("%s: the rows of %s overlap (row stride %d, %d columns)" % (who, name, ld, cols))
     return code, ld
 
 
@@ -370,9 +354,9 @@ def _vector(who, name, t, n, dtype, device):
     return t.data_ptr()
 
 
-def _no_grad(who, *tensors):
+def _no_grad(who):
     import torch
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled():
         raise ValueError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
 
 
@@ -383,14 +367,14 @@ class Fp8Rows:
 
     def __init__(self, q, scale, columns):
         import torch
-        kb = -(-columns // FP8_BLOCK)
+        kb = (columns + FP8_BLOCK - 1) // FP8_BLOCK
         if columns < 1 or q.dtype != torch.uint8 or q.dim() != 2 or q.shape[1] != kb * FP8_BLOCK or not q.is_contiguous():
             raise ValueError("Fp8Rows: q must be a contiguous uint8 [rows, %d] tensor for %d columns, got %s %s"
                              % (kb * FP8_BLOCK, columns, q.dtype, tuple(q.shape)))
-        if scale.dtype != torch.int32 or tuple(scale.shape) != (-(-kb // 4), q.shape[0]) or not scale.is_contiguous() or \
+        if scale.dtype != torch.int32 or scale.shape != ((kb + 3) // 4, q.shape[0]) or not scale.is_contiguous() or \
                 scale.device != q.device:
             raise ValueError("Fp8Rows: scale must be a contiguous int32 %s tensor beside q, got %s %s on %s"
-                             % ((-(-kb // 4), q.shape[0]), scale.dtype, tuple(scale.shape), scale.device))
+                             % (((kb + 3) // 4, q.shape[0]), scale.dtype, tuple(scale.shape), scale.device))
         self.q, self.scale, self.columns = q, scale, columns
 
     @property
@@ -413,53 +397,69 @@ def quant_fp8(x):
     """x [M, K] (f32, bf16, f16) -> Fp8Rows (cube_quant_fp8)."""
     import torch
     code, ld = _matrix("quant_fp8", "x", x)
-    _no_grad("quant_fp8", x)
+    if x.requires_grad:
+        _no_grad("quant_fp8")
+    d = x.get_device()
+    if d != torch._C._cuda_getDevice():
+        with torch.cuda.device(d):
+            return quant_fp8(x)
     M, K = x.shape
-    kb = -(-K // FP8_BLOCK)
-    with _on(x) as stream:
-        q = torch.empty((M, kb * FP8_BLOCK), dtype=torch.uint8, device=x.device)
-        scale = torch.empty((-(-kb // 4), M), dtype=torch.int32, device=x.device)
-        check(load().cube_quant_fp8(x.data_ptr(), code, ld, M, K, q.data_ptr(), kb * FP8_BLOCK, scale.data_ptr(), M, stream), "cube_quant_fp8")
-    return Fp8Rows(q, scale, K)
+    kb = (K + FP8_BLOCK - 1) // FP8_BLOCK
+    r = object.__new__(Fp8Rows)
+    r.columns = K
+    r.q = torch.empty_strided((M, kb * FP8_BLOCK), (kb * FP8_BLOCK, 1), dtype=torch.uint8, device=x.device)
+    r.scale = torch.empty_strided(((kb + 3) // 4, M), (M, 1), dtype=torch.int32, device=x.device)
+    check((_lib or load()).cube_quant_fp8(x.data_ptr(), code, ld, M, K, r.q.data_ptr(), kb * FP8_BLOCK, r.scale.data_ptr(), M,
+                                          torch._C._cuda_getCurrentRawStream(d)), "cube_quant_fp8")
+    return r
 
 
-def _fp8_call(who, a, K, w, bias, act, out, out_dtype):
-    """What gemm_fp8 and linear_fp8 check alike -> (output, its Fp8Args fields behind the activations')."""
+def _fp8_output(who, M, K, device, w, bias, act, out, out_dtype):
+    """What gemm_fp8 and linear_fp8 check alike -> (output, the fields of Fp8Args from the weight on)."""
     import torch
-    device = a.device
+    q, N = w.q, w.q.shape[0]
     if w.columns != K:
         raise ValueError("%s: the weight has %d columns, the input %d" % (who, w.columns, K))
-    if w.q.device != device:
-        raise ValueError("%s: the weight is on %s, the input on %s" % (who, w.q.device, device))
+    if q.device != device:
+        raise ValueError("%s: the weight is on %s, the input on %s" % (who, q.device, device))
     if act not in FP8_ACTS:
         raise ValueError("%s: act must be None, 'none', 'tanh' or 'relu', got %r" % (who, act))
-    M, N = a.shape[0], w.rows
-    _no_grad(who, a, bias)
     if out is None:
-        if _type_code(out_dtype) is None:
+        code, ldo = (_T or _types()).get(out_dtype), N
+        if code is None:
             raise ValueError("%s: the output must be float32, bfloat16 or float16, got %s" % (who, out_dtype))
-        out = torch.empty((M, N), dtype=out_dtype, device=device)
-    elif tuple(out.shape) != (M, N) or out.device != device or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError("%s: out must be a %s tensor of type %s on %s, got %s %s on %s"
-                         % (who, (M, N), out_dtype, device, tuple(out.shape), out.dtype, out.device))
-    code, ldo = _matrix(who, "out", out)
-    return out, (w.q.data_ptr(), w.q.shape[1], w.scale.data_ptr(), w.scale.shape[1], N, K,
-                 None if bias is None else _vector(who, "bias", bias, N, torch.float32, device), FP8_ACTS[act],
-                 out.data_ptr(), code, ldo)
+        out = torch.empty_strided((M, N), (N, 1), dtype=out_dtype, device=device)
+    else:
+        if out.shape != (M, N) or out.device != device or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError("%s: out must be a %s tensor of type %s on %s, got %s %s on %s"
+                             % (who, (M, N), out_dtype, device, tuple(out.shape), out.dtype, out.device))
+        if out.requires_grad:
+            _no_grad(who)
+        code, ldo = _matrix(who, "out", out)
+    if bias is not None:
+        if bias.requires_grad:
+            _no_grad(who)
+        bias = _vector(who, "bias", bias, N, torch.float32, device)
+    return out, (q.data_ptr(), q.shape[1], w.scale.data_ptr(), N, N, K, bias, FP8_ACTS[act], out.data_ptr(), code, ldo)
 
 
 def gemm_fp8(a, w, bias=None, act=None, out=None, out_dtype=None):
     """act(a @ w.T + bias) of two Fp8Rows (cube_gemm_fp8): a [M, K], w [N, K] -> [M, N] of out_dtype (bfloat16 unless given).
     bias: f32 [N]; act: None, 'tanh', 'relu'; out: where to (rows may be strided)."""
     import torch
-    if a.q.device.type != "cuda":
-        raise CubeHipError("gemm_fp8: the rows are on %s; they must be on an MI355X (there is no CPU fallback)" % a.q.device)
+    q = a.q
+    if not q.is_cuda:
+        raise CubeHipError("gemm_fp8: the rows are on %s; they must be on an MI355X (there is no CPU fallback)" % q.device)
+    d = q.get_device()
+    if d != torch._C._cuda_getDevice():
+        with torch.cuda.device(d):
+            return gemm_fp8(a, w, bias, act, out, out_dtype)
     if out is None and out_dtype is None:
         out_dtype = torch.bfloat16
-    with _on(a.q) as stream:
-        out, rest = _fp8_call("gemm_fp8", a.q, a.columns, w, bias, act, out, out_dtype)
-        args = Fp8Args(a.q.data_ptr(), 3, a.q.shape[1], a.scale.data_ptr(), a.scale.shape[1], a.rows, *rest)
-        check(load().cube_gemm_fp8(ctypes.byref(args), stream), "cube_gemm_fp8")
+    M = q.shape[0]
+    out, rest = _fp8_output("gemm_fp8", M, a.columns, q.device, w, bias, act, out, out_dtype)
+    args = Fp8Args(q.data_ptr(), 3, q.shape[1], a.scale.data_ptr(), M, M, *rest)
+    check((_lib or load()).cube_gemm_fp8(args, torch._C._cuda_getCurrentRawStream(d)), "cube_gemm_fp8")
     return out
 
 
@@ -468,16 +468,22 @@ def linear_fp8(x, w, bias=None, act=None, out=None, out_dtype=None):
     out_dtype (x's type unless given)."""
     import torch
     code, ld = _matrix("linear_fp8", "x", x)
+    if x.requires_grad:
+        _no_grad("linear_fp8")
+    d = x.get_device()
+    if d != torch._C._cuda_getDevice():
+        with torch.cuda.device(d):
+            return linear_fp8(x, w, bias, act, out, out_dtype)
     if out is None and out_dtype is None:
         out_dtype = x.dtype
-    with _on(x) as stream:
-        out, rest = _fp8_call("linear_fp8", x, x.shape[1], w, bias, act, out, out_dtype)
-        M, N, K = x.shape[0], w.rows, x.shape[1]
-        lib = load()
-        n = lib.cube_linear_fp8_workspace_bytes(M, N, K)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-        args = Fp8Args(x.data_ptr(), code, ld, None, 0, M, *rest)
-        check(lib.cube_linear_fp8(ctypes.byref(args), ptr(ws), n, stream), "cube_linear_fp8")
+    M, K = x.shape
+    device = x.device
+    out, rest = _fp8_output("linear_fp8", M, K, device, w, bias, act, out, out_dtype)
+    lib = _lib or load()
+    n = lib.cube_linear_fp8_workspace_bytes(M, rest[4], K)
+    ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device) if n else None
+    args = Fp8Args(x.data_ptr(), code, ld, None, 0, M, *rest)
+    check(lib.cube_linear_fp8(args, ptr(ws), n, torch._C._cuda_getCurrentRawStream(d)), "cube_linear_fp8")
     return out
 
 
@@ -487,27 +493,31 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     top_k 0, top_p 1, min_p 0: no such filter.  A row of -inf (or NaN) gives token -1, prob 0."""
     import torch
     code, ld = _matrix("sample_rows", "logits", logits)
-    _no_grad("sample_rows", logits)
+    if logits.requires_grad:
+        _no_grad("sample_rows")
+    d = logits.get_device()
+    if d != torch._C._cuda_getDevice():
+        with torch.cuda.device(d):
+            return sample_rows(logits, u, temperature, top_k, top_p, min_p)
     M, V = logits.shape
     dev = logits.device
     ptrs, scalars = [], []
-    for name, x, dtype, low in (("temperature", temperature, torch.float32, 0.0), ("top_k", top_k, torch.int32, 0),
-                                ("top_p", top_p, torch.float32, 0.0), ("min_p", min_p, torch.float32, 0.0)):
+    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
         if isinstance(x, torch.Tensor):
             ptrs.append(_vector("sample_rows", name, x, M, dtype, dev))
             scalars.append(0)
         else:
-            if not x >= low or (name != "top_k" and name != "temperature" and x > 1.0) or (name == "top_k" and int(x) != x):
+            if not x >= 0 or (name in ("top_p", "min_p") and x > 1.0) or (name == "top_k" and int(x) != x):
                 raise ValueError("sample_rows: %s=%r" % (name, x))
             ptrs.append(None)
             scalars.append(min(int(x), 0x7fffffff) if name == "top_k" else x)
     up = _vector("sample_rows", "u", u, M, torch.float64, dev)
-    with _on(logits) as stream:
-        token = torch.empty(M, dtype=torch.int32, device=dev)
-        prob = torch.empty(M, dtype=torch.float32, device=dev)
-        args = SampleArgs(logits.data_ptr(), code, ld, M, V, up, *ptrs, *scalars, token.data_ptr(), prob.data_ptr())
-        lib = load()
-        n = lib.cube_sample_workspace_bytes(M, V) if M and V else 0
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        check(lib.cube_sample_rows(ctypes.byref(args), ptr(ws), n, stream), "cube_sample_rows")
+    token = torch.empty_strided((M,), (1,), dtype=torch.int32, device=dev)
+    prob = torch.empty_strided((M,), (1,), dtype=torch.float32, device=dev)
+    lib = _lib or load()
+    n = lib.cube_sample_workspace_bytes(M, V)
+    ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=dev) if n else None
+    args = SampleArgs(logits.data_ptr(), code, ld, M, V, up, *ptrs, *scalars, token.data_ptr(), prob.data_ptr())
+    check(lib.cube_sample_rows(args, ptr(ws), n, torch._C._cuda_getCurrentRawStream(d)), "cube_sample_rows")
     return token, prob
