@@ -452,9 +452,9 @@ typedef struct cube_sample_args {
   float temperature0; int top_k0; float top_p0; float min_p0;
   int32_t* token; float* prob;
 } cube_sample_args;
-/* ws: device memory of cube_sample_workspace_bytes(M, V) bytes (0 for short rows), 16-byte aligned, the call's own until it has
+/* ws: device memory of cube_sample_workspace_bytes(type, M, V) bytes (0 for short rows), 16-byte aligned, the call's own until it has
  * run on the stream.                                                                                                      */
-size_t cube_sample_workspace_bytes(int M, int V);
+size_t cube_sample_workspace_bytes(int type, int M, int V);
 int cube_sample_rows(const cube_sample_args* args, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -15,9 +15,13 @@
 // atomics come in), and at 2^-41 or finer they decide as 64-bit floating point would (a 32-bit running sum over a large
 // vocabulary is off by more than the distance between two neighbouring tokens' borders).
 //
-// Three forms, by the length of a row (sizes measured at the entry point below): one wave sorts a row of up to 256 logits by
-// counting; one workgroup keeps a row of up to 32768 as keys in LDS; longer ones go through four launches in which slices of a
-// row work side by side and meet in a histogram and a list of the few logits that can still decide.
+// Forms, by the length and type of a row (sizes measured at the entry point below):
+//   short   up to 256 logits: one wave sorts the row by counting;
+//   mid     one workgroup keeps the row as keys in LDS; a histogram over equal steps of the logit, then the members of the one bin
+//           that matters are sorted;
+//   half    16-bit logits have 65536 values: a workgroup counts every value of a row (or of a slice of it) in LDS, and everything
+//           is decided from the counts, with one exponential for each value that occurs;
+//   long    f32: slices of a row meet in a histogram and in a list of the few logits that can still decide.
 #include "common.h"
 #include "../../include/cube_hip.h"
 
@@ -90,14 +94,13 @@ struct Settings {
 };
 
 struct Weigher {
-  double top, inv_t, floor_x;  // largest logit, 1 / T, ln(min-p)
-  uint32_t top_key; int S;
-  __device__ Weigher(const Settings& s, uint32_t best, int bits) : top_key(best), S(bits) {
-    top = (double)value_of(best);
+  double inv_t, floor_x;  // 1 / T, ln(min-p)
+  float top; int S;       // largest logit
+  __device__ Weigher(const Settings& s, float best, int bits) : top(best), S(bits) {
     inv_t = 1.0 / (double)s.temp;
     floor_x = s.m > 0.0f ? log(s.m < 1.0f ? (double)s.m : 1.0) : -INFINITY;
   }
-  __device__ __forceinline__ double x(uint32_t key) const { return key == top_key ? 0.0 : ((double)value_of(key) - top) * inv_t; }
+  __device__ __forceinline__ double x(float v) const { return v == top ? 0.0 : ((double)v - (double)top) * inv_t; }
   // 2^shift * exp(x), x <= 0: 2^(n + f) with |f| <= 1/2, 2^f by the series of exp(f ln 2) to the 11th power (the 12th is below
   // 2^-47 of the value).  NaN (0 * inf: an infinite temperature beside an infinite logit) counts as -1100, nothing.
   __device__ __forceinline__ double power(double x, int shift) const {
@@ -122,8 +125,9 @@ struct Weigher {
   __device__ __forceinline__ uint64_t at(double x) const {
     return (uint64_t)__double_as_longlong(power(x, S) + 4503599627370496.0) & 0xfffffffffffffull;
   }
-  __device__ __forceinline__ uint64_t operator()(uint32_t key) const { return at(x(key)); }
-  __device__ float prob(uint32_t key, uint64_t kept) const { return (float)(power(x(key), S) / (double)kept); }
+  __device__ __forceinline__ uint64_t of(float v) const { return at(x(v)); }
+  __device__ __forceinline__ uint64_t operator()(uint32_t key) const { return of(value_of(key)); }
+  __device__ __forceinline__ float prob(float v, uint64_t kept) const { return (float)(power(x(v), S) / (double)kept); }
 };
 
 // ---- wave and workgroup helpers -------------------------------------------------------------------------------------------
@@ -282,7 +286,7 @@ template <int WG, class E> __device__ Choice decide(Scratch& s, E each, const Se
   uint64_t heavy = 0;  // weight of those that min-p keeps
   each([&](uint32_t k) {
     if (k >= least) {
-      const double x = w.x(k);
+      const double x = w.x(value_of(k));
       const uint64_t v = w.at(x);
       if (v) atomicAdd((unsigned long long*)&s.high[k >> (32 - D1)], (unsigned long long)v);
       if (x >= w.floor_x) heavy += v;
@@ -308,6 +312,49 @@ template <int WG, class E> __device__ Choice decide(Scratch& s, E each, const Se
   const Found f = find_bin<WG, 1 << D1>(s, r, 0, t, first);
   const Place at = refine<WG, D1, false>(s, each, w, f.bin, f.before, t);
   return {at.key, at.tie, kept};
+}
+
+// One wave, candidates in order: lane l has the places l*E .. l*E + E - 1 (key 0 behind the last).  All that a row needs beyond its
+// first V is there, or st.k bounds it.  -> the chosen place
+template <int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Settings& st, const Weigher& w, int V, float& prob) {
+  const int lane = threadIdx.x & 63;
+  const bool limited = st.limited(V);
+  uint64_t wt[E], run[E], sum = 0;
+  double x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    x[e] = w.x(value_of(q[e]));
+    wt[e] = q[e] && !(limited && lane * E + e >= st.k) ? w.at(x[e]) : 0;
+    sum += wt[e];
+    run[e] = sum;
+  }
+  const uint64_t incl = wave_scan(sum), before = incl - sum;
+  const uint64_t total = shfl64(incl, 63);
+  uint64_t kept = total;
+  const uint64_t goal = st.goal(total);
+  if (st.p < 1.0f || st.m > 0.0f) {
+    uint64_t mine = 0;  // running sum at the last place of this lane that stays
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t c = before + run[e];
+      const bool stays = wt[e] && (!(st.p < 1.0f) || c - wt[e] <= goal) && (!(st.m > 0.0f) || x[e] >= w.floor_x);
+      mine = stays ? c : mine;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { const uint64_t t = shfl64(mine, lane ^ o); mine = t > mine ? t : mine; }
+    kept = mine;
+  }
+  const uint64_t t = st.draw(kept);
+  int at = 0;
+  float pr = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint64_t c = before + run[e];
+    if (c - wt[e] <= t && t < c) { at = lane * E + e; pr = w.prob(value_of(q[e]), kept); }
+  }
+  const int owner = __ffsll(__ballot(before <= t && t < incl)) - 1;
+  prob = __shfl(pr, owner, 64);
+  return __shfl(at, owner, 64);
 }
 
 // ---- up to 256 logits: one wave a row ---------------------------------------------------------------------------------------
@@ -383,50 +430,96 @@ __global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, i
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 
-  const Weigher w(st, best, S);
-  const bool limited = st.limited(V);
   uint32_t q[E];
-  uint64_t wt[E], run[E], sum = 0;
-  double x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) q[e] = s_sorted[wave][lane * E + e];
+  const Weigher w(st, value_of(best), S);
+  float prob;
+  const int at = choose_sorted<E>(q, st, w, V, prob);
+  if (lane == 0) { a.token[r] = (int)s_order[wave][at]; if (a.prob) a.prob[r] = prob; }
+}
+
+// ---- lists of a few candidates ----------------------------------------------------------------------------------------------
+// Entries are key << 32 | ~index: larger is earlier in the order.
+constexpr int FEW = 256;
+struct alignas(16) Few {  // in LDS
+  uint64_t entry[FEW], sorted[FEW];
+  uint32_t place[FEW];
+  uint32_t n;
+  uint32_t key, index;
+  float prob;
+  uint64_t end;
+};
+static_assert(sizeof(Few) % 16 == 0, "keys behind it are read 16 bytes at a time");
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
+__device__ __forceinline__ void append(Few& f, uint64_t entry) {
+  const uint32_t at = atomicAdd(&f.n, 1u);
+  if (at < FEW) f.entry[at] = entry;
+}
+// sorts f.entry[0 .. n), n <= FEW, into f.sorted (0 behind): an entry's place is the number of larger ones; the workgroup's
+// threads share the counting
+template <int WG> __device__ void sort_few(Few& f) {
+  const int n = (int)f.n;
+  for (int i = threadIdx.x; i < FEW; i += WG) { f.sorted[i] = 0; f.place[i] = 0; }
+  __syncthreads();
+  constexpr int PARTS = WG / FEW;
+  const int e = threadIdx.x % FEW, part = threadIdx.x / FEW;
+  if (e < n) {
+    const uint64_t mine = f.entry[e];
+    uint32_t before = 0;
+    for (int i = part; i < n; i += PARTS) before += f.entry[i] > mine ? 1 : 0;
+    atomicAdd(&f.place[e], before);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < n) f.sorted[f.place[threadIdx.x]] = f.entry[threadIdx.x];
+  __syncthreads();
+}
+// One wave: in the sorted entries, with `before` in front of them, the first place whose running weight exceeds target (there is
+// one) -> f.key, f.index, f.end (the running weight up to and with it)
+__device__ void place_few(Few& f, const Weigher& w, uint64_t before, uint64_t target) {
+  constexpr int E = FEW / 64;
+  const int lane = threadIdx.x & 63;
+  uint64_t q[E], wt[E], sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int pos = lane * E + e;
-    q[e] = s_sorted[wave][pos];
-    x[e] = w.x(q[e]);
-    wt[e] = q[e] && !(limited && pos >= st.k) ? w.at(x[e]) : 0;
+    q[e] = f.sorted[lane * E + e];
+    wt[e] = q[e] ? w((uint32_t)(q[e] >> 32)) : 0;
     sum += wt[e];
-    run[e] = sum;
   }
-  const uint64_t incl = wave_scan(sum), before = incl - sum;
-  const uint64_t total = shfl64(incl, 63);
-  uint64_t kept = total;
-  const uint64_t goal = st.goal(total);
-  if (st.p < 1.0f || st.m > 0.0f) {
-    uint64_t mine = 0;  // running sum at the last place of this lane that stays
+  uint64_t c = before + wave_scan(sum) - sum;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint64_t c = before + run[e];
-      const bool stays = wt[e] && (!(st.p < 1.0f) || c - wt[e] <= goal) && (!(st.m > 0.0f) || x[e] >= w.floor_x);
-      mine = stays ? c : mine;
+  for (int e = 0; e < E; ++e) {
+    if (c <= target && target < c + wt[e]) {
+      f.key = (uint32_t)(q[e] >> 32);
+      f.index = ~(uint32_t)q[e];
+      f.end = c + wt[e];
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const uint64_t t = shfl64(mine, lane ^ o); mine = t > mine ? t : mine; }
-    kept = mine;
-  }
-  const uint64_t t = st.draw(kept);
-  if (before <= t && t < incl) {  // one lane
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint64_t c = before + run[e];
-      if (c - wt[e] <= t && t < c) {
-        a.token[r] = (int)s_order[wave][lane * E + e];
-        if (a.prob) a.prob[r] = w.prob(q[e], kept);
-      }
-    }
+    c += wt[e];
   }
 }
 
-// ---- up to 32768 logits: one workgroup a row, keys in LDS -------------------------------------------------------------------
+// Equal steps of the logit below the largest one, 32 wide in all (32 T for temperatures above 1): in the region that matters a bin
+// then holds few logits whatever their scale.  Falls monotonically with the key, so bins are in the candidates' order.
+struct Steps {
+  float top, scale, last;
+  __device__ Steps(float best, float temp, int bins) : top(best), last((float)(bins - 1)) { scale = (float)(bins / 32) / (temp > 1.0f ? temp : 1.0f); }
+  __device__ __forceinline__ int operator()(uint32_t key) const {
+    const float v = value_of(key);
+    return v == top ? 0 : (int)fminf((top - v) * scale, last);  // (inf and NaN: the last bin)
+  }
+};
+
+// Bins from the first one up, a run of neighbours per thread.
+template <int WG, int BINS, class G> __device__ Runs scan_up(Scratch& s, G get) {
+  return scan_bins<WG, BINS>(s, [&](int b) { return get(BINS - 1 - b); });
+}
+template <int WG, int BINS, class G> __device__ Found find_up(Scratch& s, const Runs& r, uint64_t target, G get) {
+  Found f = find_bin<WG, BINS>(s, r, 0, target, [&](int b) { return get(BINS - 1 - b); });
+  f.bin = BINS - 1 - f.bin;
+  return f;
+}
+
+// ---- mid: one workgroup a row, keys in LDS ----------------------------------------------------------------------------------
 constexpr int MID_V = 32768;
 
 // every thread four neighbouring keys at a time; n4: a multiple of four
@@ -438,13 +531,104 @@ template <int WG> struct LdsKeys {
       f(k.x); f(k.y); f(k.z); f(k.w);
     }
   }
+  template <class F> __device__ __forceinline__ void with_index(F f) const {
+    for (int i = 4 * (int)threadIdx.x; i < n4; i += 4 * WG) {
+      const uint4 k = *(const uint4*)&keys[i];
+      f(k.x, i); f(k.y, i + 1); f(k.z, i + 2); f(k.w, i + 3);
+    }
+  }
 };
+
+// The row's decision through the histogram over steps; false where more than FEW logits share the bin that matters (many equal
+// ones, a very flat row, a top-k set of hundreds): nothing is decided then.
+template <int WG, int BINS, class K>
+__device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Settings& st, const Weigher& w, uint32_t best, int V) {
+  static_assert(BINS <= (1 << D1) && BINS % WG == 0, "the histogram lies in Scratch::high");
+  const Steps step(value_of(best), st.temp, BINS);
+  auto get = [&](int b) { return s.high[b]; };
+  auto clear = [&] {
+    for (int b = threadIdx.x; b < BINS; b += WG) s.high[b] = 0;
+    if (threadIdx.x == 0) f.n = 0;
+    __syncthreads();
+  };
+  if (st.limited(V)) {
+    clear();
+    keys([&](uint32_t k) { if (k) atomicAdd((unsigned long long*)&s.high[step(k)], 1ull); });
+    __syncthreads();
+    const Runs r = scan_up<WG, BINS>(s, get);
+    if ((uint64_t)st.k < r.total || r.total <= FEW) {
+      uint32_t bin = BINS - 1;
+      if ((uint64_t)st.k < r.total) {
+        const Found at = find_up<WG, BINS>(s, r, (uint64_t)st.k - 1, get);
+        if (at.before + s.high[at.bin] > FEW) return false;
+        bin = at.bin;
+      }
+      keys.with_index([&](uint32_t k, int i) { if (k && step(k) <= (int)bin) append(f, entry_of(k, (uint32_t)(i - lead))); });
+      __syncthreads();
+      sort_few<WG>(f);
+      if (threadIdx.x < 64) {
+        uint32_t q[FEW / 64];
+#pragma unroll
+        for (int e = 0; e < FEW / 64; ++e) q[e] = (uint32_t)(f.sorted[threadIdx.x * (FEW / 64) + e] >> 32);
+        float prob;
+        const int at = choose_sorted<FEW / 64>(q, st, w, V, prob);
+        if (threadIdx.x == 0) { f.index = ~(uint32_t)f.sorted[at]; f.prob = prob; }
+      }
+      __syncthreads();
+      return true;
+    }
+    // no more candidates than k: not limited
+  }
+  clear();
+  uint64_t heavy = 0;  // weight of those that min-p keeps
+  keys([&](uint32_t k) {
+    if (k) {
+      const double x = w.x(value_of(k));
+      const uint64_t v = w.at(x);
+      if (v) atomicAdd((unsigned long long*)&s.high[step(k)], (unsigned long long)v);
+      if (x >= w.floor_x) heavy += v;
+    }
+  });
+  __syncthreads();
+  const Runs r = scan_up<WG, BINS>(s, get);
+  // the place in which the running weight passes a target: the members of its bin, sorted
+  auto place = [&](uint64_t target) {
+    const Found at = find_up<WG, BINS>(s, r, target, get);
+    keys.with_index([&](uint32_t k, int i) { if (k && step(k) == (int)at.bin) append(f, entry_of(k, (uint32_t)(i - lead))); });
+    __syncthreads();
+    if (f.n > FEW) return false;
+    sort_few<WG>(f);
+    if (threadIdx.x < 64) place_few(f, w, at.before, target);
+    __syncthreads();
+    return true;
+  };
+  uint64_t kept = r.total;
+  if (st.p < 1.0f) {
+    const uint64_t t = st.goal(r.total);
+    if (t < r.total) {
+      if (!place(t)) return false;
+      kept = f.end;
+      __syncthreads();
+      if (threadIdx.x == 0) f.n = 0;
+      __syncthreads();
+    }
+  }
+  if (st.m > 0.0f) {
+    heavy = block_sum<WG>(s, heavy);
+    kept = heavy < kept ? heavy : kept;
+  }
+  if (!place(st.draw(kept))) return false;
+  if (threadIdx.x == 0) f.prob = w.prob(value_of(f.key), kept);
+  __syncthreads();
+  return true;
+}
 
 template <class T, int WG>
 __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int S) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Scratch& s = *(Scratch*)smem;
-  uint32_t* keys = (uint32_t*)(smem + sizeof(Scratch));
+  Few& few = *(Few*)(smem + sizeof(Scratch));
+  uint32_t* keys = (uint32_t*)(smem + sizeof(Scratch) + sizeof(Few));
   constexpr int N = Granule<T>::N;
   const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
@@ -468,9 +652,14 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
   Choice c = {best, 0, 0};
   float prob = 1.0f;
   if (!st.greedy()) {
-    const Weigher w(st, best, S);
+    const Weigher w(st, value_of(best), S);
+    if (decide_few<WG, WG == 256 ? 1024 : 2048>(s, few, each, row.lead, st, w, best, a.V)) {
+      if (threadIdx.x == 0) { a.token[r] = (int)few.index; if (a.prob) a.prob[r] = few.prob; }
+      return;
+    }
+    __syncthreads();
     c = decide<WG>(s, each, st, w, a.V);
-    prob = w.prob(c.key, c.kept);
+    prob = w.prob(value_of(c.key), c.kept);
   }
   // the c.tie-th key equal to c.key in order of index: each wave counts its span (256 keys a step), the owner walks its own
   const int steps = (n4 + 255) / 256, per = (steps + WG / 64 - 1) / (WG / 64);
@@ -506,12 +695,441 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
   }
 }
 
-// ---- longer rows: slices side by side ---------------------------------------------------------------------------------------
-// 1 largest key of every slice, and the row's histogram cleared;  2 histogram of the first 12 bits over the row: counts for a
-// top-k row, weights for another;  3 the bins in which the targets can fall are known: their logits into the row's list;
-// 4 one workgroup decides from the list and the histogram.  A list that runs over (very many equal logits) sends the fourth
-// launch over the whole row instead.
-constexpr int DL = 12, LONG_BINS = 1 << DL;
+// ---- half: 16-bit logits by the counts of their values ----------------------------------------------------------------------
+// A slice's counts: one 32-bit word per magnitude (the 15 bits without the sign), the number of its logits in the low half and
+// of its negative ones in the high half; a slice has at most 65528 logits, so neither runs over.  Groups of 128 magnitudes (an
+// octave of bf16).  In the candidates' order group g comes 255 - g-th for positive values, falling inside, and 256 + g-th for
+// negative ones, rising.
+constexpr int HWG = 1024;
+constexpr int MAGS = 32768, GROUP = 128, GROUPS = MAGS / GROUP;
+constexpr int HALF_GRANULES = 8191;  // of 8 logits, per slice
+
+struct HalfSlice {  // of the workspace: the counts of the groups that `has` marks
+  uint32_t count[MAGS];
+  uint64_t has[GROUPS / 64];
+};
+
+template <class T> struct Half;
+template <> struct Half<bf16_t> { static constexpr uint32_t INF = 0x7f80; };
+template <> struct Half<_Float16> { static constexpr uint32_t INF = 0x7c00; };
+template <class T> __device__ __forceinline__ float half_value(uint32_t raw) { return as_float(__builtin_bit_cast(T, (uint16_t)raw)); }
+
+// the raw 16-byte granules of a row; f(word) for the two logits of each 32-bit word, whole granules only, and g(raw) for the rest
+template <class T, class F, class G> __device__ __forceinline__ void half_words(const Row<T>& row, int lo, int hi, F f, G g) {
+  const uint16_t* at = (const uint16_t*)row.at;
+#pragma unroll 4
+  for (int j = lo + (int)threadIdx.x; j < hi; j += HWG) {
+    const int i0 = j * 8 - row.lead;
+    if (i0 >= 0 && i0 + 8 <= row.V) {
+      const uint4 v = *(const uint4*)(at + i0);
+      f(v.x); f(v.y); f(v.z); f(v.w);
+    } else {
+      for (int i = i0 < 0 ? 0 : i0; i < i0 + 8 && i < row.V; ++i) g(at[i]);
+    }
+  }
+}
+// counts of granules lo .. hi - 1 into `count` (LDS)
+template <class T> __device__ void count_half(uint32_t* count, const Row<T>& row, int lo, int hi) {
+  for (int i = threadIdx.x; i < MAGS / 4; i += HWG) ((uint4*)count)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  auto one = [&](uint32_t raw) { atomicAdd(&count[raw & 0x7fffu], 1u + ((raw & 0x8000u) << 1)); };
+  half_words(row, lo, hi, [&](uint32_t w) { one(w & 0xffffu); one(w >> 16); }, one);
+  __syncthreads();
+}
+
+template <class T>
+__global__ __launch_bounds__(HWG) void half_count_kernel(cube_sample_args a, int r0, HalfSlice* ws, int per) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t count[];
+  const int r = r0 + blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  HalfSlice& out = ws[(size_t)blockIdx.y * gridDim.x + blockIdx.x];
+  const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
+  count_half(count, row, lo, hi);
+  __shared__ uint32_t any[HWG / 64];
+  constexpr int G = GROUPS / (HWG / 64);  // a wave's groups
+  uint32_t mask = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int at = (wave * G + g) * (GROUP / 2) + lane;
+    const uint2 c = ((const uint2*)count)[at];
+    if (__ballot((c.x | c.y) != 0)) {
+      mask |= 1u << g;
+      ((uint2*)out.count)[at] = c;
+    }
+  }
+  static_assert(G == 16, "four waves' masks make one word of `has`");
+  if (lane == 0) any[wave] = mask;
+  __syncthreads();
+  if (threadIdx.x < GROUPS / 64) {
+    uint64_t h = 0;
+    for (int i = 0; i < 4; ++i) h |= (uint64_t)any[4 * threadIdx.x + i] << (16 * i);
+    out.has[threadIdx.x] = h;
+  }
+}
+
+struct HalfScratch {  // in LDS
+  uint64_t weight[2 * GROUPS];  // by order
+  uint32_t count[2 * GROUPS];
+  uint64_t has[GROUPS / 64];
+  uint64_t heavy;
+  uint32_t top;                 // magnitude of the largest candidate, with its sign; 0xffffffff: none
+  uint32_t raw, tie, ties, slice;
+  float prob;
+  uint32_t part[HWG / 64];
+};
+
+// Counts of the two neighbouring magnitudes 2 * lane, 2 * lane + 1 of a group: from LDS, or summed over the slices of the workspace
+struct LdsCounts {
+  const uint32_t* count;
+  __device__ __forceinline__ void operator()(int g, uint32_t (&all)[2], uint32_t (&neg)[2]) const {
+    const uint2 c = ((const uint2*)count)[g * (GROUP / 2) + (threadIdx.x & 63)];
+    all[0] = c.x & 0xffffu; neg[0] = c.x >> 16; all[1] = c.y & 0xffffu; neg[1] = c.y >> 16;
+  }
+};
+constexpr int HALF_SLICES = 96;  // of a row, at most: 65 cover 2^22 logits
+struct SliceCounts {
+  const HalfSlice* slice; int n;
+  const uint64_t (*has)[GROUPS / 64];  // of every slice, in LDS
+  __device__ __forceinline__ void operator()(int g, uint32_t (&all)[2], uint32_t (&neg)[2]) const {
+    const int lane = threadIdx.x & 63, at = g * (GROUP / 2) + lane;
+    all[0] = all[1] = neg[0] = neg[1] = 0;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+      uint64_t left = __ballot(i0 + lane < n && ((has[i0 + lane < n ? i0 + lane : i0][g >> 6] >> (g & 63)) & 1));
+      while (left) {  // eight slices' loads at a time
+        uint2 c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          c[u] = make_uint2(0, 0);
+          if (left) {
+            c[u] = ((const uint2*)slice[i0 + __ffsll((long long)left) - 1].count)[at];
+            left &= left - 1;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          all[0] += c[u].x & 0xffffu; neg[0] += c[u].x >> 16; all[1] += c[u].y & 0xffffu; neg[1] += c[u].y >> 16;
+        }
+      }
+    }
+  }
+};
+// the candidates among them: negative counts for NEG (below the infinity), positive ones else (up to it; zero takes both signs)
+template <class T, bool NEG> __device__ __forceinline__ void valid2(int g, const uint32_t (&all)[2], const uint32_t (&neg)[2], uint32_t (&c)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t mag = (uint32_t)(g * GROUP + 2 * (threadIdx.x & 63) + i);
+    if (NEG) c[i] = mag != 0 && mag < Half<T>::INF ? neg[i] : 0;
+    else c[i] = mag == 0 ? all[i] : mag <= Half<T>::INF ? all[i] - neg[i] : 0;
+  }
+}
+
+struct Spot { uint32_t raw, tie, ties; uint64_t before, one; __device__ uint64_t end() const { return before + (uint64_t)(tie + 1) * one; } };
+// One wave: the value at which the running count (BY_COUNT) or weight passes target; before, one: weights
+template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfScratch& s, const C& counts, const Weigher& w, uint64_t target) {
+  const int lane = threadIdx.x & 63;
+  constexpr int R = 2 * GROUPS / 64;
+  uint64_t sc = 0, sw = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) { sc += s.count[lane * R + i]; sw += s.weight[lane * R + i]; }
+  uint64_t bc = wave_scan(sc) - sc, bw = wave_scan(sw) - sw;
+  const uint64_t b = BY_COUNT ? bc : bw;
+  int owner = __ffsll(__ballot(b <= target && target < b + (BY_COUNT ? sc : sw))) - 1;
+  bc = shfl64(bc, owner);
+  bw = shfl64(bw, owner);
+  int order = owner * R;
+  for (int i = 0; i < R - 1; ++i) {  // uniform
+    const uint64_t c = s.count[order], v = s.weight[order];
+    if (target < (BY_COUNT ? bc + c : bw + v)) break;
+    bc += c;
+    bw += v;
+    ++order;
+  }
+  const bool neg_side = order >= GROUPS;
+  const int g = neg_side ? order - GROUPS : GROUPS - 1 - order;
+  uint32_t all[2], neg[2], c[2];
+  counts(g, all, neg);
+  if (neg_side) valid2<T, true>(g, all, neg, c); else valid2<T, false>(g, all, neg, c);
+  // in falling order: negative values as they lie, positive ones from the other end
+  uint64_t v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t raw = (uint32_t)(g * GROUP + 2 * lane + i) | (neg_side ? 0x8000u : 0u);
+    v[i] = c[i] ? (uint64_t)c[i] * w.of(half_value<T>(raw)) : 0;
+  }
+  sc = (uint64_t)c[0] + c[1];
+  sw = v[0] + v[1];
+  const uint64_t ic = wave_scan(sc), iw = wave_scan(sw);
+  bc += neg_side ? ic - sc : shfl64(ic, 63) - ic;
+  bw += neg_side ? iw - sw : shfl64(iw, 63) - iw;
+  Spot out = {0, 0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = neg_side ? j : 1 - j;
+    const uint32_t ci = i ? c[1] : c[0];
+    const uint64_t vi = i ? v[1] : v[0];
+    const uint64_t here = BY_COUNT ? bc : bw, mine = BY_COUNT ? ci : vi;
+    if (here <= target && target < here + mine) {
+      out.raw = (uint32_t)(g * GROUP + 2 * lane + i) | (neg_side ? 0x8000u : 0u);
+      out.one = vi / ci;
+      out.tie = (uint32_t)((target - here) / (BY_COUNT ? 1 : out.one));
+      out.ties = ci;
+      out.before = bw;
+    }
+    bc += ci;
+    bw += vi;
+  }
+  owner = __ffsll(__ballot(out.ties != 0)) - 1;
+  out.raw = __shfl((int)out.raw, owner, 64);
+  out.tie = __shfl((int)out.tie, owner, 64);
+  out.ties = __shfl((int)out.ties, owner, 64);
+  out.before = shfl64(out.before, owner);
+  out.one = shfl64(out.one, owner);
+  return out;
+}
+
+// The workgroup's decision for a row from its counts (s.has filled): s.raw, s.tie, s.ties, s.prob; false for an empty row.
+template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C& counts, const Settings& st, int V, int S) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < 2 * GROUPS; i += HWG) { s.weight[i] = 0; s.count[i] = 0; }
+  if (threadIdx.x == 0) { s.heavy = 0; s.top = 0xffffffffu; }
+  __syncthreads();
+  // the largest candidate (wave 0): in the uppermost marked group that has a positive one, else the lowest with a negative one
+  if (wave == 0) {
+    bool found = false;
+    for (int word = GROUPS / 64 - 1; word >= 0 && !found; --word) {
+      for (uint64_t left = s.has[word]; left && !found;) {
+        const int bit = 63 - __clzll((long long)left);
+        left &= ~(1ull << bit);
+        uint32_t all[2], neg[2], c[2];
+        counts(64 * word + bit, all, neg);
+        valid2<T, false>(64 * word + bit, all, neg, c);
+        const unsigned long long hit = __ballot((c[0] | c[1]) != 0);
+        found = hit != 0;
+        if (found && lane == 63 - __clzll((long long)hit)) s.top = (uint32_t)((64 * word + bit) * GROUP + 2 * lane + (c[1] ? 1 : 0));
+      }
+    }
+    for (int word = 0; word < GROUPS / 64 && !found; ++word) {
+      for (uint64_t left = s.has[word]; left && !found;) {
+        const int bit = __ffsll((long long)left) - 1;
+        left &= left - 1;
+        uint32_t all[2], neg[2], c[2];
+        counts(64 * word + bit, all, neg);
+        valid2<T, true>(64 * word + bit, all, neg, c);
+        const unsigned long long hit = __ballot((c[0] | c[1]) != 0);
+        found = hit != 0;
+        if (found && lane == __ffsll((long long)hit) - 1) s.top = (uint32_t)((64 * word + bit) * GROUP + 2 * lane + (c[0] ? 0 : 1)) | 0x8000u;
+      }
+    }
+  }
+  __syncthreads();
+  if (s.top == 0xffffffffu) return false;
+  const float top = half_value<T>(s.top);
+  const Weigher w(st, top, S);
+  const bool greedy = st.greedy();
+  for (int g = wave; g < GROUPS; g += HWG / 64) {  // a wave's groups: sums of both signs
+    if (!((s.has[g >> 6] >> (g & 63)) & 1)) continue;
+    uint32_t all[2], neg[2], c[2];
+    counts(g, all, neg);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      if (side) valid2<T, true>(g, all, neg, c); else valid2<T, false>(g, all, neg, c);
+      if (!__ballot((c[0] | c[1]) != 0)) continue;
+      uint64_t sum = 0, heavy = 0;
+      if (!greedy) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (c[i]) {
+            const double x = w.x(half_value<T>((uint32_t)(g * GROUP + 2 * lane + i) | (side ? 0x8000u : 0u)));
+            const uint64_t v = (uint64_t)c[i] * w.at(x);
+            sum += v;
+            if (x >= w.floor_x) heavy += v;
+          }
+        sum = wave_sum(sum);
+        if (st.m > 0.0f) heavy = wave_sum(heavy);
+      }
+      const uint32_t n = (uint32_t)wave_sum((uint64_t)c[0] + c[1]);
+      if (lane == 0) {
+        const int order = side ? GROUPS + g : GROUPS - 1 - g;
+        s.weight[order] = sum;
+        s.count[order] = n;
+        if (st.m > 0.0f && heavy) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
+      }
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    Spot at;
+    float prob = 1.0f;
+    if (greedy) {
+      at = spot_half<T, true>(s, counts, w, 0);
+    } else {
+      constexpr int R = 2 * GROUPS / 64;
+      uint64_t total = 0, n = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) { total += s.weight[lane * R + i]; n += s.count[lane * R + i]; }
+      total = wave_sum(total);
+      n = wave_sum(n);
+      if (st.limited(V) && (uint64_t)st.k < n) total = spot_half<T, true>(s, counts, w, (uint64_t)st.k - 1).end();
+      uint64_t kept = total;
+      if (st.p < 1.0f) {
+        const uint64_t t = st.goal(total);
+        if (t < total) {
+          const uint64_t end = spot_half<T, false>(s, counts, w, t).end();
+          kept = end < kept ? end : kept;
+        }
+      }
+      if (st.m > 0.0f) kept = s.heavy < kept ? s.heavy : kept;
+      at = spot_half<T, false>(s, counts, w, st.draw(kept));
+      prob = w.prob(half_value<T>(at.raw), kept);
+    }
+    if (lane == 0) { s.raw = at.raw; s.tie = at.tie; s.ties = at.ties; s.prob = prob; }
+  }
+  __syncthreads();
+  return true;
+}
+
+// The tie-th logit of value `raw` (0: of either sign) among granules lo .. hi - 1, in order of index; one of `ties` there.
+template <class T> __device__ void find_half(HalfScratch& s, const Row<T>& row, int lo, int hi, uint32_t raw, uint32_t tie, uint32_t ties, int32_t* token) {
+  const uint16_t* at = (const uint16_t*)row.at;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t mask = raw == 0 ? 0x7fffu : 0xffffu;
+  auto matches = [&](int j) {  // bit i: logit i of granule j
+    uint32_t m = 0;
+    if (j >= hi) return m;
+    const int i0 = j * 8 - row.lead;
+    if (i0 >= 0 && i0 + 8 <= row.V) {
+      const uint4 v = *(const uint4*)(at + i0);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m |= (w[i] & mask) == raw ? 1u << (2 * i) : 0;
+        m |= ((w[i] >> 16) & mask) == raw ? 2u << (2 * i) : 0;
+      }
+    } else {
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i >= 0 && i0 + i < row.V && (at[i0 + i] & mask) == raw) m |= 1u << i;
+    }
+    return m;
+  };
+  if (ties == 1) {  // the only one: no order to keep
+#pragma unroll 4
+    for (int j = lo + (int)threadIdx.x; j < hi; j += HWG) {
+      const uint32_t m = matches(j);
+      if (m) *token = j * 8 - row.lead + __ffs(m) - 1;
+    }
+    return;
+  }
+  const int span = ((hi - lo + HWG / 64 - 1) / (HWG / 64) + 63) / 64 * 64;  // a wave's granules
+  const int w0 = lo + wave * span, w1 = w0 + span < hi ? w0 + span : hi;
+  uint32_t mine = 0;
+#pragma unroll 4
+  for (int j = w0; j < w1; j += 64) mine += __popc(matches(j + lane));
+  mine = (uint32_t)wave_sum(mine);
+  if (lane == 0) s.part[wave] = mine;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int i = 0; i < wave; ++i) before += s.part[i];
+  if (tie < before || tie >= before + mine) return;
+  for (int j = w0; j < w1; j += 64) {
+    uint32_t m = matches(j + lane);
+    const uint32_t n = __popc(m), incl = (uint32_t)wave_scan(n), all = (uint32_t)shfl64(incl, 63);
+    if (tie < before + all) {
+      const uint32_t first = before + incl - n;
+      if (tie >= first && tie < first + n) {
+        for (uint32_t i = first; i < tie; ++i) m &= m - 1;
+        *token = (j + lane) * 8 - row.lead + __ffs(m) - 1;
+      }
+      return;
+    }
+    before += all;
+  }
+}
+
+// the counts of a row's slices -> its token
+template <class T>
+__global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, int r0, const HalfSlice* ws, int slices, int per, int S) {
+  __shared__ HalfScratch s;
+  const int r = r0 + blockIdx.x, lane = threadIdx.x & 63;
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  const Settings st(a, r);
+  __shared__ uint64_t has[HALF_SLICES][GROUPS / 64];
+  const SliceCounts counts = {ws + (size_t)blockIdx.x * slices, slices, has};
+  if ((int)threadIdx.x < slices * (GROUPS / 64)) has[threadIdx.x / (GROUPS / 64)][threadIdx.x % (GROUPS / 64)] =
+      counts.slice[threadIdx.x / (GROUPS / 64)].has[threadIdx.x % (GROUPS / 64)];
+  __syncthreads();
+  if (threadIdx.x < GROUPS / 64) {
+    uint64_t h = 0;
+    for (int i = 0; i < slices; ++i) h |= has[i][threadIdx.x];
+    s.has[threadIdx.x] = h;
+  }
+  if (!decide_half<T>(s, counts, st, a.V, S)) {
+    if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
+    return;
+  }
+  if (threadIdx.x < 64) {  // which slice has the tie-th of them
+    const uint32_t mag = s.raw & 0x7fffu, g = mag / GROUP;
+    uint32_t before = 0;
+    for (int i0 = 0; i0 < slices; i0 += 64) {
+      const int i = i0 + lane;
+      uint32_t n = 0;
+      if (i < slices && ((has[i][g >> 6] >> (g & 63)) & 1)) {
+        const uint32_t c = counts.slice[i].count[mag];
+        n = mag == 0 ? c & 0xffffu : s.raw & 0x8000u ? c >> 16 : (c & 0xffffu) - (c >> 16);
+      }
+      const uint32_t incl = (uint32_t)wave_scan(n), all = (uint32_t)shfl64(incl, 63);
+      const uint32_t first = before + incl - n;
+      const bool here = s.tie >= first && s.tie < first + n;
+      if (__ballot(here)) {
+        const uint32_t tie = s.tie;
+        if (here) { s.slice = i; s.tie = tie - first; s.ties = n; }
+        break;
+      }
+      before += all;
+    }
+  }
+  __syncthreads();
+  const int lo = (int)s.slice * per, hi = lo + per < row.granules ? lo + per : row.granules;
+  if (threadIdx.x == 0 && a.prob) a.prob[r] = s.prob;
+  find_half(s, row, lo, hi, s.raw, s.tie, s.ties, &a.token[r]);
+}
+
+// a row of one slice in one launch: the counts stay in LDS
+template <class T>
+__global__ __launch_bounds__(HWG) void half_row_kernel(cube_sample_args a, int S) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t count[];
+  HalfScratch& s = *(HalfScratch*)(count + MAGS);
+  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  const Settings st(a, r);
+  count_half(count, row, 0, row.granules);
+  constexpr int G = GROUPS / (HWG / 64);
+  uint32_t mask = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const uint2 c = ((const uint2*)count)[(wave * G + g) * (GROUP / 2) + lane];
+    if (__ballot((c.x | c.y) != 0)) mask |= 1u << g;
+  }
+  if (lane == 0) s.part[wave] = mask;
+  __syncthreads();
+  if (threadIdx.x < GROUPS / 64) {
+    uint64_t h = 0;
+    for (int i = 0; i < 4; ++i) h |= (uint64_t)s.part[4 * threadIdx.x + i] << (16 * i);
+    s.has[threadIdx.x] = h;
+  }
+  if (!decide_half<T>(s, LdsCounts{count}, st, a.V, S)) {
+    if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
+    return;
+  }
+  if (threadIdx.x == 0 && a.prob) a.prob[r] = s.prob;
+  find_half(s, row, 0, row.granules, s.raw, s.tie, s.ties, &a.token[r]);
+}
+
+// ---- long: f32 rows in slices side by side -----------------------------------------------------------------------------------
+// 1 largest key of every slice, and the row's histogram cleared;  2 histogram over steps of the logit: counts for a top-k row,
+// weights for another;  3 the bins in which the targets can fall are known: their logits into the row's list;  4 one workgroup
+// decides from the list and the histogram.  A list that runs over (very many equal logits) sends the fourth launch over the
+// whole row instead.
+constexpr int LONG_BINS = 4096;
 constexpr int LIST = 16384;
 constexpr int LWG = 1024;
 constexpr int ROWS_AT_ONCE = 256;  // rows of one pass of the four launches: bounds the workspace
@@ -519,7 +1137,7 @@ constexpr int MAX_SLICES = 256;
 
 struct LongRow {  // of the workspace
   uint64_t hist[LONG_BINS];
-  uint64_t list[LIST];  // key << 32 | index
+  uint64_t list[LIST];  // entries
   uint64_t heavy;       // weight of those that min-p keeps
   uint32_t top[MAX_SLICES];
   uint32_t listed;
@@ -529,23 +1147,21 @@ __device__ __forceinline__ uint32_t row_top(const LongRow& l, int slices, Scratc
   return block_max<LWG>(s, (int)threadIdx.x < slices ? l.top[threadIdx.x] : 0u);
 }
 
-template <class T>
 __global__ __launch_bounds__(LWG) void long_top_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
   __shared__ uint32_t part[LWG / 64];
-  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y, slices = gridDim.x;
   LongRow& l = rows[blockIdx.y];
   for (int b = blockIdx.x * LWG + threadIdx.x; b < LONG_BINS; b += slices * LWG) l.hist[b] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) { l.heavy = 0; l.listed = 0; }
-  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   uint32_t best = 0;
 #pragma unroll 4
   for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-    uint32_t k[N];
+    uint32_t k[4];
     row.keys(j, k);
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = k[i] > best ? k[i] : best;
+    for (int i = 0; i < 4; ++i) best = k[i] > best ? k[i] : best;
   }
   best = wave_max(best);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = best;
@@ -556,11 +1172,9 @@ __global__ __launch_bounds__(LWG) void long_top_kernel(cube_sample_args a, int r
   }
 }
 
-template <class T>
 __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int r0, LongRow* rows, int per, int S) {
   __shared__ uint64_t hist[LONG_BINS];
   __shared__ Scratch s;
-  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y;
   LongRow& l = rows[blockIdx.y];
   const Settings st(a, r);
@@ -568,27 +1182,30 @@ __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int 
   if (best == 0 || st.greedy()) return;
   for (int b = threadIdx.x; b < LONG_BINS; b += LWG) hist[b] = 0;
   __syncthreads();
-  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  const Steps step(value_of(best), st.temp, LONG_BINS);
+  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   if (st.limited(a.V)) {
+#pragma unroll 2
     for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-      uint32_t k[N];
+      uint32_t k[4];
       row.keys(j, k);
 #pragma unroll
-      for (int i = 0; i < N; ++i) if (k[i]) atomicAdd((unsigned long long*)&hist[k[i] >> (32 - DL)], 1ull);
+      for (int i = 0; i < 4; ++i) if (k[i]) atomicAdd((unsigned long long*)&hist[step(k[i])], 1ull);
     }
   } else {
-    const Weigher w(st, best, S);
+    const Weigher w(st, value_of(best), S);
     uint64_t heavy = 0;
+#pragma unroll 2
     for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-      uint32_t k[N];
+      uint32_t k[4];
       row.keys(j, k);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
+      for (int i = 0; i < 4; ++i) {
         if (k[i]) {
-          const double x = w.x(k[i]);
+          const double x = w.x(value_of(k[i]));
           const uint64_t v = w.at(x);
-          if (v) atomicAdd((unsigned long long*)&hist[k[i] >> (32 - DL)], (unsigned long long)v);
+          if (v) atomicAdd((unsigned long long*)&hist[step(k[i])], (unsigned long long)v);
           if (x >= w.floor_x) heavy += v;
         }
       }
@@ -614,7 +1231,7 @@ template <class G> __device__ Open open_bins(Scratch& s, const Runs& r, const Se
     o.goal = st.goal(r.total);
     if (o.goal < r.total) {
       o.ends = true;
-      o.end = find_bin<LWG, LONG_BINS>(s, r, 0, o.goal, get);
+      o.end = find_up<LWG, LONG_BINS>(s, r, o.goal, get);
       o.least = o.goal + 1;  // the set's sum is at least the goal and at most the end of the bin
       o.most = o.end.before + get(o.end.bin);
     }
@@ -624,51 +1241,45 @@ template <class G> __device__ Open open_bins(Scratch& s, const Runs& r, const Se
     o.least = heavy < o.least ? heavy : o.least;
     o.most = heavy < o.most ? heavy : o.most;
   }
-  o.from = find_bin<LWG, LONG_BINS>(s, r, 0, st.draw(o.least), get).bin;
-  o.to = o.least == o.most ? o.from : find_bin<LWG, LONG_BINS>(s, r, 0, st.draw(o.most), get).bin;
+  o.from = find_up<LWG, LONG_BINS>(s, r, st.draw(o.least), get).bin;
+  o.to = o.least == o.most ? o.from : find_up<LWG, LONG_BINS>(s, r, st.draw(o.most), get).bin;
   return o;
 }
 
-template <class T>
 __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
   __shared__ Scratch s;
-  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y, lane = threadIdx.x & 63;
   LongRow& l = rows[blockIdx.y];
   const Settings st(a, r);
   const uint32_t best = row_top(l, gridDim.x, s);
   if (best == 0) return;
-  // keys in [a0, a1] or [b0, b1] are listed
-  uint32_t a0 = best, a1 = best, b0 = 1, b1 = 0;
+  const Steps step(value_of(best), st.greedy() ? 1.0f : st.temp, LONG_BINS);
+  // candidates in the bins from .. to and in the bin `end` are listed; of a greedy row those equal to the largest
+  int from = 0, to = 0, end = -1;
   if (!st.greedy()) {
     auto get = [&](int b) { return l.hist[b]; };
-    const Runs runs = scan_bins<LWG, LONG_BINS>(s, get);
-    a1 = 0xffffffffu;
+    const Runs runs = scan_up<LWG, LONG_BINS>(s, get);
     if (st.limited(a.V)) {
-      a0 = 1;
-      if ((uint64_t)st.k < runs.total) a0 = find_bin<LWG, LONG_BINS>(s, runs, 0, (uint64_t)st.k - 1, get).bin << (32 - DL);
+      to = LONG_BINS - 1;
+      if ((uint64_t)st.k < runs.total) to = (int)find_up<LWG, LONG_BINS>(s, runs, (uint64_t)st.k - 1, get).bin;
     } else {
       const Open o = open_bins(s, runs, st, l.heavy, get);
-      a0 = o.to << (32 - DL);
-      a1 = (o.from << (32 - DL)) | ((1u << (32 - DL)) - 1);
-      if (o.ends) { b0 = o.end.bin << (32 - DL); b1 = b0 | ((1u << (32 - DL)) - 1); }
+      from = (int)o.from;
+      to = (int)o.to;
+      if (o.ends) end = (int)o.end.bin;
     }
   }
-  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   for (int j0 = lo; j0 < hi; j0 += LWG) {
     const int j = j0 + threadIdx.x;
-    uint32_t k[N], n = 0;
-    bool in[N];
-    if (j < hi) {
-      row.keys(j, k);
-    } else {
+    uint32_t k[4] = {0, 0, 0, 0}, n = 0;
+    bool in[4];
+    if (j < hi) row.keys(j, k);
 #pragma unroll
-      for (int i = 0; i < N; ++i) k[i] = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      in[i] = (k[i] >= a0 && k[i] <= a1) || (k[i] >= b0 && k[i] <= b1);
+    for (int i = 0; i < 4; ++i) {
+      const int b = step(k[i]);
+      in[i] = k[i] && ((b >= from && b <= to) || b == end) && (!st.greedy() || k[i] == best);
       n += in[i];
     }
     if (__ballot(n != 0) == 0) continue;
@@ -677,39 +1288,48 @@ __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int 
     if (lane == 63) base = atomicAdd(&l.listed, incl);
     uint32_t at = (uint32_t)__shfl((int)base, 63, 64) + incl - n;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < 4; ++i)
       if (in[i]) {
-        if (at < LIST) l.list[at] = ((uint64_t)k[i] << 32) | (uint32_t)(j * N + i - row.lead);
+        if (at < LIST) l.list[at] = entry_of(k[i], (uint32_t)(j * 4 + i - row.lead));
         ++at;
       }
   }
 }
 
-// the listed logits of a row, or all of them
+// the listed logits of a row (of one bin only where `bin` is not negative), or all of a row's
 struct ListKeys {
   const uint64_t* list; int n;
   template <class F> __device__ __forceinline__ void operator()(F f) const {
     for (int i = threadIdx.x; i < n; i += LWG) f((uint32_t)(list[i] >> 32));
   }
 };
-template <class T> struct RowKeys {
-  const Row<T>& row;
+struct RowKeys {
+  const Row<float>& row;
   template <class F> __device__ __forceinline__ void operator()(F f) const {
-    constexpr int N = Granule<T>::N;
     for (int j = threadIdx.x; j < row.granules; j += LWG) {
-      uint32_t k[N];
+      uint32_t k[4];
       row.keys(j, k);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f(k[i]);
+      for (int i = 0; i < 4; ++i) f(k[i]);
     }
   }
 };
+// the key at which the running weight passes target among the keys that each() gives, `before` in front of them
+template <class E> __device__ Place search(Scratch& s, E each, const Weigher& w, uint64_t before, uint64_t target) {
+  for (int b = threadIdx.x; b < (1 << D1); b += LWG) s.high[b] = 0;
+  __syncthreads();
+  each([&](uint32_t k) { atomicAdd((unsigned long long*)&s.high[k >> (32 - D1)], (unsigned long long)w(k)); });
+  __syncthreads();
+  auto first = [&](int b) { return s.high[b]; };
+  const Found f = find_bin<LWG, 1 << D1>(s, scan_bins<LWG, 1 << D1>(s, first), before, target, first);
+  return refine<LWG, D1, false>(s, each, w, f.bin, f.before, target);
+}
 
-template <class T>
 __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, int r0, LongRow* rows, int slices, int S) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Scratch& s = *(Scratch*)smem;
-  uint64_t* list = (uint64_t*)(smem + sizeof(Scratch));
+  Few& few = *(Few*)(smem + sizeof(Scratch));
+  uint64_t* list = (uint64_t*)(smem + sizeof(Scratch) + sizeof(Few));
   const int r = r0 + blockIdx.x;
   LongRow& l = rows[blockIdx.x];
   const Settings st(a, r);
@@ -718,35 +1338,71 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
     if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
-  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const bool whole = l.listed > LIST;  // the list ran over: decide from the row itself
   const int n = whole ? 0 : (int)l.listed;
   for (int i = threadIdx.x; i < n; i += LWG) list[i] = l.list[i];
+  if (threadIdx.x == 0) few.n = 0;
   __syncthreads();
   Choice c = {best, 0, 0};
   float prob = 1.0f;
   if (!st.greedy()) {
-    const Weigher w(st, best, S);
-    const ListKeys some = {list, n};
+    const Weigher w(st, value_of(best), S);
     if (whole) {
-      c = decide<LWG>(s, RowKeys<T>{row}, st, w, a.V);
+      c = decide<LWG>(s, RowKeys{row}, st, w, a.V);
     } else if (st.limited(a.V)) {
-      c = decide<LWG>(s, some, st, w, a.V);
+      if (n <= FEW) {
+        for (int i = threadIdx.x; i < n; i += LWG) few.entry[i] = list[i];
+        if (threadIdx.x == 0) few.n = n;
+        __syncthreads();
+        sort_few<LWG>(few);
+        if (threadIdx.x < 64) {
+          uint32_t q[FEW / 64];
+#pragma unroll
+          for (int e = 0; e < FEW / 64; ++e) q[e] = (uint32_t)(few.sorted[threadIdx.x * (FEW / 64) + e] >> 32);
+          const int at = choose_sorted<FEW / 64>(q, st, w, a.V, prob);
+          if (threadIdx.x == 0) { a.token[r] = (int)~(uint32_t)few.sorted[at]; if (a.prob) a.prob[r] = prob; }
+        }
+        return;
+      }
+      c = decide<LWG>(s, ListKeys{list, n}, st, w, a.V);
     } else {
       auto get = [&](int b) { return l.hist[b]; };
-      const Runs runs = scan_bins<LWG, LONG_BINS>(s, get);
+      const Steps step(value_of(best), st.temp, LONG_BINS);
+      const Runs runs = scan_up<LWG, LONG_BINS>(s, get);
       const Open o = open_bins(s, runs, st, l.heavy, get);
+      // where the running weight passes a target, inside a bin of the list: a few members are sorted, more are searched
+      auto place = [&](const Found& at, uint64_t target, Place& out) {
+        for (int i = threadIdx.x; i < n; i += LWG) if (step((uint32_t)(list[i] >> 32)) == (int)at.bin) append(few, list[i]);
+        __syncthreads();
+        if (few.n <= FEW) {
+          sort_few<LWG>(few);
+          if (threadIdx.x < 64) place_few(few, w, at.before, target);
+          __syncthreads();
+          return true;
+        }
+        out = search(s, [&](auto f) {
+          for (int i = threadIdx.x; i < n; i += LWG) { const uint32_t k = (uint32_t)(list[i] >> 32); if (step(k) == (int)at.bin) f(k); }
+        }, w, at.before, target);
+        return false;
+      };
       uint64_t kept = o.most;
+      Place at;
       if (o.ends) {
-        const uint64_t end = refine<LWG, DL, false>(s, some, w, o.end.bin, o.end.before, o.goal).end();
+        const uint64_t end = place(o.end, o.goal, at) ? few.end : at.end();
         kept = end < kept ? end : kept;
+        __syncthreads();
+        if (threadIdx.x == 0) few.n = 0;
+        __syncthreads();
       }
       const uint64_t t = st.draw(kept);
-      const Found f = find_bin<LWG, LONG_BINS>(s, runs, 0, t, get);
-      const Place at = refine<LWG, DL, false>(s, some, w, f.bin, f.before, t);
+      if (place(find_up<LWG, LONG_BINS>(s, runs, t, get), t, at)) {
+        if (threadIdx.x == 0) { a.token[r] = (int)few.index; if (a.prob) a.prob[r] = w.prob(value_of(few.key), kept); }
+        return;
+      }
       c = {at.key, at.tie, kept};
     }
-    prob = w.prob(c.key, c.kept);
+    prob = w.prob(value_of(c.key), c.kept);
   }
   // the c.tie-th smallest index among the logits equal to c.key: two digits of 11 bits of the index, from below
   uint32_t prefix = 0, left = c.tie;
@@ -758,15 +1414,14 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
       if (shift == 11 || i >> 11 == prefix) atomicAdd((unsigned long long*)&s.high[2047 - ((i >> shift) & 2047)], 1ull);
     };
     if (whole) {
-      constexpr int N = Granule<T>::N;
       for (int j = threadIdx.x; j < row.granules; j += LWG) {
-        uint32_t k[N];
+        uint32_t k[4];
         row.keys(j, k);
 #pragma unroll
-        for (int i = 0; i < N; ++i) if (k[i] == c.key) add((uint32_t)(j * N + i - row.lead));
+        for (int i = 0; i < 4; ++i) if (k[i] == c.key) add((uint32_t)(j * 4 + i - row.lead));
       }
     } else {
-      for (int i = threadIdx.x; i < n; i += LWG) if ((uint32_t)(list[i] >> 32) == c.key) add((uint32_t)list[i]);
+      for (int i = threadIdx.x; i < n; i += LWG) if ((uint32_t)(list[i] >> 32) == c.key) add(~(uint32_t)list[i]);
     }
     __syncthreads();
     auto get = [&](int b) { return s.high[b]; };
@@ -790,18 +1445,18 @@ template <class T> int launch_short(const cube_sample_args& a, int S, hipStream_
 
 template <class T, int WG> int launch_mid(const cube_sample_args& a, int S, hipStream_t st) {
   static CubeLdsReservation lds;
-  const size_t bytes = sizeof(Scratch) + 4 * (size_t)((a.V + 2 * Granule<T>::N + 3) / 4 * 4);
+  const size_t bytes = sizeof(Scratch) + sizeof(Few) + 4 * (size_t)((a.V + 2 * Granule<T>::N + 3) / 4 * 4);
   if (!lds.ensure((const void*)sample_mid_kernel<T, WG>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
   hipLaunchKernelGGL((sample_mid_kernel<T, WG>), dim3(a.M), dim3(WG), bytes, st, a, S);
   CUBE_CHECK_LAUNCH("cube_sample_rows");
   return CUBE_OK;
 }
 
-template <class T> int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
+int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
   static CubeLdsReservation lds;
-  const size_t bytes = sizeof(Scratch) + 8 * LIST;
-  if (!lds.ensure((const void*)long_choose_kernel<T>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
-  const int granules = (a.V + 2 * Granule<T>::N - 2) / Granule<T>::N;  // of the longest row (one that starts inside a granule)
+  const size_t bytes = sizeof(Scratch) + sizeof(Few) + 8 * LIST;
+  if (!lds.ensure((const void*)long_choose_kernel, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
+  const int granules = (a.V + 2 * 4 - 2) / 4;  // of a row that starts inside a granule
   for (int r0 = 0; r0 < a.M; r0 += ROWS_AT_ONCE) {
     const int n = a.M - r0 < ROWS_AT_ONCE ? a.M - r0 : ROWS_AT_ONCE;
     // slices of one granule a thread at least, about two workgroups a CU over all rows
@@ -811,29 +1466,77 @@ template <class T> int launch_long(const cube_sample_args& a, int S, LongRow* ws
     slices = slices < MAX_SLICES ? slices : MAX_SLICES;
     const int per = (granules + slices - 1) / slices;
     const dim3 grid(slices, n);
-    hipLaunchKernelGGL((long_top_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
-    hipLaunchKernelGGL((long_hist_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per, S);
-    hipLaunchKernelGGL((long_list_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
-    hipLaunchKernelGGL((long_choose_kernel<T>), dim3(n), dim3(LWG), bytes, st, a, r0, ws, slices, S);
+    hipLaunchKernelGGL(long_top_kernel, grid, dim3(LWG), 0, st, a, r0, ws, per);
+    hipLaunchKernelGGL(long_hist_kernel, grid, dim3(LWG), 0, st, a, r0, ws, per, S);
+    hipLaunchKernelGGL(long_list_kernel, grid, dim3(LWG), 0, st, a, r0, ws, per);
+    hipLaunchKernelGGL(long_choose_kernel, dim3(n), dim3(LWG), bytes, st, a, r0, ws, slices, S);
     CUBE_CHECK_LAUNCH("cube_sample_rows");
   }
   return CUBE_OK;
 }
 
-bool is_long(int M, int V) { return V > MID_V; }
+// slices of a 16-bit row, and rows of one pass of the two launches
+constexpr int HALF_AT_ONCE = 1024;  // slices
+struct HalfPlan { int slices, per, rows; };
+HalfPlan half_plan(int M, int V) {
+  const int granules = (V + 2 * 8 - 2) / 8;
+  HalfPlan p;
+  p.slices = (granules + HALF_GRANULES - 1) / HALF_GRANULES;
+  p.rows = HALF_AT_ONCE / p.slices < M ? HALF_AT_ONCE / p.slices : M;  // V <= 2^22: at most 65 slices
+  if (p.slices > 1 || M < 64) {
+    // few rows: more and shorter slices, up to one workgroup a CU, but four granules a thread at least: the second launch adds
+    // the slices' counts (1 x 250002: 31 slices of one granule 64 us, 8 of four TODO us)
+    const int most = (granules + 4 * HWG - 1) / (4 * HWG), want = 256 / p.rows;
+    const int more = most < want ? most : want;
+    p.slices = more > p.slices ? more : p.slices;
+    p.slices = p.slices < HALF_SLICES ? p.slices : HALF_SLICES;
+  }
+  p.per = (granules + p.slices - 1) / p.slices;
+  return p;
+}
+template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* ws, hipStream_t st) {
+  constexpr size_t bytes = 4 * MAGS;
+  const HalfPlan p = half_plan(a.M, a.V);
+  if (p.slices == 1) {
+    static CubeLdsReservation lds;
+    constexpr size_t all = bytes + sizeof(HalfScratch);
+    if (!lds.ensure((const void*)half_row_kernel<T>, all)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
+    hipLaunchKernelGGL((half_row_kernel<T>), dim3(a.M), dim3(HWG), all, st, a, S);
+    CUBE_CHECK_LAUNCH("cube_sample_rows");
+    return CUBE_OK;
+  }
+  static CubeLdsReservation lds;
+  if (!lds.ensure((const void*)half_count_kernel<T>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
+  for (int r0 = 0; r0 < a.M; r0 += p.rows) {
+    const int n = a.M - r0 < p.rows ? a.M - r0 : p.rows;
+    hipLaunchKernelGGL((half_count_kernel<T>), dim3(p.slices, n), dim3(HWG), bytes, st, a, r0, ws, p.per);
+    hipLaunchKernelGGL((half_choose_kernel<T>), dim3(n), dim3(HWG), 0, st, a, r0, ws, p.slices, p.per, S);
+    CUBE_CHECK_LAUNCH("cube_sample_rows");
+  }
+  return CUBE_OK;
+}
+
+constexpr int HALF_V = 8192;  // 16-bit rows longer than this are counted by value
 
 template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStream_t st) {
   if (a.V <= SHORT_V) return launch_short<T>(a, S, st);
-  if (is_long(a.M, a.V)) return launch_long<T>(a, S, (LongRow*)ws, st);
+  if constexpr (sizeof(T) == 2) {
+    if (a.V > HALF_V) return launch_half<T>(a, S, (HalfSlice*)ws, st);
+  } else {
+    if (a.V > MID_V) return launch_long(a, S, (LongRow*)ws, st);
+  }
   // 256 threads keep several rows on a CU; above 4096 logits a row's own passes are what takes time
   return a.V <= 4096 ? launch_mid<T, 256>(a, S, st) : launch_mid<T, 1024>(a, S, st);
 }
 
 }  // namespace
 
-extern "C" size_t cube_sample_workspace_bytes(int M, int V) {
-  if (M <= 0 || V <= 0 || V > CUBE_SAMPLE_MAX_V || !is_long(M, V)) return 0;
-  return sizeof(LongRow) * (size_t)(M < ROWS_AT_ONCE ? M : ROWS_AT_ONCE);
+extern "C" size_t cube_sample_workspace_bytes(int type, int M, int V) {
+  if (M <= 0 || V <= 0 || V > CUBE_SAMPLE_MAX_V) return 0;
+  if (type == CUBE_T_F32) return V > MID_V ? sizeof(LongRow) * (size_t)(M < ROWS_AT_ONCE ? M : ROWS_AT_ONCE) : 0;
+  if (V <= HALF_V) return 0;
+  const HalfPlan p = half_plan(M, V);
+  return p.slices > 1 ? sizeof(HalfSlice) * (size_t)p.slices * p.rows : 0;
 }
 
 extern "C" int cube_sample_rows(const cube_sample_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -847,7 +1550,7 @@ extern "C" int cube_sample_rows(const cube_sample_args* a, void* ws, size_t ws_b
   if ((uintptr_t)a->logits % (a->type == CUBE_T_F32 ? 4 : 2) || ((uintptr_t)a->u & 7) ||
       (((uintptr_t)a->token | (uintptr_t)a->prob | (uintptr_t)a->temperature | (uintptr_t)a->top_k | (uintptr_t)a->top_p | (uintptr_t)a->min_p) & 3))
     CUBE_FAIL(CUBE_ERR_ALIGN, "cube_sample_rows: a pointer is not aligned to its type");
-  const size_t need = cube_sample_workspace_bytes(a->M, a->V);
+  const size_t need = cube_sample_workspace_bytes(a->type, a->M, a->V);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: workspace of %zu bytes (need %zu, 16-byte aligned)", ws_bytes, need);
   int bits = 0;

@@ -172,7 +172,7 @@ SIGNATURES = {
     "cube_gemm_fp8": (c_int, [ctypes.POINTER(Fp8Args), c_void_p]),
     "cube_linear_fp8_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "cube_linear_fp8": (c_int, [ctypes.POINTER(Fp8Args), c_void_p, c_size_t, c_void_p]),
-    "cube_sample_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "cube_sample_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "cube_sample_rows": (c_int, [ctypes.POINTER(SampleArgs), c_void_p, c_size_t, c_void_p]),
 }
 
@@ -516,7 +516,7 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     token = torch.empty_strided((M,), (1,), dtype=torch.int32, device=dev)
     prob = torch.empty_strided((M,), (1,), dtype=torch.float32, device=dev)
     lib = _lib or load()
-    n = lib.cube_sample_workspace_bytes(M, V)
+    n = lib.cube_sample_workspace_bytes(code, M, V)
     ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=dev) if n else None
     args = SampleArgs(logits.data_ptr(), code, ld, M, V, up, *ptrs, *scalars, token.data_ptr(), prob.data_ptr())
     check(lib.cube_sample_rows(args, ptr(ws), n, torch._C._cuda_getCurrentRawStream(d)), "cube_sample_rows")

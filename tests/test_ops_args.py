@@ -76,8 +76,8 @@ def test_sample_rows_refuses_a_workspace_that_is_short():
     lib = hip.load()
     V = 1 << 20
     a = hip.SampleArgs(P, 0, V, 8, V, P, None, None, None, None, 1.0, 0, 1.0, 0.0, P, P)
-    need = lib.cube_sample_workspace_bytes(8, V)
-    assert need > 0 and lib.cube_sample_workspace_bytes(8, 200) == 0
+    need = lib.cube_sample_workspace_bytes(0, 8, V)
+    assert need > 0 and lib.cube_sample_workspace_bytes(0, 8, 200) == 0
     for ws, n in ((None, need), (P, need - 1), (P + 8, need)):
         _err(lib.cube_sample_rows(ctypes.byref(a), ws, n, None))
 
