@@ -68,14 +68,13 @@ __device__ __forceinline__ uint32_t amax_bits(const float* v) {
   }
   return m;
 }
-// maximum over the 16 lanes that share a block
+// maximum over the 16 lanes that share a block: rotations within a DPP row
+template <int CTRL> __device__ __forceinline__ uint32_t max_rot(uint32_t m) {
+  const uint32_t t = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, 0xf, 0xf, false);
+  return t > m ? t : m;
+}
 __device__ __forceinline__ uint32_t max16(uint32_t m) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    const uint32_t t = (uint32_t)__shfl_xor((int)m, o, 64);
-    m = t > m ? t : m;
-  }
-  return m;
+  return max_rot<0x128>(max_rot<0x124>(max_rot<0x122>(max_rot<0x121>(m))));
 }
 // E8M0 byte of a block whose largest finite magnitude has these bits.  448 = 1.75 * 2^8: with max = f * 2^E the exponent is
 // E - 8 for f <= 1.75 and E - 7 above; what would fall under 2^-127 (magnitudes below 2^-119, zero among them) stays there
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(256) void quant_kernel(const T* __restrict__ x, lon
 struct Fp8Params {
   const uint8_t* A; const uint32_t* A_scale; long long lda; int lds_a; int M;
   const uint8_t* W; const uint32_t* W_scale; long long ldw; int lds_w; int N;
-  int K, KB; const float* bias; int act; void* out; int out_type; long long ldo; int vec_out;
+  int K, KB; const float* bias; int act; void* out; int out_type; long long ldo; int out_align;  // 16, 4 or a value's size: what every row starts on
   int m_tiles; int n_tiles;
 };
 
@@ -161,7 +160,7 @@ __device__ __forceinline__ void store4(const Fp8Params& p, int m, int n, f32x4 c
   if (m >= p.M || n >= p.N) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i) c[i] = activate(c[i], p.act);
-  const bool whole = p.vec_out && n + 4 <= p.N;
+  const bool whole = p.out_align == 16 && n + 4 <= p.N;
   const long long at = (long long)m * p.ldo + n;
   if (p.out_type == CUBE_T_F32) {
     float* o = (float*)p.out + at;
@@ -230,58 +229,72 @@ __device__ __forceinline__ void dma4(const void* g, void* l) {
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // Tiles of BM rows x BN columns, WM x WN waves; one block of 128 columns of K a step.  A stage in LDS: BM + BN rows of 128 bytes
-// whose 16-byte chunks are XOR-swizzled by row & 7 (the swizzle rides on the DMA source address; fragment reads of 8 lanes then
-// cover all banks), and the scale word of every row.  ST stages: step k computes while k + 1 .. k + ST - 1 are on their way; the
+// whose 16-byte chunks are XOR-swizzled by (row >> 1) & 7 (the swizzle rides on the DMA source address; the 16 rows of a fragment
+// read then cover all 64 banks: by row & 7 they met in pairs), and the scale word of every row.  ST stages: step k computes while k + 1 .. k + ST - 1 are on their way; the
 // wait for step k counts the later stages' loads instead of draining them.
 // Which 32 of the 128 columns a lane group holds does not matter as long as both operands agree, since a step shares its scales.
 template <int BM, int BN, int WM, int WN, int ST, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params p) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // 1-KiB DMA pieces (8 rows) a wave issues per step
-  constexpr int PS = (BM + BN) / 64 / NW;                // pieces of 64 scale words
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % (64 * NW) == 0, "every wave issues whole pieces");
+  constexpr int SP = (BM + BN) / 64, PS = (SP + NW - 1) / NW;  // pieces of 64 scale words (waves without one load the last again)
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0, "every wave issues whole pieces");
   constexpr int ROWS = (BM + BN) * BLK, STAGE = ROWS + (BM + BN) * 4;
   constexpr int LOADS = PA + PB + PS;                    // a wave's loads per stage
+  constexpr int PER = (LOADS + TM - 1) / TM;             // of them, with each row tile's products
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wid / WN, wn = wid % WN;
-  // workgroups go round-robin over the 8 XCDs: the column tiles of a row tile get consecutive slots of one XCD, whose L2 then
-  // holds that row tile's activations once
+  // Workgroups go round-robin over the 8 XCDs, each with an L2 of its own.  An XCD has every eighth row tile and takes them four at a
+  // time, column tile by column tile: the 32 workgroups it runs at once then cover 4 x 8 tiles and share 12 operand tiles (2 x 16 of
+  // a row-major order share 18: 3 % more time at 8192x4096x4096)
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-  const int mt = (slot / p.n_tiles) * 8 + xcd, nt = slot % p.n_tiles;
+  const int rows_of = (p.m_tiles + 7) / 8, group = slot / (4 * p.n_tiles), in = slot - group * 4 * p.n_tiles;
+  const int high = rows_of - 4 * group < 4 ? rows_of - 4 * group : 4;  // row tiles of the group
+  const int nt = in / high, mt = (4 * group + in - nt * high) * 8 + xcd;
   if (mt >= p.m_tiles) return;  // whole workgroup, before any barrier
   const int m0 = mt * BM, n0 = nt * BN;
 
-  const uint8_t* src[PA + PB];
-  const uint32_t* s_src[PS];
-  const int pr = lane >> 3, chunk = (lane & 7) ^ (pr & 7);
+  // a load's address: the tile's first row (uniform) and 32 bits of offset inside the tile (255 rows of at most 2^24 bytes)
+  const uint8_t* a_base = p.A + (long long)m0 * p.lda;
+  const uint8_t* b_base = p.W + (long long)n0 * p.ldw;
+  uint32_t off[PA + PB], s_off[PS];
+  const int pr = lane >> 3, chunk = (lane & 7) ^ ((4 * (wid & 1) + (pr >> 1)) & 7);  // (row >> 1) & 7: a wave's pieces are NW apart
+  static_assert(NW % 2 == 0, "so that their rows agree in bit 3");
 #pragma unroll
   for (int i = 0; i < PA; ++i) {  // rows behind the last one read the last one; their results are not stored
-    const int r = m0 + 8 * (wid + NW * i) + pr;
-    src[i] = p.A + (long long)(r < p.M ? r : p.M - 1) * p.lda + chunk * 16;
+    const int r = 8 * (wid + NW * i) + pr;
+    off[i] = (uint32_t)(r < p.M - m0 ? r : p.M - 1 - m0) * (uint32_t)p.lda + chunk * 16;
   }
 #pragma unroll
   for (int i = 0; i < PB; ++i) {
-    const int r = n0 + 8 * (wid + NW * i) + pr;
-    src[PA + i] = p.W + (long long)(r < p.N ? r : p.N - 1) * p.ldw + chunk * 16;
+    const int r = 8 * (wid + NW * i) + pr;
+    off[PA + i] = (uint32_t)(r < p.N - n0 ? r : p.N - 1 - n0) * (uint32_t)p.ldw + chunk * 16;
   }
-  long long s_step[PS];
 #pragma unroll
   for (int i = 0; i < PS; ++i) {
-    const int t = 64 * (wid + NW * i) + lane;  // row of the stage: activations, then weights (64 | BM: a piece is of one kind)
-    const bool of_a = 64 * (wid + NW * i) < BM;
-    const int r = of_a ? m0 + t : n0 + t - BM, last = (of_a ? p.M : p.N) - 1;
-    s_src[i] = (of_a ? p.A_scale : p.W_scale) + (r < last ? r : last);
-    s_step[i] = of_a ? p.lds_a : p.lds_w;
+    const int piece = wid + NW * i < SP ? wid + NW * i : SP - 1;
+    const int t = 64 * piece + lane;  // row of the stage: activations, then weights (64 | BM: a piece is of one kind)
+    const bool of_a = 64 * piece < BM;
+    const int r = of_a ? t : t - BM, last = (of_a ? p.M - m0 : p.N - n0) - 1;
+    s_off[i] = 4 * (uint32_t)(r < last ? r : last);
   }
-  auto fill = [&](int k) {
+  // load `i` of stage k: activations, weights, scale words
+  auto load = [&](int k, int i) {
     unsigned char* buf = smem + (k % ST) * STAGE;
+    if (i < PA) {
+      dma16(a_base + (size_t)k * BLK + off[i], buf + 8 * (wid + NW * i) * BLK);
+    } else if (i < PA + PB) {
+      dma16(b_base + (size_t)k * BLK + off[i], buf + (BM + 8 * (wid + NW * (i - PA))) * BLK);
+    } else {
+      const int of = wid + NW * (i - PA - PB), t = of < SP ? of : SP - 1;
+      const uint32_t* s = 64 * t < BM ? p.A_scale + (long long)(k >> 2) * p.lds_a + m0 : p.W_scale + (long long)(k >> 2) * p.lds_w + n0;
+      dma4((const uint8_t*)s + s_off[i - PA - PB], buf + ROWS + 64 * t * 4);
+    }
+  };
+  auto fill = [&](int k) {
 #pragma unroll
-    for (int i = 0; i < PA; ++i) dma16(src[i] + (size_t)k * BLK, buf + 8 * (wid + NW * i) * BLK);
-#pragma unroll
-    for (int i = 0; i < PB; ++i) dma16(src[PA + i] + (size_t)k * BLK, buf + (BM + 8 * (wid + NW * i)) * BLK);
-#pragma unroll
-    for (int i = 0; i < PS; ++i) dma4(s_src[i] + (long long)(k >> 2) * s_step[i], buf + ROWS + 64 * (wid + NW * i) * 4);
+    for (int i = 0; i < LOADS; ++i) load(k, i);
   };
   const int l15 = lane & 15, g = lane >> 4;
   f32x4 bias[TN];
@@ -297,38 +310,121 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
 #pragma unroll
   for (int k = 0; k < ST - 1; ++k)
     if (k < p.KB) fill(k);
-  const int c0 = ((2 * g) ^ (l15 & 7)) << 4, c1 = ((2 * g + 1) ^ (l15 & 7)) << 4;  // this lane's two chunks of a row
-  for (int k = 0; k < p.KB; ++k) {
+  // this lane's two chunks of a row of a fragment
+  const int o0 = l15 * BLK + ((g ^ (l15 >> 1)) << 4), o1 = l15 * BLK + (((g + 4) ^ (l15 >> 1)) << 4);
+  // One step.  MORE: with the loads of stage k + ST - 1, which go out between the products (all at once in front of them they held
+  // up the fragment reads); no branch inside, so that they stay there.
+  auto step = [&](int k, auto MORE) {
     const unsigned char* cur = smem + (k % ST) * STAGE;
-    // step k has landed once no more loads are open than the later stages'; the barrier says so for every wave's pieces, and
-    // that all waves are done with the stage that is filled next
-    if (k + ST - 2 < p.KB) wait_vm<(ST - 2) * LOADS>(); else wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (k + ST - 1 < p.KB) fill(k + ST - 1);
     const int shift = 8 * (k & 3);
-    auto frag = [&](int row) {
-      const unsigned char* b = cur + row * BLK;
-      const i32x4 lo = *(const i32x4*)(b + c0), hi = *(const i32x4*)(b + c1);
-      return Operand<EXACT>((i32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]},
-                            *(const uint32_t*)(cur + ROWS + row * 4) >> shift);
+    auto frag = [&](int tile) {  // of the stage's tiles of 16 rows
+      const i32x4 lo = *(const i32x4*)(cur + tile * 16 * BLK + o0), hi = *(const i32x4*)(cur + tile * 16 * BLK + o1);
+      return (i32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
+    auto scale = [&](int tile) { return *(const uint32_t*)(cur + ROWS + (tile * 16 + l15) * 4) >> shift; };
     Operand<EXACT> w[TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) w[j] = frag(BM + (wn * TN + j) * 16 + l15);
+    for (int j = 0; j < TN; ++j) w[j] = Operand<EXACT>(frag(BM / 16 + wn * TN + j), scale(BM / 16 + wn * TN + j));
+    uint32_t ea[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const Operand<EXACT> a = frag((wm * TM + i) * 16 + l15);
+    for (int i = 0; i < TM; ++i) ea[i] = scale(wm * TM + i);
+    i32x8 next = frag(wm * TM);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {  // a row tile's fragment is read while the one before it is multiplied
+      const Operand<EXACT> a(next, ea[i]);
+      if (i + 1 < TM) next = frag(wm * TM + i + 1);
+      if constexpr (decltype(MORE)::value) {
+#pragma unroll
+        for (int u = i * PER; u < (i + 1) * PER && u < LOADS; ++u) load(k + ST - 1, u);
+      }
+      if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);  // the compiler would put the read right in front of its use
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = mma(w[j], a, acc[i][j]);
+      if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  // step k has landed once no more loads are open than the later stages'; the barrier in the step says so for every wave's pieces, and
+  // that all waves are done with the stage that is filled next
+  int k = 0;
+  for (; k < p.KB - (ST - 1); ++k) {
+    wait_vm<(ST - 2) * LOADS>();
+    step(k, std::true_type{});
   }
+  for (; k < p.KB; ++k) {
+    wait_vm<0>();
+    step(k, std::false_type{});
+  }
+
+  // ---- results: activation and rounding in registers, then through LDS (a wave its own part), so that whole rows of the wave's
+  // columns go out 16 bytes a lane; 16-byte chunks XOR-swizzled by the row
+  if (p.act == CUBE_FP8_TANH) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = activate(acc[i][j][r], CUBE_FP8_TANH);
+  } else if (p.act == CUBE_FP8_RELU) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = activate(acc[i][j][r], CUBE_FP8_RELU);
+  }
+  constexpr int ES = EXACT ? 4 : 2, RB = 16 * TN * ES, SWZ = RB >= 128 ? 7 : RB / 16 - 1;  // bytes of a value, of a row
+  static_assert((RB & (RB - 1)) == 0 && RB >= 32, "the swizzle stays inside the row");
+  static_assert(NW * 16 * TM * RB <= ST * STAGE, "the results fit in the stages' LDS");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();  // all waves are done with the last stage
+  asm volatile("" ::: "memory");
+  unsigned char* mine = smem + wid * 16 * TM * RB;
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-      store4(p, m0 + (wm * TM + i) * 16 + l15, n0 + (wn * TN + j) * 16 + 4 * g, acc[i][j]);
+    for (int j = 0; j < TN; ++j) {
+      const f32x4 c = acc[i][j];
+      unsigned char* row = mine + (16 * i + l15) * RB;
+      const int byte = (16 * j + 4 * g) * ES;
+      unsigned char* at = row + ((((byte >> 4) ^ (l15 & SWZ)) << 4) | (byte & 15));
+      if constexpr (EXACT) {
+        *(f32x4*)at = c;
+      } else {
+        uint16_t h[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          h[r] = p.out_type == CUBE_T_BF16 ? f32_to_bf16(c[r]) : __builtin_bit_cast(uint16_t, (_Float16)c[r]);
+        *(uint2*)at = make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+      }
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int mw = m0 + wm * TM * 16, nw = n0 + wn * TN * 16;  // the wave's part of the output
+  unsigned char* out = (unsigned char*)p.out;
+  // units of U bytes, as wide as the output's rows are aligned; a unit that would pass the last column makes it single values
+  auto copy = [&](auto unit) {
+    using U = decltype(unit);
+    constexpr int UNITS = RB / (int)sizeof(U), PER_UNIT = (int)sizeof(U) / ES, WIDE = UNITS < 64 ? UNITS : 64, R = 64 / WIDE;
+#pragma unroll 4
+    for (int row0 = 0; row0 < 16 * TM; row0 += R) {
+      const int row = row0 + lane / WIDE;
+      if (mw + row < p.M) {
+#pragma unroll
+        for (int u = lane % WIDE; u < UNITS; u += WIDE) {
+          const int byte = u * (int)sizeof(U);
+          const U v = *(const U*)(mine + row * RB + ((((byte >> 4) ^ (row & SWZ)) << 4) | (byte & 15)));
+          if (nw + u * PER_UNIT < p.N) *(U*)(out + ((long long)(mw + row) * p.ldo + nw) * ES + byte) = v;
+        }
+      }
+    }
+  };
+  const int align = nw + 16 * TN <= p.N ? p.out_align : ES;
+  if (align == 16) copy(uint4{});
+  else if (align == 4 || ES == 4) copy(uint32_t{});
+  else copy(uint16_t{});
 }
 
 // Few rows: the weights are read once, straight into registers, 16 columns a workgroup, and its 8 waves share K (wave v takes the
@@ -491,11 +587,19 @@ bool fused(int M, int K) { return M <= FEW_ROWS && (long long)M * few_stride(kbl
 int launch_gemm(Fp8Params& p, hipStream_t st) {
   const bool exact = p.out_type == CUBE_T_F32;
   if (p.M <= FEW_ROWS) return launch_few<uint8_t, true>(p, st);
-  const long long big = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (!exact && big >= 256) return launch_tiles<256, 256, 2, 4, 2, false>(p, st);
-  const long long mid = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
-  if (mid >= 128) return exact ? launch_tiles<128, 128, 2, 2, 2, true>(p, st) : launch_tiles<128, 128, 2, 2, 2, false>(p, st);
-  return exact ? launch_tiles<64, 64, 2, 1, 4, true>(p, st) : launch_tiles<64, 64, 2, 1, 4, false>(p, st);
+  // The largest tile that still gives every CU work, by the number of tiles (times of one launch, 16-bit output unless said):
+  //   256x256: 8192x4096x4096 110 us (128x128: 125 us), where their last round fills 4 of 5 CUs:  5000x4000x2000, 320 of them,
+  //     63 us (54 us), 8192x3000x1024, 384, 42 us (39 us)
+  //   128x128 (two workgroups a CU): 8192x768x768 11.7 us (128x64 13.2, 64x64 15.1), 8000x520x8000 54 us (64, 67);
+  //     256 of them, one a CU, lose: 2048x2048x2048 18.3 us (128x64 15.3)
+  //   128x64: 4096x1024x1024 9.7 us (64x64 12.1), 8192x500x768 f32 14.9 us (18.4)
+  //   64x64 with four stages: 128x768x4096 10.8 us (128x64 15.0), 1001x500x300 f32 6.5 us (7.5)
+  auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+  const long long big = tiles(256, 256), rounds = (big + 255) / 256;
+  if (!exact && 5 * big >= 4 * 256 * rounds) return launch_tiles<256, 256, 2, 4, 2, false>(p, st);
+  if (tiles(128, 128) > 256) return exact ? launch_tiles<128, 128, 2, 2, 2, true>(p, st) : launch_tiles<128, 128, 2, 2, 2, false>(p, st);
+  if (tiles(64, 64) > 512) return exact ? launch_tiles<128, 64, 4, 1, 3, true>(p, st) : launch_tiles<128, 64, 4, 1, 3, false>(p, st);
+  return exact ? launch_tiles<64, 64, 2, 2, 4, true>(p, st) : launch_tiles<64, 64, 2, 2, 4, false>(p, st);
 }
 
 size_t quant_bytes(int M, int K) {
@@ -513,6 +617,7 @@ int check_args(const cube_fp8_args* a, const char* who) {
   if (a->ldw < (long long)kblocks(a->K) * BLK || a->lds_w < a->N || a->ldo < a->N)
     CUBE_FAIL(CUBE_ERR_ARG, "%s: ldw=%lld (>= %lld), lds_w=%d (>= N=%d), ldo=%lld (>= N)", who, a->ldw, (long long)kblocks(a->K) * BLK,
               a->lds_w, a->N, a->ldo);
+  if (a->ldw > MAX_K) CUBE_FAIL(CUBE_ERR_ARG, "%s: ldw=%lld is over %d", who, a->ldw, MAX_K);
   if (((uintptr_t)a->W & 15) || a->ldw % 16) CUBE_FAIL(CUBE_ERR_ALIGN, "%s: rows of W are not 16-byte aligned", who);
   if (((uintptr_t)a->W_scale | (uintptr_t)a->bias) & 3) CUBE_FAIL(CUBE_ERR_ALIGN, "%s: W_scale / bias are not 4-byte aligned", who);
   if ((uintptr_t)a->out % type_size(a->out_type)) CUBE_FAIL(CUBE_ERR_ALIGN, "%s: out is not aligned to its type", who);
@@ -525,7 +630,8 @@ Fp8Params params(const cube_fp8_args* a) {
   p.W = (const uint8_t*)a->W; p.W_scale = a->W_scale; p.ldw = a->ldw; p.lds_w = a->lds_w; p.N = a->N;
   p.K = a->K; p.KB = kblocks(a->K); p.bias = a->bias; p.act = a->act; p.out = a->out; p.out_type = a->out_type; p.ldo = a->ldo;
   const int es = type_size(a->out_type);
-  p.vec_out = (uintptr_t)a->out % (4 * es) == 0 && a->ldo % 4 == 0;
+  const uintptr_t at = (uintptr_t)a->out | (uintptr_t)(a->ldo * es);
+  p.out_align = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : es;
   return p;
 }
 
@@ -553,8 +659,8 @@ extern "C" int cube_gemm_fp8(const cube_fp8_args* a, void* stream) {
   const int rc = check_args(a, "cube_gemm_fp8");
   if (rc) return rc;
   if (a->M == 0 || a->N == 0) return CUBE_OK;
-  if (!a->A_scale || a->lda < (long long)kblocks(a->K) * BLK || a->lds_a < a->M)
-    CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: null A_scale, lda=%lld (>= %lld) or lds_a=%d (>= M=%d)", a->lda, (long long)kblocks(a->K) * BLK,
+  if (!a->A_scale || a->lda < (long long)kblocks(a->K) * BLK || a->lds_a < a->M || a->lda > MAX_K)
+    CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: null A_scale, lda=%lld (>= %lld, <= 2^24) or lds_a=%d (>= M=%d)", a->lda, (long long)kblocks(a->K) * BLK,
               a->lds_a, a->M);
   if (((uintptr_t)a->A & 15) || a->lda % 16 || ((uintptr_t)a->A_scale & 3))
     CUBE_FAIL(CUBE_ERR_ALIGN, "cube_gemm_fp8: rows of A are not 16-byte aligned, or A_scale not 4-byte aligned");

@@ -132,24 +132,37 @@ struct Weigher {
 
 // ---- wave and workgroup helpers -------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int src) {
-  return (uint64_t)(uint32_t)__shfl((int)(uint32_t)v, src, 64) | ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(v >> 32), src, 64) << 32);
+// Sums and maxima over a wave through DPP moves (whole waves only; a cross-lane LDS shuffle takes some ten times as long): shifts
+// within rows of 16 lanes, then a row's last lane to the row behind it, then lane 31 to the upper half.  What has no source is 0.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t from_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) { const uint32_t t = (uint32_t)__shfl_xor((int)v, o, 64); v = t > v ? t : v; }
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t from_lane(uint64_t v) {
+  return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)v) | ((uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32);
+}
+template <class V> __device__ __forceinline__ V wave_scan(V v) {  // inclusive
+  v += from_lane<0x111, 0xf>(v);
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v);
+  v += from_lane<0x143, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += shfl64(v, (threadIdx.x & 63) ^ o);
-  return v;
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }  // lane: uniform
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+  return (uint64_t)lane_value((uint32_t)v, lane) | ((uint64_t)lane_value((uint32_t)(v >> 32), lane) << 32);
 }
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const uint64_t t = shfl64(v, lane >= o ? lane - o : lane); v += lane >= o ? t : 0; }
-  return v;
+template <class V> __device__ __forceinline__ V wave_sum(V v) { return lane_value(wave_scan(v), 63); }
+template <class V> __device__ __forceinline__ V larger(V a, V b) { return a > b ? a : b; }
+template <class V> __device__ __forceinline__ V wave_max(V v) {
+  v = larger(v, from_lane<0x111, 0xf>(v));
+  v = larger(v, from_lane<0x112, 0xf>(v));
+  v = larger(v, from_lane<0x114, 0xf>(v));
+  v = larger(v, from_lane<0x118, 0xf>(v));
+  v = larger(v, from_lane<0x142, 0xa>(v));
+  v = larger(v, from_lane<0x143, 0xc>(v));
+  return lane_value(v, 63);
 }
 
 constexpr int D1 = 11, D2 = 10;  // bits of the first two digits of a key within a workgroup; the third has the rest
@@ -329,7 +342,7 @@ template <int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Sett
     run[e] = sum;
   }
   const uint64_t incl = wave_scan(sum), before = incl - sum;
-  const uint64_t total = shfl64(incl, 63);
+  const uint64_t total = lane_value(incl, 63);
   uint64_t kept = total;
   const uint64_t goal = st.goal(total);
   if (st.p < 1.0f || st.m > 0.0f) {
@@ -340,9 +353,7 @@ template <int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Sett
       const bool stays = wt[e] && (!(st.p < 1.0f) || c - wt[e] <= goal) && (!(st.m > 0.0f) || x[e] >= w.floor_x);
       mine = stays ? c : mine;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const uint64_t t = shfl64(mine, lane ^ o); mine = t > mine ? t : mine; }
-    kept = mine;
+    kept = wave_max(mine);
   }
   const uint64_t t = st.draw(kept);
   int at = 0;
@@ -353,8 +364,8 @@ template <int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Sett
     if (c - wt[e] <= t && t < c) { at = lane * E + e; pr = w.prob(value_of(q[e]), kept); }
   }
   const int owner = __ffsll(__ballot(before <= t && t < incl)) - 1;
-  prob = __shfl(pr, owner, 64);
-  return __shfl(at, owner, 64);
+  prob = __uint_as_float(lane_value(__float_as_uint(pr), owner));
+  return (int)lane_value((uint32_t)at, owner);
 }
 
 // ---- up to 256 logits: one wave a row ---------------------------------------------------------------------------------------
@@ -672,7 +683,7 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
   };
   uint32_t mine = 0, k[4];
   for (int i = lo; i < hi; ++i) mine += ties4(i, k);
-  mine = (uint32_t)wave_sum(mine);
+  mine = wave_sum(mine);
   if (lane == 0) s.part32[wave] = mine;
   __syncthreads();
   uint32_t before = 0;
@@ -680,7 +691,7 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
   if (c.tie < before || c.tie >= before + mine) return;
   for (int i = lo; i < hi; ++i) {
     const uint32_t n = ties4(i, k);
-    const uint32_t incl = (uint32_t)wave_scan(n), all = (uint32_t)shfl64(incl, 63);
+    const uint32_t incl = wave_scan(n), all = lane_value(incl, 63);
     if (c.tie < before + all) {
       uint32_t at = before + incl - n;
 #pragma unroll
@@ -768,37 +779,47 @@ __global__ __launch_bounds__(HWG) void half_count_kernel(cube_sample_args a, int
 }
 
 struct HalfScratch {  // in LDS
-  uint64_t weight[2 * GROUPS];  // by order
+  uint64_t weight[2 * GROUPS];  // by order; after prefix_half: running sums
   uint32_t count[2 * GROUPS];
   uint64_t has[GROUPS / 64];
   uint64_t heavy;
-  uint32_t top;                 // magnitude of the largest candidate, with its sign; 0xffffffff: none
   uint32_t raw, tie, ties, slice;
   float prob;
   uint32_t part[HWG / 64];
 };
 
-// Counts of the two neighbouring magnitudes 2 * lane, 2 * lane + 1 of a group: from LDS, or summed over the slices of the workspace
+// Counts of the two neighbouring magnitudes 2 * lane, 2 * lane + 1 of a group: all and negative.  From LDS, or summed over the slices
+// of the workspace (and kept in LDS for the groups of the first SLOTS marks: a search comes back to a group).
+struct Pair2 { uint32_t all[2], neg[2]; };
 struct LdsCounts {
   const uint32_t* count;
-  __device__ __forceinline__ void operator()(int g, uint32_t (&all)[2], uint32_t (&neg)[2]) const {
+  __device__ __forceinline__ Pair2 load(int g) const {
     const uint2 c = ((const uint2*)count)[g * (GROUP / 2) + (threadIdx.x & 63)];
-    all[0] = c.x & 0xffffu; neg[0] = c.x >> 16; all[1] = c.y & 0xffffu; neg[1] = c.y >> 16;
+    return {{c.x & 0xffffu, c.y & 0xffffu}, {c.x >> 16, c.y >> 16}};
   }
+  __device__ __forceinline__ Pair2 again(const HalfScratch&, int g) const { return load(g); }
+  __device__ __forceinline__ void keep(const HalfScratch&, int, const Pair2&) const {}
 };
 constexpr int HALF_SLICES = 96;  // of a row, at most: 65 cover 2^22 logits
+constexpr int SLOTS = 128;
 struct SliceCounts {
   const HalfSlice* slice; int n;
   const uint64_t (*has)[GROUPS / 64];  // of every slice, in LDS
-  __device__ __forceinline__ void operator()(int g, uint32_t (&all)[2], uint32_t (&neg)[2]) const {
+  uint4* kept;                         // [SLOTS][64], in LDS
+  __device__ __forceinline__ int slot(const HalfScratch& s, int g) const {  // marked groups before g
+    int r = 0;
+    for (int i = 0; i < (g >> 6); ++i) r += __popcll(s.has[i]);
+    return r + __popcll(s.has[g >> 6] & ((1ull << (g & 63)) - 1));
+  }
+  __device__ __forceinline__ Pair2 load(int g) const {
     const int lane = threadIdx.x & 63, at = g * (GROUP / 2) + lane;
-    all[0] = all[1] = neg[0] = neg[1] = 0;
+    Pair2 r = {{0, 0}, {0, 0}};
     for (int i0 = 0; i0 < n; i0 += 64) {
       uint64_t left = __ballot(i0 + lane < n && ((has[i0 + lane < n ? i0 + lane : i0][g >> 6] >> (g & 63)) & 1));
-      while (left) {  // eight slices' loads at a time
-        uint2 c[8];
+      while (left) {  // sixteen slices' loads at a time
+        uint2 c[16];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < 16; ++u) {
           c[u] = make_uint2(0, 0);
           if (left) {
             c[u] = ((const uint2*)slice[i0 + __ffsll((long long)left) - 1].count)[at];
@@ -806,70 +827,93 @@ struct SliceCounts {
           }
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          all[0] += c[u].x & 0xffffu; neg[0] += c[u].x >> 16; all[1] += c[u].y & 0xffffu; neg[1] += c[u].y >> 16;
+        for (int u = 0; u < 16; ++u) {
+          r.all[0] += c[u].x & 0xffffu; r.neg[0] += c[u].x >> 16; r.all[1] += c[u].y & 0xffffu; r.neg[1] += c[u].y >> 16;
         }
       }
     }
+    return r;
+  }
+  __device__ __forceinline__ void keep(const HalfScratch& s, int g, const Pair2& c) const {
+    const int at = slot(s, g);
+    if (at < SLOTS) kept[at * 64 + (threadIdx.x & 63)] = make_uint4(c.all[0], c.all[1], c.neg[0], c.neg[1]);
+  }
+  __device__ __forceinline__ Pair2 again(const HalfScratch& s, int g) const {
+    const int at = slot(s, g);
+    if (at >= SLOTS) return load(g);
+    const uint4 c = kept[at * 64 + (threadIdx.x & 63)];
+    return {{c.x, c.y}, {c.z, c.w}};
   }
 };
-// the candidates among them: negative counts for NEG (below the infinity), positive ones else (up to it; zero takes both signs)
-template <class T, bool NEG> __device__ __forceinline__ void valid2(int g, const uint32_t (&all)[2], const uint32_t (&neg)[2], uint32_t (&c)[2]) {
+// the candidates among them: negative counts for `neg` (below the infinity), positive ones else (up to it; zero takes both signs)
+template <class T> __device__ __forceinline__ void valid2(int g, bool neg, const Pair2& p, uint32_t (&c)[2]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t mag = (uint32_t)(g * GROUP + 2 * (threadIdx.x & 63) + i);
-    if (NEG) c[i] = mag != 0 && mag < Half<T>::INF ? neg[i] : 0;
-    else c[i] = mag == 0 ? all[i] : mag <= Half<T>::INF ? all[i] - neg[i] : 0;
+    if (neg) c[i] = mag != 0 && mag < Half<T>::INF ? p.neg[i] : 0;
+    else c[i] = mag == 0 ? p.all[i] : mag <= Half<T>::INF ? p.all[i] - p.neg[i] : 0;
   }
+}
+__device__ __forceinline__ uint32_t half_raw(int g, bool neg, int i) {
+  return (uint32_t)(g * GROUP + 2 * ((int)threadIdx.x & 63) + i) | (neg ? 0x8000u : 0u);
+}
+__device__ __forceinline__ int group_of(int order) { return order < GROUPS ? GROUPS - 1 - order : order - GROUPS; }
+
+// One wave: counts and weights by order become running sums
+__device__ __forceinline__ void prefix_half(HalfScratch& s) {
+  constexpr int R = 2 * GROUPS / 64;
+  const int lane = threadIdx.x & 63;
+  uint32_t c[R], cs = 0;
+  uint64_t w[R], ws = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    cs += s.count[lane * R + i];
+    ws += s.weight[lane * R + i];
+    c[i] = cs;
+    w[i] = ws;
+  }
+  cs = wave_scan(cs) - cs;
+  ws = wave_scan(ws) - ws;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    s.count[lane * R + i] = cs + c[i];
+    s.weight[lane * R + i] = ws + w[i];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 struct Spot { uint32_t raw, tie, ties; uint64_t before, one; __device__ uint64_t end() const { return before + (uint64_t)(tie + 1) * one; } };
-// One wave: the value at which the running count (BY_COUNT) or weight passes target; before, one: weights
+// One wave: the value at which the running count (BY_COUNT) or weight passes target (the total does); before, one: weights
 template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfScratch& s, const C& counts, const Weigher& w, uint64_t target) {
   const int lane = threadIdx.x & 63;
   constexpr int R = 2 * GROUPS / 64;
-  uint64_t sc = 0, sw = 0;
-#pragma unroll
-  for (int i = 0; i < R; ++i) { sc += s.count[lane * R + i]; sw += s.weight[lane * R + i]; }
-  uint64_t bc = wave_scan(sc) - sc, bw = wave_scan(sw) - sw;
-  const uint64_t b = BY_COUNT ? bc : bw;
-  int owner = __ffsll(__ballot(b <= target && target < b + (BY_COUNT ? sc : sw))) - 1;
-  bc = shfl64(bc, owner);
-  bw = shfl64(bw, owner);
-  int order = owner * R;
-  for (int i = 0; i < R - 1; ++i) {  // uniform
-    const uint64_t c = s.count[order], v = s.weight[order];
-    if (target < (BY_COUNT ? bc + c : bw + v)) break;
-    bc += c;
-    bw += v;
-    ++order;
-  }
-  const bool neg_side = order >= GROUPS;
-  const int g = neg_side ? order - GROUPS : GROUPS - 1 - order;
-  uint32_t all[2], neg[2], c[2];
-  counts(g, all, neg);
-  if (neg_side) valid2<T, true>(g, all, neg, c); else valid2<T, false>(g, all, neg, c);
-  // in falling order: negative values as they lie, positive ones from the other end
+  // 64 running sums, R apart, then the R between them
+  auto sum = [&](int i) { return BY_COUNT ? (uint64_t)s.count[i] : s.weight[i]; };
+  int order = R * (__ffsll(__ballot(target < sum(lane * R + R - 1))) - 1);
+  order += __ffsll(__ballot(lane < R && target < sum(order + (lane < R ? lane : 0)))) - 1;
+  uint64_t bc = order > 0 ? s.count[order - 1] : 0, bw = order > 0 ? s.weight[order - 1] : 0;
+  const bool neg = order >= GROUPS;
+  const int g = group_of(order);
+  uint32_t c[2];
+  valid2<T>(g, neg, counts.again(s, g), c);
   uint64_t v[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t raw = (uint32_t)(g * GROUP + 2 * lane + i) | (neg_side ? 0x8000u : 0u);
-    v[i] = c[i] ? (uint64_t)c[i] * w.of(half_value<T>(raw)) : 0;
-  }
-  sc = (uint64_t)c[0] + c[1];
-  sw = v[0] + v[1];
-  const uint64_t ic = wave_scan(sc), iw = wave_scan(sw);
-  bc += neg_side ? ic - sc : shfl64(ic, 63) - ic;
-  bw += neg_side ? iw - sw : shfl64(iw, 63) - iw;
+  for (int i = 0; i < 2; ++i) v[i] = c[i] ? (uint64_t)c[i] * w.of(half_value<T>(half_raw(g, neg, i))) : 0;
+  // in falling order: negative values as they lie, positive ones from the other end
+  const uint32_t sc = c[0] + c[1], ic = wave_scan(sc);
+  const uint64_t sw = v[0] + v[1], iw = wave_scan(sw);
+  bc += neg ? ic - sc : lane_value(ic, 63) - ic;
+  bw += neg ? iw - sw : lane_value(iw, 63) - iw;
   Spot out = {0, 0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int i = neg_side ? j : 1 - j;
+    const int i = neg ? j : 1 - j;
     const uint32_t ci = i ? c[1] : c[0];
     const uint64_t vi = i ? v[1] : v[0];
     const uint64_t here = BY_COUNT ? bc : bw, mine = BY_COUNT ? ci : vi;
     if (here <= target && target < here + mine) {
-      out.raw = (uint32_t)(g * GROUP + 2 * lane + i) | (neg_side ? 0x8000u : 0u);
+      out.raw = half_raw(g, neg, i);
       out.one = vi / ci;
       out.tie = (uint32_t)((target - here) / (BY_COUNT ? 1 : out.one));
       out.ties = ci;
@@ -878,98 +922,88 @@ template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfS
     bc += ci;
     bw += vi;
   }
-  owner = __ffsll(__ballot(out.ties != 0)) - 1;
-  out.raw = __shfl((int)out.raw, owner, 64);
-  out.tie = __shfl((int)out.tie, owner, 64);
-  out.ties = __shfl((int)out.ties, owner, 64);
-  out.before = shfl64(out.before, owner);
-  out.one = shfl64(out.one, owner);
+  const int owner = __ffsll(__ballot(out.ties != 0)) - 1;
+  out.raw = lane_value(out.raw, owner);
+  out.tie = lane_value(out.tie, owner);
+  out.ties = lane_value(out.ties, owner);
+  out.before = lane_value(out.before, owner);
+  out.one = lane_value(out.one, owner);
   return out;
 }
 
 // The workgroup's decision for a row from its counts (s.has filled): s.raw, s.tie, s.ties, s.prob; false for an empty row.
 template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C& counts, const Settings& st, int V, int S) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int R = 2 * GROUPS / 64;
   for (int i = threadIdx.x; i < 2 * GROUPS; i += HWG) { s.weight[i] = 0; s.count[i] = 0; }
-  if (threadIdx.x == 0) { s.heavy = 0; s.top = 0xffffffffu; }
+  if (threadIdx.x == 0) s.heavy = 0;
   __syncthreads();
-  // the largest candidate (wave 0): in the uppermost marked group that has a positive one, else the lowest with a negative one
-  if (wave == 0) {
-    bool found = false;
-    for (int word = GROUPS / 64 - 1; word >= 0 && !found; --word) {
-      for (uint64_t left = s.has[word]; left && !found;) {
-        const int bit = 63 - __clzll((long long)left);
-        left &= ~(1ull << bit);
-        uint32_t all[2], neg[2], c[2];
-        counts(64 * word + bit, all, neg);
-        valid2<T, false>(64 * word + bit, all, neg, c);
-        const unsigned long long hit = __ballot((c[0] | c[1]) != 0);
-        found = hit != 0;
-        if (found && lane == 63 - __clzll((long long)hit)) s.top = (uint32_t)((64 * word + bit) * GROUP + 2 * lane + (c[1] ? 1 : 0));
-      }
-    }
-    for (int word = 0; word < GROUPS / 64 && !found; ++word) {
-      for (uint64_t left = s.has[word]; left && !found;) {
-        const int bit = __ffsll((long long)left) - 1;
-        left &= left - 1;
-        uint32_t all[2], neg[2], c[2];
-        counts(64 * word + bit, all, neg);
-        valid2<T, true>(64 * word + bit, all, neg, c);
-        const unsigned long long hit = __ballot((c[0] | c[1]) != 0);
-        found = hit != 0;
-        if (found && lane == __ffsll((long long)hit) - 1) s.top = (uint32_t)((64 * word + bit) * GROUP + 2 * lane + (c[0] ? 0 : 1)) | 0x8000u;
-      }
-    }
-  }
+  // the marked groups, the waves in turn: candidates of both signs
+  auto groups = [&](auto f) {
+    int turn = 0;
+    for (int word = 0; word < GROUPS / 64; ++word)
+      for (uint64_t left = s.has[word]; left; left &= left - 1)
+        if (turn++ % (HWG / 64) == wave) f(64 * word + __ffsll((long long)left) - 1);
+  };
+  groups([&](int g) {
+    const Pair2 p = counts.load(g);
+    counts.keep(s, g, p);
+    uint32_t pos[2], neg[2];
+    valid2<T>(g, false, p, pos);
+    valid2<T>(g, true, p, neg);
+    const uint32_t np = wave_sum(pos[0] + pos[1]), nn = wave_sum(neg[0] + neg[1]);
+    if (lane == 0) { s.count[GROUPS - 1 - g] = np; s.count[GROUPS + g] = nn; }
+  });
   __syncthreads();
-  if (s.top == 0xffffffffu) return false;
-  const float top = half_value<T>(s.top);
-  const Weigher w(st, top, S);
+  // the largest candidate, in the first order that has one (every wave finds it)
+  uint32_t first = 2 * GROUPS;
+#pragma unroll
+  for (int i = R - 1; i >= 0; --i) first = s.count[lane * R + i] ? lane * R + i : first;
+  const unsigned long long some = __ballot(first < 2 * GROUPS);
+  if (!some) return false;
+  const int order = (int)lane_value(first, __ffsll(some) - 1);
+  uint32_t c[2];
+  valid2<T>(group_of(order), order >= GROUPS, counts.again(s, group_of(order)), c);
+  const unsigned long long hit = __ballot((c[0] | c[1]) != 0);
+  const int at = order < GROUPS ? 63 - __clzll((long long)hit) : __ffsll(hit) - 1;
+  const uint32_t mine = half_raw(group_of(order), order >= GROUPS, order < GROUPS ? (c[1] ? 1 : 0) : (c[0] ? 0 : 1));
+  const Weigher w(st, half_value<T>(lane_value(mine, at)), S);
   const bool greedy = st.greedy();
-  for (int g = wave; g < GROUPS; g += HWG / 64) {  // a wave's groups: sums of both signs
-    if (!((s.has[g >> 6] >> (g & 63)) & 1)) continue;
-    uint32_t all[2], neg[2], c[2];
-    counts(g, all, neg);
+  if (!greedy) {
+    groups([&](int g) {
+      const Pair2 p = counts.again(s, g);
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      if (side) valid2<T, true>(g, all, neg, c); else valid2<T, false>(g, all, neg, c);
-      if (!__ballot((c[0] | c[1]) != 0)) continue;
-      uint64_t sum = 0, heavy = 0;
-      if (!greedy) {
+      for (int side = 0; side < 2; ++side) {
+        uint32_t c[2];
+        valid2<T>(g, side != 0, p, c);
+        if (!__ballot((c[0] | c[1]) != 0)) continue;
+        uint64_t sum = 0, heavy = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (c[i]) {
-            const double x = w.x(half_value<T>((uint32_t)(g * GROUP + 2 * lane + i) | (side ? 0x8000u : 0u)));
-            const uint64_t v = (uint64_t)c[i] * w.at(x);
-            sum += v;
-            if (x >= w.floor_x) heavy += v;
-          }
+        for (int i = 0; i < 2; ++i) {
+          const double x = w.x(half_value<T>(half_raw(g, side != 0, i)));
+          const uint64_t v = c[i] ? (uint64_t)c[i] * w.at(x) : 0;
+          sum += v;
+          if (x >= w.floor_x) heavy += v;
+        }
         sum = wave_sum(sum);
-        if (st.m > 0.0f) heavy = wave_sum(heavy);
+        if (lane == 0) s.weight[side ? GROUPS + g : GROUPS - 1 - g] = sum;
+        if (st.m > 0.0f) {
+          heavy = wave_sum(heavy);
+          if (lane == 0 && heavy) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
+        }
       }
-      const uint32_t n = (uint32_t)wave_sum((uint64_t)c[0] + c[1]);
-      if (lane == 0) {
-        const int order = side ? GROUPS + g : GROUPS - 1 - g;
-        s.weight[order] = sum;
-        s.count[order] = n;
-        if (st.m > 0.0f && heavy) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
-      }
-    }
+    });
+    __syncthreads();
   }
-  __syncthreads();
   if (wave == 0) {
+    prefix_half(s);
     Spot at;
     float prob = 1.0f;
     if (greedy) {
       at = spot_half<T, true>(s, counts, w, 0);
     } else {
-      constexpr int R = 2 * GROUPS / 64;
-      uint64_t total = 0, n = 0;
-#pragma unroll
-      for (int i = 0; i < R; ++i) { total += s.weight[lane * R + i]; n += s.count[lane * R + i]; }
-      total = wave_sum(total);
-      n = wave_sum(n);
-      if (st.limited(V) && (uint64_t)st.k < n) total = spot_half<T, true>(s, counts, w, (uint64_t)st.k - 1).end();
+      uint64_t total = s.weight[2 * GROUPS - 1];
+      if (st.limited(V) && (uint32_t)st.k < s.count[2 * GROUPS - 1]) total = spot_half<T, true>(s, counts, w, (uint64_t)st.k - 1).end();
       uint64_t kept = total;
       if (st.p < 1.0f) {
         const uint64_t t = st.goal(total);
@@ -1024,7 +1058,7 @@ template <class T> __device__ void find_half(HalfScratch& s, const Row<T>& row, 
   uint32_t mine = 0;
 #pragma unroll 4
   for (int j = w0; j < w1; j += 64) mine += __popc(matches(j + lane));
-  mine = (uint32_t)wave_sum(mine);
+  mine = wave_sum(mine);
   if (lane == 0) s.part[wave] = mine;
   __syncthreads();
   uint32_t before = 0;
@@ -1032,7 +1066,7 @@ template <class T> __device__ void find_half(HalfScratch& s, const Row<T>& row, 
   if (tie < before || tie >= before + mine) return;
   for (int j = w0; j < w1; j += 64) {
     uint32_t m = matches(j + lane);
-    const uint32_t n = __popc(m), incl = (uint32_t)wave_scan(n), all = (uint32_t)shfl64(incl, 63);
+    const uint32_t n = __popc(m), incl = wave_scan(n), all = lane_value(incl, 63);
     if (tie < before + all) {
       const uint32_t first = before + incl - n;
       if (tie >= first && tie < first + n) {
@@ -1048,12 +1082,13 @@ template <class T> __device__ void find_half(HalfScratch& s, const Row<T>& row, 
 // the counts of a row's slices -> its token
 template <class T>
 __global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, int r0, const HalfSlice* ws, int slices, int per, int S) {
+  extern __shared__ __attribute__((aligned(16))) uint4 kept[];  // [SLOTS][64]
   __shared__ HalfScratch s;
   const int r = r0 + blockIdx.x, lane = threadIdx.x & 63;
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const Settings st(a, r);
   __shared__ uint64_t has[HALF_SLICES][GROUPS / 64];
-  const SliceCounts counts = {ws + (size_t)blockIdx.x * slices, slices, has};
+  const SliceCounts counts = {ws + (size_t)blockIdx.x * slices, slices, has, kept};
   if ((int)threadIdx.x < slices * (GROUPS / 64)) has[threadIdx.x / (GROUPS / 64)][threadIdx.x % (GROUPS / 64)] =
       counts.slice[threadIdx.x / (GROUPS / 64)].has[threadIdx.x % (GROUPS / 64)];
   __syncthreads();
@@ -1076,7 +1111,7 @@ __global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, in
         const uint32_t c = counts.slice[i].count[mag];
         n = mag == 0 ? c & 0xffffu : s.raw & 0x8000u ? c >> 16 : (c & 0xffffu) - (c >> 16);
       }
-      const uint32_t incl = (uint32_t)wave_scan(n), all = (uint32_t)shfl64(incl, 63);
+      const uint32_t incl = wave_scan(n), all = lane_value(incl, 63);
       const uint32_t first = before + incl - n;
       const bool here = s.tie >= first && s.tie < first + n;
       if (__ballot(here)) {
@@ -1283,10 +1318,10 @@ __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int 
       n += in[i];
     }
     if (__ballot(n != 0) == 0) continue;
-    const uint32_t incl = (uint32_t)wave_scan(n);
+    const uint32_t incl = wave_scan(n);
     uint32_t base = 0;
     if (lane == 63) base = atomicAdd(&l.listed, incl);
-    uint32_t at = (uint32_t)__shfl((int)base, 63, 64) + incl - n;
+    uint32_t at = lane_value(base, 63) + incl - n;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (in[i]) {
@@ -1484,9 +1519,9 @@ HalfPlan half_plan(int M, int V) {
   p.slices = (granules + HALF_GRANULES - 1) / HALF_GRANULES;
   p.rows = HALF_AT_ONCE / p.slices < M ? HALF_AT_ONCE / p.slices : M;  // V <= 2^22: at most 65 slices
   if (p.slices > 1 || M < 64) {
-    // few rows: more and shorter slices, up to one workgroup a CU, but four granules a thread at least: the second launch adds
-    // the slices' counts (1 x 250002: 31 slices of one granule 64 us, 8 of four TODO us)
-    const int most = (granules + 4 * HWG - 1) / (4 * HWG), want = 256 / p.rows;
+    // few rows: more and shorter slices, up to one workgroup a CU, but eight of four granules a thread at most: the second launch
+    // has one workgroup to add the slices' counts (1 x 250002: 31 slices 64 us, 8 slices 23 us)
+    const int most = (granules + 4 * HWG - 1) / (4 * HWG), want = 256 / p.rows < 8 ? 256 / p.rows : 8;
     const int more = most < want ? most : want;
     p.slices = more > p.slices ? more : p.slices;
     p.slices = p.slices < HALF_SLICES ? p.slices : HALF_SLICES;
@@ -1505,12 +1540,14 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
     CUBE_CHECK_LAUNCH("cube_sample_rows");
     return CUBE_OK;
   }
-  static CubeLdsReservation lds;
-  if (!lds.ensure((const void*)half_count_kernel<T>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
+  static CubeLdsReservation lds, lds2;
+  constexpr size_t kept = 16 * 64 * SLOTS + 16;  // (16: always past the size that needs no reservation)
+  if (!lds.ensure((const void*)half_count_kernel<T>, bytes) || !lds2.ensure((const void*)half_choose_kernel<T>, kept))
+    CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
   for (int r0 = 0; r0 < a.M; r0 += p.rows) {
     const int n = a.M - r0 < p.rows ? a.M - r0 : p.rows;
     hipLaunchKernelGGL((half_count_kernel<T>), dim3(p.slices, n), dim3(HWG), bytes, st, a, r0, ws, p.per);
-    hipLaunchKernelGGL((half_choose_kernel<T>), dim3(n), dim3(HWG), 0, st, a, r0, ws, p.slices, p.per, S);
+    hipLaunchKernelGGL((half_choose_kernel<T>), dim3(n), dim3(HWG), kept, st, a, r0, ws, p.slices, p.per, S);
     CUBE_CHECK_LAUNCH("cube_sample_rows");
   }
   return CUBE_OK;
