@@ -233,8 +233,10 @@ template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_wai
 // read then cover all 64 banks: by row & 7 they met in pairs), and the scale word of every row.  ST stages: step k computes while k + 1 .. k + ST - 1 are on their way; the
 // wait for step k counts the later stages' loads instead of draining them.
 // Which 32 of the 128 columns a lane group holds does not matter as long as both operands agree, since a step shares its scales.
-template <int BM, int BN, int WM, int WN, int ST, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params p) {
+// KS > 1: as many groups of WM x WN waves share K (each a stretch of its own through stages of its own) and meet in LDS at the end,
+// in group order: for few tiles with a long K.
+template <int BM, int BN, int WM, int WN, int ST, int KS, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN * KS) void gemm_fp8_kernel(const Fp8Params p) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // 1-KiB DMA pieces (8 rows) a wave issues per step
   constexpr int SP = (BM + BN) / 64, PS = (SP + NW - 1) / NW;  // pieces of 64 scale words (waves without one load the last again)
@@ -242,17 +244,20 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
   constexpr int ROWS = (BM + BN) * BLK, STAGE = ROWS + (BM + BN) * 4;
   constexpr int LOADS = PA + PB + PS;                    // a wave's loads per stage
   constexpr int PER = (LOADS + TM - 1) / TM;             // of them, with each row tile's products
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  extern __shared__ __attribute__((aligned(16))) unsigned char all_smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave / NW, wid = wave % NW;
+  unsigned char* smem = all_smem + kg * ST * STAGE;
   const int wm = wid / WN, wn = wid % WN;
-  // Workgroups go round-robin over the 8 XCDs, each with an L2 of its own.  An XCD has every eighth row tile and takes them four at a
-  // time, column tile by column tile: the 32 workgroups it runs at once then cover 4 x 8 tiles and share 12 operand tiles (2 x 16 of
-  // a row-major order share 18: 3 % more time at 8192x4096x4096)
-  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-  const int rows_of = (p.m_tiles + 7) / 8, group = slot / (4 * p.n_tiles), in = slot - group * 4 * p.n_tiles;
-  const int high = rows_of - 4 * group < 4 ? rows_of - 4 * group : 4;  // row tiles of the group
-  const int nt = in / high, mt = (4 * group + in - nt * high) * 8 + xcd;
-  if (mt >= p.m_tiles) return;  // whole workgroup, before any barrier
+  // Workgroups go round-robin over the 8 XCDs, each with an L2 of its own.  The tiles are counted in groups of four row tiles, column
+  // by column, and an XCD gets an eighth of that count: the 32 workgroups it runs at once then cover 4 x 8 tiles and share 12 operand
+  // tiles (2 x 16 of a row-major order share 18: 3 % more time at 8192x4096x4096), and no XCD has more than one tile over another.
+  const int tiles = p.m_tiles * p.n_tiles, eighth = (tiles + 7) / 8;
+  const int tile = (blockIdx.x & 7) * eighth + (blockIdx.x >> 3);
+  if (tile >= tiles) return;  // whole workgroup, before any barrier
+  const int group = tile / (4 * p.n_tiles), in = tile - group * 4 * p.n_tiles;
+  const int high = p.m_tiles - 4 * group < 4 ? p.m_tiles - 4 * group : 4;  // row tiles of the group
+  const int nt = in / high, mt = 4 * group + in - nt * high;
   const int m0 = mt * BM, n0 = nt * BN;
 
   // a load's address: the tile's first row (uniform) and 32 bits of offset inside the tile (255 rows of at most 2^24 bytes)
@@ -279,16 +284,19 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
     const int r = of_a ? t : t - BM, last = (of_a ? p.M - m0 : p.N - n0) - 1;
     s_off[i] = 4 * (uint32_t)(r < last ? r : last);
   }
-  // load `i` of stage k: activations, weights, scale words
+  // this group's steps
+  const int per = (p.KB + KS - 1) / KS, first = kg * per;
+  const int steps = KS == 1 ? p.KB : p.KB - first < per ? (p.KB > first ? p.KB - first : 0) : per;
+  // load `i` of this group's step k: activations, weights, scale words
   auto load = [&](int k, int i) {
     unsigned char* buf = smem + (k % ST) * STAGE;
     if (i < PA) {
-      dma16(a_base + (size_t)k * BLK + off[i], buf + 8 * (wid + NW * i) * BLK);
+      dma16(a_base + (size_t)(first + k) * BLK + off[i], buf + 8 * (wid + NW * i) * BLK);
     } else if (i < PA + PB) {
-      dma16(b_base + (size_t)k * BLK + off[i], buf + (BM + 8 * (wid + NW * (i - PA))) * BLK);
+      dma16(b_base + (size_t)(first + k) * BLK + off[i], buf + (BM + 8 * (wid + NW * (i - PA))) * BLK);
     } else {
       const int of = wid + NW * (i - PA - PB), t = of < SP ? of : SP - 1;
-      const uint32_t* s = 64 * t < BM ? p.A_scale + (long long)(k >> 2) * p.lds_a + m0 : p.W_scale + (long long)(k >> 2) * p.lds_w + n0;
+      const uint32_t* s = 64 * t < BM ? p.A_scale + (long long)((first + k) >> 2) * p.lds_a + m0 : p.W_scale + (long long)((first + k) >> 2) * p.lds_w + n0;
       dma4((const uint8_t*)s + s_off[i - PA - PB], buf + ROWS + 64 * t * 4);
     }
   };
@@ -305,21 +313,24 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = bias[j];
+    for (int j = 0; j < TN; ++j) acc[i][j] = KS == 1 || kg == 0 ? bias[j] : (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
 #pragma unroll
   for (int k = 0; k < ST - 1; ++k)
-    if (k < p.KB) fill(k);
+    if (k < steps) fill(k);
   // this lane's two chunks of a row of a fragment
   const int o0 = l15 * BLK + ((g ^ (l15 >> 1)) << 4), o1 = l15 * BLK + (((g + 4) ^ (l15 >> 1)) << 4);
   // One step.  MORE: with the loads of stage k + ST - 1, which go out between the products (all at once in front of them they held
   // up the fragment reads); no branch inside, so that they stay there.
-  auto step = [&](int k, auto MORE) {
-    const unsigned char* cur = smem + (k % ST) * STAGE;
+  auto meet = [&] {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int shift = 8 * (k & 3);
+  };
+  auto step = [&](int k, auto MORE) {
+    const unsigned char* cur = smem + (k % ST) * STAGE;
+    meet();
+    const int shift = 8 * ((first + k) & 3);
     auto frag = [&](int tile) {  // of the stage's tiles of 16 rows
       const i32x4 lo = *(const i32x4*)(cur + tile * 16 * BLK + o0), hi = *(const i32x4*)(cur + tile * 16 * BLK + o1);
       return (i32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -349,13 +360,37 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
   // step k has landed once no more loads are open than the later stages'; the barrier in the step says so for every wave's pieces, and
   // that all waves are done with the stage that is filled next
   int k = 0;
-  for (; k < p.KB - (ST - 1); ++k) {
+  for (; k < steps - (ST - 1); ++k) {
     wait_vm<(ST - 2) * LOADS>();
     step(k, std::true_type{});
   }
-  for (; k < p.KB; ++k) {
+  for (; k < steps; ++k) {
     wait_vm<0>();
     step(k, std::false_type{});
+  }
+  if constexpr (KS > 1) {
+    for (; k < per; ++k) meet();  // a group with fewer steps comes to as many barriers
+    meet();
+    f32x4* part = (f32x4*)all_smem;  // [KS - 1][waves][TM][TN][64]
+    static_assert((KS - 1) * NW * TM * TN * 1024 <= KS * ST * STAGE, "the partial sums fit in the stages' LDS");
+    if (kg > 0) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) part[((((kg - 1) * NW + wid) * TM + i) * TN + j) * 64 + lane] = acc[i][j];
+    }
+    meet();
+    if (kg > 0) return;
+#pragma unroll
+    for (int q = 0; q < KS - 1; ++q)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const f32x4 o = part[(((q * NW + wid) * TM + i) * TN + j) * 64 + lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] += o[r];
+        }
   }
 
   // ---- results: activation and rounding in registers, then through LDS (a wave its own part), so that whole rows of the wave's
@@ -377,10 +412,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
   }
   constexpr int ES = EXACT ? 4 : 2, RB = 16 * TN * ES, SWZ = RB >= 128 ? 7 : RB / 16 - 1;  // bytes of a value, of a row
   static_assert((RB & (RB - 1)) == 0 && RB >= 32, "the swizzle stays inside the row");
-  static_assert(NW * 16 * TM * RB <= ST * STAGE, "the results fit in the stages' LDS");
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();  // all waves are done with the last stage
-  asm volatile("" ::: "memory");
+  static_assert(NW * 16 * TM * RB <= KS * ST * STAGE, "the results fit in the stages' LDS");
+  meet();  // all waves are done with the last stage (and with the partial sums)
   unsigned char* mine = smem + wid * 16 * TM * RB;
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -427,22 +460,31 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_fp8_kernel(const Fp8Params 
   else copy(uint16_t{});
 }
 
-// Few rows: the weights are read once, straight into registers, 16 columns a workgroup, and its 8 waves share K (wave v takes the
-// blocks v, v + 8, ...); their sums meet in LDS, in wave order.  T: the type of the activations.  Plain rows are quantised into LDS
+// Few rows: the weights are read once, straight into registers, in tiles of 16 columns.  KW = 8: a workgroup has a tile and its 8
+// waves share K (wave v takes the blocks v, v + 8, ...); their sums meet in LDS, in wave order.  KW = 1: every wave has a tile of its
+// own and all of K (no barrier), where there are tiles enough for all waves.  T: the type of the activations.  Plain rows are quantised into LDS
 // by every workgroup for itself (the first weight loads are already on their way); e4m3 rows are read where they are.
-constexpr int FEW_ROWS = 64, FEW_WAVES = 8, FEW_LDS = 64 * 1024, FEW_AHEAD = 4;
+constexpr int FEW_ROWS = 32, FUSED_ROWS = 48, FEW_WAVES = 8, FEW_LDS = 38 * 1024, FEW_AHEAD = 4, FEW_GRID = 1024;
 __host__ __device__ inline int few_stride(int KB) { return KB * BLK + 16; }  // bytes of a row in LDS: 16 rows then cover all banks
-template <class T, bool VEC, int MT, bool EXACT>
+__host__ __device__ inline long long few_rows_bytes(int rows, int KB) { return ((long long)rows * (few_stride(KB) + KB) + 15) / 16 * 16; }  // with scales
+template <class T, bool VEC, int MT, int KW, bool EXACT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void few_fp8_kernel(const Fp8Params p) {
   constexpr bool PLAIN = !std::is_same<T, uint8_t>::value;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l15 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
-  const int rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
-  const int nr = n0 + l15 < p.N ? n0 + l15 : p.N - 1;
-  const uint8_t* wrow = p.W + (long long)nr * p.ldw + g * 32;
-  const uint32_t* ws = p.W_scale + nr;
+  const int kw = KW == 1 ? 0 : wave;  // this wave's first block of K
+  int n0 = (KW == 1 ? blockIdx.x * FEW_WAVES + wave : blockIdx.x) * 16;
+  const int n_step = (KW == 1 ? gridDim.x * FEW_WAVES : gridDim.x) * 16;
+  const int rows = p.M;  // at most 16 * MT
+  const uint8_t* wrow;
+  const uint32_t* ws;
+  auto columns = [&](int n) {
+    const int nr = n + l15 < p.N ? n + l15 : p.N - 1;
+    wrow = p.W + (long long)nr * p.ldw + g * 32;
+    ws = p.W_scale + nr;
+  };
+  columns(n0);
   i32x4 wq[FEW_AHEAD][2];
   uint32_t we[FEW_AHEAD];
   auto load_w = [&](int u, int kb) {
@@ -453,24 +495,34 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_fp8_kernel(const Fp8Params
     }
   };
 #pragma unroll
-  for (int u = 0; u < FEW_AHEAD; ++u) load_w(u, wave + FEW_WAVES * u);
-  const f32x4 bias = bias4(p, n0 + 4 * g);
+  for (int u = 0; u < FEW_AHEAD; ++u) load_w(u, kw + KW * u);
 
   const int stride = few_stride(p.KB);
   unsigned char* a_scale = smem + (size_t)rows * stride;  // [rows][KB] scale bytes
   if constexpr (PLAIN) {
-    const T* x = (const T*)p.A + (long long)m0 * p.lda;
+    const T* x = (const T*)p.A;
     const int per = p.KB * (BLK / 8), total = rows * per;  // pieces of 8 columns; 16 lanes a block, so blocks never straddle waves
-    for (int i = threadIdx.x; i < (total + 63) / 64 * 64; i += 64 * FEW_WAVES) {
-      const bool on = i < total;
-      const int r = on ? i / per : 0, c = on ? (i - r * per) * 8 : 0;
-      float v[8];
-      load_cols<T, VEC>(x + (long long)r * p.lda, c, on ? p.K : 0, v);
-      const int byte = scale_byte(max16(amax_bits(v)));
-      const uint2 q = quant8(v, byte);
-      if (on) {
-        *(uint2*)(smem + (size_t)r * stride + c) = q;
-        if ((lane & 15) == 0) a_scale[r * p.KB + c / BLK] = (unsigned char)byte;
+    constexpr int BATCH = 4;  // pieces of a thread whose loads are on their way together
+    for (int i0 = threadIdx.x; i0 < (total + 63) / 64 * 64; i0 += 64 * FEW_WAVES * BATCH) {
+      float v[BATCH][8];
+      int r[BATCH], c[BATCH];
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + 64 * FEW_WAVES * u;
+        if (i - lane >= total) break;  // whole waves
+        r[u] = i < total ? i / per : 0;
+        c[u] = i < total ? (i - r[u] * per) * 8 : 0;
+        load_cols<T, VEC>(x + (long long)r[u] * p.lda, c[u], i < total ? p.K : 0, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        if (i0 + 64 * FEW_WAVES * u - lane >= total) break;
+        const int byte = scale_byte(max16(amax_bits(v[u])));
+        const uint2 q = quant8(v[u], byte);
+        if (i0 + 64 * FEW_WAVES * u < total) {
+          *(uint2*)(smem + (size_t)r[u] * stride + c[u]) = q;
+          if ((lane & 15) == 0) a_scale[r[u] * p.KB + c[u] / BLK] = (unsigned char)byte;
+        }
       }
     }
     __syncthreads();
@@ -478,52 +530,75 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_fp8_kernel(const Fp8Params
   int ar[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) ar[t] = 16 * t + l15 < rows ? 16 * t + l15 : rows - 1;
-  f32x4 acc[MT];
+  f32x4* part = (f32x4*)(smem + (PLAIN ? few_rows_bytes(rows, p.KB) : 0));
+  // column tiles in turn: the activations in LDS serve them all (KW = 8: a workgroup's waves come to the end together)
+  while (KW != 1 || n0 < p.N) {
+    f32x4 acc[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kb0 = wave; kb0 < p.KB; kb0 += FEW_WAVES * FEW_AHEAD) {
+    for (int t = 0; t < MT; ++t) acc[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const f32x4 bias = bias4(p, n0 + 4 * g);
+    const int n_next = n0 + n_step;
+    for (int kb0 = kw; kb0 < p.KB; kb0 += KW * FEW_AHEAD) {
 #pragma unroll
-    for (int u = 0; u < FEW_AHEAD; ++u) {
-      const int kb = kb0 + FEW_WAVES * u;
-      if (kb < p.KB) {  // wave-uniform
-        const Operand<EXACT> w((i32x8){wq[u][0][0], wq[u][0][1], wq[u][0][2], wq[u][0][3], wq[u][1][0], wq[u][1][1], wq[u][1][2], wq[u][1][3]},
-                               we[u] >> (8 * (kb & 3)));
-        load_w(u, kb + FEW_WAVES * FEW_AHEAD);
+      for (int u = 0; u < FEW_AHEAD; ++u) {
+        const int kb = kb0 + KW * u;
+        if (kb < p.KB) {  // wave-uniform
+          const Operand<EXACT> w((i32x8){wq[u][0][0], wq[u][0][1], wq[u][0][2], wq[u][0][3], wq[u][1][0], wq[u][1][1], wq[u][1][2], wq[u][1][3]},
+                                 we[u] >> (8 * (kb & 3)));
+          load_w(u, kb + KW * FEW_AHEAD);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          i32x4 lo, hi;
-          uint32_t e;
-          if constexpr (PLAIN) {
-            const unsigned char* b = smem + (size_t)ar[t] * stride + kb * BLK + g * 32;
-            lo = *(const i32x4*)b;
-            hi = *(const i32x4*)(b + 16);
-            e = a_scale[ar[t] * p.KB + kb];
-          } else {
-            const uint8_t* b = p.A + (long long)(m0 + ar[t]) * p.lda + (size_t)kb * BLK + g * 32;
-            lo = *(const i32x4*)b;
-            hi = *(const i32x4*)(b + 16);
-            e = p.A_scale[(long long)(kb >> 2) * p.lds_a + m0 + ar[t]] >> (8 * (kb & 3));
+          for (int t = 0; t < MT; ++t) {
+            i32x4 lo, hi;
+            uint32_t e;
+            if constexpr (PLAIN) {
+              const unsigned char* b = smem + (size_t)ar[t] * stride + kb * BLK + g * 32;
+              lo = *(const i32x4*)b;
+              hi = *(const i32x4*)(b + 16);
+              e = a_scale[ar[t] * p.KB + kb];
+            } else {
+              const uint8_t* b = p.A + (long long)ar[t] * p.lda + (size_t)kb * BLK + g * 32;
+              lo = *(const i32x4*)b;
+              hi = *(const i32x4*)(b + 16);
+              e = p.A_scale[(long long)(kb >> 2) * p.lds_a + ar[t]] >> (8 * (kb & 3));
+            }
+            const Operand<EXACT> a((i32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, e);
+            acc[t] = mma(w, a, acc[t]);
           }
-          const Operand<EXACT> a((i32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, e);
-          acc[t] = mma(w, a, acc[t]);
         }
       }
     }
-  }
-  __syncthreads();  // the activations in LDS are done with
-  f32x4* part = (f32x4*)smem;
+    if (n_next < p.N) {  // the next tile's first weights, under the sums
+      columns(n_next);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) part[(wave * MT + t) * 64 + lane] = acc[t];
-  __syncthreads();
-  if (wave < MT) {
-    f32x4 c = bias;
-#pragma unroll
-    for (int v = 0; v < FEW_WAVES; ++v) {
-      const f32x4 o = part[(v * MT + wave) * 64 + lane];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] += o[i];
+      for (int u = 0; u < FEW_AHEAD; ++u) load_w(u, kw + KW * u);
     }
-    store4(p, m0 + 16 * wave + l15, n0 + 4 * g, c);
+    if constexpr (KW == 1) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        f32x4 c = acc[t];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] += bias[i];
+        store4(p, 16 * t + l15, n0 + 4 * g, c);
+      }
+      n0 = n_next;
+      continue;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[(wave * MT + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    if (wave < MT) {
+      f32x4 c = bias;
+#pragma unroll
+      for (int v = 0; v < FEW_WAVES; ++v) {
+        const f32x4 o = part[(v * MT + wave) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] += o[i];
+      }
+      store4(p, 16 * wave + l15, n0 + 4 * g, c);
+    }
+    if (n_next >= p.N) break;
+    n0 = n_next;
+    __syncthreads();  // the sums in LDS have been read
   }
 }
 
@@ -548,58 +623,68 @@ int quant_any(const void* x, int type, long long ld_x, int M, int K, void* q, lo
   return launch_quant<_Float16>(x, ld_x, M, K, q, ld_q, scale, ld_s, st);
 }
 
-template <int BM, int BN, int WM, int WN, int ST, bool EXACT> int launch_tiles(Fp8Params& p, hipStream_t st) {
-  constexpr int LDS = ST * (BM + BN) * (BLK + 4);
+template <int BM, int BN, int WM, int WN, int ST, int KS, bool EXACT> int launch_tiles(Fp8Params& p, hipStream_t st) {
+  constexpr int LDS = KS * ST * (BM + BN) * (BLK + 4);
   static CubeLdsReservation lds;
   p.m_tiles = (p.M + BM - 1) / BM;
   p.n_tiles = (p.N + BN - 1) / BN;
-  const long long blocks = (long long)((p.m_tiles + 7) / 8 * 8) * p.n_tiles;
-  if (blocks > 0x7fffffffLL) CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: %d x %d outputs are too many", p.M, p.N);
-  if (!lds.ensure((const void*)gemm_fp8_kernel<BM, BN, WM, WN, ST, EXACT>, LDS)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_gemm_fp8: LDS reservation failed");
-  hipLaunchKernelGGL((gemm_fp8_kernel<BM, BN, WM, WN, ST, EXACT>), dim3((unsigned)blocks), dim3(64 * WM * WN), LDS, st, p);
+  const long long blocks = ((long long)p.m_tiles * p.n_tiles + 7) / 8 * 8;
+  if (blocks > 0x7ffffff0LL) CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: %d x %d outputs are too many", p.M, p.N);
+  if (!lds.ensure((const void*)gemm_fp8_kernel<BM, BN, WM, WN, ST, KS, EXACT>, LDS)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_gemm_fp8: LDS reservation failed");
+  hipLaunchKernelGGL((gemm_fp8_kernel<BM, BN, WM, WN, ST, KS, EXACT>), dim3((unsigned)blocks), dim3(64 * WM * WN * KS), LDS, st, p);
   CUBE_CHECK_LAUNCH("cube_gemm_fp8");
   return CUBE_OK;
 }
 
-template <class T, bool VEC, int MT, bool EXACT> int launch_few(const Fp8Params& p, hipStream_t st) {
+template <class T, bool VEC, int MT, int KW, bool EXACT> int launch_few(const Fp8Params& p, hipStream_t st) {
   static CubeLdsReservation lds;
-  const int rows = p.M < 16 * MT ? p.M : 16 * MT;
-  const size_t sums = (size_t)FEW_WAVES * MT * 64 * 16;
-  const size_t act = std::is_same<T, uint8_t>::value ? 0 : (size_t)rows * (few_stride(p.KB) + p.KB);
-  const size_t bytes = act > sums ? act : sums;
-  if (!lds.ensure((const void*)few_fp8_kernel<T, VEC, MT, EXACT>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_gemm_fp8: LDS reservation failed");
-  const dim3 grid((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT));
-  if (grid.y > 65535u) CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: %d rows are too many", p.M);
-  hipLaunchKernelGGL((few_fp8_kernel<T, VEC, MT, EXACT>), grid, dim3(64 * FEW_WAVES), bytes, st, p);
+  const int rows = p.M;
+  const size_t bytes = (size_t)FEW_WAVES * MT * 64 * 16 + (std::is_same<T, uint8_t>::value ? 0 : few_rows_bytes(rows, p.KB));
+  if (!lds.ensure((const void*)few_fp8_kernel<T, VEC, MT, KW, EXACT>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_gemm_fp8: LDS reservation failed");
+  const int tiles = KW == 1 ? (p.N + 16 * FEW_WAVES - 1) / (16 * FEW_WAVES) : (p.N + 15) / 16;
+  const dim3 grid(tiles < FEW_GRID ? tiles : FEW_GRID);
+  hipLaunchKernelGGL((few_fp8_kernel<T, VEC, MT, KW, EXACT>), grid, dim3(64 * FEW_WAVES), bytes, st, p);
   CUBE_CHECK_LAUNCH("cube_gemm_fp8");
   return CUBE_OK;
+}
+template <class T, bool VEC, int MT> int launch_few(const Fp8Params& p, hipStream_t st) {
+  const bool exact = p.out_type == CUBE_T_F32;
+  // a tile for every wave of four workgroups a CU (1 row, 768 columns, 250002 outputs: 38 us, the weights' bytes at the rate of a
+  // copy; shared tiles 71)
+  if (p.N >= 16 * FEW_WAVES * FEW_GRID) return exact ? launch_few<T, VEC, MT, 1, true>(p, st) : launch_few<T, VEC, MT, 1, false>(p, st);
+  return exact ? launch_few<T, VEC, MT, FEW_WAVES, true>(p, st) : launch_few<T, VEC, MT, FEW_WAVES, false>(p, st);
 }
 template <class T, bool VEC> int launch_few(const Fp8Params& p, hipStream_t st) {
-  const bool exact = p.out_type == CUBE_T_F32;
-  if (p.M <= 16) return exact ? launch_few<T, VEC, 1, true>(p, st) : launch_few<T, VEC, 1, false>(p, st);
-  if (p.M <= 32) return exact ? launch_few<T, VEC, 2, true>(p, st) : launch_few<T, VEC, 2, false>(p, st);
-  return exact ? launch_few<T, VEC, 4, true>(p, st) : launch_few<T, VEC, 4, false>(p, st);
+  if (p.M <= 16) return launch_few<T, VEC, 1>(p, st);
+  if (p.M <= 32) return launch_few<T, VEC, 2>(p, st);
+  return launch_few<T, VEC, 3>(p, st);
 }
 
-// plain rows that the few-row kernel quantises by itself: few, and short enough to lie in LDS beside each other
-bool fused(int M, int K) { return M <= FEW_ROWS && (long long)M * few_stride(kblocks(K)) <= FEW_LDS; }
+// The few-row kernel reads the weights once for up to 32 rows (4096x4096: 16 rows 6.5 us, tiles 9.8; 40 rows 13, tiles 10).  It also
+// saves the launch that quantises, while every workgroup quantising all rows costs less: up to 48 rows of some 36000 values in all
+// (768x768: 33 rows 6.9 us, two launches 8.8; 64 rows 10.4, two launches 8.8;  4096x4096: 4 rows 8.6 us, 16 rows 16, two launches 11).
+bool fused(int M, int K) { return M <= FUSED_ROWS && few_rows_bytes(M, kblocks(K)) <= FEW_LDS; }
 
 int launch_gemm(Fp8Params& p, hipStream_t st) {
   const bool exact = p.out_type == CUBE_T_F32;
-  if (p.M <= FEW_ROWS) return launch_few<uint8_t, true>(p, st);
+  if (p.M <= 16) return launch_few<uint8_t, true, 1>(p, st);
+  if (p.M <= FEW_ROWS) return launch_few<uint8_t, true, 2>(p, st);
   // The largest tile that still gives every CU work, by the number of tiles (times of one launch, 16-bit output unless said):
   //   256x256: 8192x4096x4096 110 us (128x128: 125 us), where their last round fills 4 of 5 CUs:  5000x4000x2000, 320 of them,
   //     63 us (54 us), 8192x3000x1024, 384, 42 us (39 us)
   //   128x128 (two workgroups a CU): 8192x768x768 11.7 us (128x64 13.2, 64x64 15.1), 8000x520x8000 54 us (64, 67);
   //     256 of them, one a CU, lose: 2048x2048x2048 18.3 us (128x64 15.3)
   //   128x64: 4096x1024x1024 9.7 us (64x64 12.1), 8192x500x768 f32 14.9 us (18.4)
-  //   64x64 with four stages: 128x768x4096 10.8 us (128x64 15.0), 1001x500x300 f32 6.5 us (7.5)
+  //   64x64 with four stages: 512x768x768 4.8 us (128x64 5.9), 1001x500x300 f32 6.5 us (7.5)
+  //   the same with four wave groups along K: 65x4096x4096 10.3 us (one group 12.8), 65x64x8000 f32 21.4 us (32.5); with a K of
+  //     1024 and less it loses: 65x4096x1024 6.1 us (5.7)
   auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   const long long big = tiles(256, 256), rounds = (big + 255) / 256;
-  if (!exact && 5 * big >= 4 * 256 * rounds) return launch_tiles<256, 256, 2, 4, 2, false>(p, st);
-  if (tiles(128, 128) > 256) return exact ? launch_tiles<128, 128, 2, 2, 2, true>(p, st) : launch_tiles<128, 128, 2, 2, 2, false>(p, st);
-  if (tiles(64, 64) > 512) return exact ? launch_tiles<128, 64, 4, 1, 3, true>(p, st) : launch_tiles<128, 64, 4, 1, 3, false>(p, st);
-  return exact ? launch_tiles<64, 64, 2, 2, 4, true>(p, st) : launch_tiles<64, 64, 2, 2, 4, false>(p, st);
+  if (!exact && 5 * big >= 4 * 256 * rounds) return launch_tiles<256, 256, 2, 4, 2, 1, false>(p, st);
+  if (tiles(128, 128) > 256) return exact ? launch_tiles<128, 128, 2, 2, 2, 1, true>(p, st) : launch_tiles<128, 128, 2, 2, 2, 1, false>(p, st);
+  if (tiles(64, 64) > 512) return exact ? launch_tiles<128, 64, 4, 1, 3, 1, true>(p, st) : launch_tiles<128, 64, 4, 1, 3, 1, false>(p, st);
+  if (tiles(64, 64) <= 256 && p.KB >= 16) return exact ? launch_tiles<64, 64, 2, 2, 2, 4, true>(p, st) : launch_tiles<64, 64, 2, 2, 2, 4, false>(p, st);
+  return exact ? launch_tiles<64, 64, 2, 2, 4, 1, true>(p, st) : launch_tiles<64, 64, 2, 2, 4, 1, false>(p, st);
 }
 
 size_t quant_bytes(int M, int K) {

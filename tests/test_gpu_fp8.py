@@ -145,7 +145,8 @@ def test_quant_writes_nothing_behind_its_rows(dev):
 
 SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 129), (16, 16, 512), (17, 100, 640), (33, 768, 768), (63, 65, 1000), (64, 64, 64), (100, 33, 257),
           (127, 129, 128), (128, 128, 1024), (129, 300, 300), (257, 255, 900), (300, 500, 300), (513, 130, 2304), (1, 1000, 4096),
-          (5, 2000, 1536), (40, 24, 8192), (1030, 520, 384)]
+          (5, 2000, 1536), (40, 24, 8192), (1030, 520, 384), (28, 300, 3000), (64, 200, 2049), (250, 64, 5000),
+          (2100, 1000, 260), (1500, 1500, 129), (4000, 4050, 200)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -159,6 +160,20 @@ def test_gemm_of_integers_is_exact(dev, M, N, K):
     for t in ("bf16", "f16"):
         got = hip.gemm_fp8(a, w, torch.from_numpy(bias).to(dev), out_dtype=TYPES[t])
         assert torch.equal(got.cpu(), torch.from_numpy(want).float().to(TYPES[t]))
+
+
+@pytest.mark.parametrize("M", [1, 16, 20, 33, 48, 60, 130])
+def test_gemm_and_linear_of_a_vocabulary(dev, M):
+    """Far more outputs than workgroups (131072 and over: every wave has columns of its own), few and many rows."""
+    rng = np.random.default_rng(M)
+    N, K = 131072 + 77, 260
+    w = integer_rows(rng, 1000, K, dev)
+    w = hip.Fp8Rows(w.q.repeat(132, 1)[:N].contiguous(), w.scale.repeat(1, 132)[:, :N].contiguous(), K)
+    x = torch.randint(-3, 4, (M, K), generator=torch.Generator().manual_seed(M)).float()
+    x[:, ::128] = 448.0                                      # the scale of every block is 1: the small integers stay what they are
+    want = torch.from_numpy(np.tile(np_(x) @ values(hip.Fp8Rows(w.q[:1000].contiguous(), w.scale[:, :1000].contiguous(), K))[:, :K].T, (1, 132))[:, :N])
+    for got in (hip.linear_fp8(x.to(dev), w), hip.gemm_fp8(hip.quant_fp8(x.to(dev)), w, out_dtype=torch.float32)):
+        assert torch.equal(got.double().cpu(), want)
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
