@@ -353,7 +353,9 @@ int cube_label_score(const void* hl, const void* hl_lo, int ld_hl, int col_x2, i
  *             q[b, k*ld_tap + :]) (Conv1d(k=taps) over [query | encoder_output] with the query
  *             constant along the word, e_enc = the encoder part + bias, computed once per batch);
  *             att = softmax over all S positions; x[b, col_ctx..+C) = sum_t att[t] * enc[b*S+t, 0..C).
- * enc, char_emb, x: bf16 hi (+ lo) planes.  S <= 256, P <= 128, C <= 512, C % 8 == 0.              */
+ * enc, char_emb, x: bf16 hi (+ lo) planes.  S <= 256, P <= 128, C <= 512, C % 8 == 0.
+ * pick (may be NULL): int32 [B], the previous step's characters where they were chosen otherwise (cube_sample_rows); they take the
+ * place of the arg-max, and what lies outside [0, n_char) counts as `eol`.  The case stays the arg-max.                */
 typedef struct cube_lemma_attend_args {
   const float* q; int ld_q; int taps; int P; int ld_tap;
   int col_char; int n_char; int col_case; int n_case;
@@ -365,6 +367,7 @@ typedef struct cube_lemma_attend_args {
   int step; int attend;
   int32_t* out_char; int32_t* out_case; int ld_out;
   int eol; int32_t* done; int32_t* n_done;
+  const int32_t* pick;
 } cube_lemma_attend_args;
 int cube_lemma_attend(const cube_lemma_attend_args* args, void* stream);
 

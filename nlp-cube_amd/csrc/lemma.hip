@@ -50,7 +50,13 @@ __global__ __launch_bounds__(256) void lemma_attend_kernel(cube_lemma_attend_arg
   uint16_t* xrow = (uint16_t*)a.x + (size_t)b * a.ld_x;
   uint16_t* xrow_lo = a.x_lo ? (uint16_t*)a.x_lo + (size_t)b * a.ld_x : nullptr;
   if (a.step > 0) {
-    const int ch = wave_argmax(q + a.col_char, a.n_char, lane);
+    int ch;
+    if (a.pick) {
+      ch = a.pick[b];
+      if (ch < 0 || ch >= a.n_char) ch = a.eol;
+    } else {
+      ch = wave_argmax(q + a.col_char, a.n_char, lane);
+    }
     const int cs = wave_argmax(q + a.col_case, a.n_case, lane);
     if (lane == 0) {
       a.out_char[(size_t)b * a.ld_out + a.step - 1] = ch;
@@ -200,8 +206,8 @@ extern "C" int cube_lemma_attend(const cube_lemma_attend_args* a, void* stream) 
     if (!a->out_char || !a->out_case || !a->done || !a->n_done || !a->char_emb || a->step > a->ld_out)
       CUBE_FAIL(CUBE_ERR_ARG, "cube_lemma_attend: step %d needs out_char/out_case [B, ld_out >= step], done, n_done, char_emb", a->step);
     if (a->n_char <= 0 || a->n_case <= 0 || a->col_char < 0 || a->col_case < 0 || a->col_char + a->n_char > a->ld_q ||
-        a->col_case + a->n_case > a->ld_q || a->ld_emb < a->E)
-      CUBE_FAIL(CUBE_ERR_ARG, "cube_lemma_attend: logits columns outside q / embedding table too narrow");
+        a->col_case + a->n_case > a->ld_q || a->ld_emb < a->E || (a->pick && (a->eol < 0 || a->eol >= a->n_char)))
+      CUBE_FAIL(CUBE_ERR_ARG, "cube_lemma_attend: logits columns outside q / embedding table too narrow / eol outside the characters");
   }
   if (a->attend) {
     if (!a->v || !a->e_enc || !a->enc) CUBE_FAIL(CUBE_ERR_ARG, "cube_lemma_attend: null v / e_enc / enc");

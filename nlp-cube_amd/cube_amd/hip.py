@@ -75,6 +75,7 @@ class LemmaAttendArgs(ctypes.Structure):
         ("step", c_int), ("attend", c_int),
         ("out_char", c_void_p), ("out_case", c_void_p), ("ld_out", c_int),
         ("eol", c_int), ("done", c_void_p), ("n_done", c_void_p),
+        ("pick", c_void_p),
     ]
 
 

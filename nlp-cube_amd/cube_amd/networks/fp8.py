@@ -1,0 +1,52 @@
+"""nn.Linear in 8-bit floating point (`cube_linear_fp8`): weights quantised once, rows on the way.  For the Linear layers of a
+transformer that runs beside the parser (the LM encoder of cube/networks/lm.py:121-211 is one); inference only."""
+import torch
+
+from cube_amd import hip
+
+
+class Fp8Linear(torch.nn.Module):
+    """Stands for `linear` (same call, same shapes, the input's type out): e4m3 weights with one power-of-two scale per row and 128
+    columns, activations quantised the same way per call, fp32 sums.  Made on the device of `linear`'s weight, an MI355X."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        rows = hip.quant_fp8(linear.weight.detach())
+        self.register_buffer("q", rows.q)
+        self.register_buffer("scale", rows.scale)
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float())
+        self._rows = rows
+
+    def _apply(self, fn, *args, **kwargs):
+        bias = self.bias
+        super()._apply(fn, *args, **kwargs)
+        if bias is not None:
+            self.bias = bias.to(self.q.device)   # .half() and the like round it: what is added to the sums stays fp32
+        self._rows = hip.Fp8Rows(self.q, self.scale, self.in_features)
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._rows = hip.Fp8Rows(self.q, self.scale, self.in_features)
+
+    def forward(self, x):
+        rows = x.reshape(-1, self.in_features)
+        if rows.stride(1) != 1 or rows.stride(0) < self.in_features:   # transposed or broadcast rows
+            rows = rows.contiguous()
+        y = hip.linear_fp8(rows, self._rows, self.bias)
+        return y.reshape(x.shape[:-1] + (self.out_features,))
+
+    def extra_repr(self):
+        return "in_features=%d, out_features=%d, bias=%s" % (self.in_features, self.out_features, self.bias is not None)
+
+
+def quantise_linears(module):
+    """Every nn.Linear below `module` (itself excepted) -> Fp8Linear, in place.  -> how many."""
+    n = 0
+    for parent in list(module.modules()):
+        for name, child in list(parent.named_children()):
+            if type(child) is torch.nn.Linear:
+                setattr(parent, name, Fp8Linear(child))
+                n += 1
+    return n

@@ -223,8 +223,9 @@ class Lemmatizer:
         return dict(B=B, S=S, enc=enc, e_enc=e_enc, ld_e=ae["N"], _ints=ints)
 
     @hip.on_device
-    def _decode(self, ed, max_steps=None, keep_logits=False, defer=False):
-        """Greedy decoding (lemmatizer.py:126-169).  -> (out_char i32 [B, n], out_case i32 [B, n], n, logits)
+    def _decode(self, ed, max_steps=None, keep_logits=False, defer=False, sampling=None):
+        """Greedy decoding (lemmatizer.py:126-169), or with `sampling` (networks/sampling.py) characters drawn from the same logits
+        (cube_sample_rows; the end symbol among them, the start symbol not), the case greedy as before.  -> (out_char i32 [B, n], out_case i32 [B, n], n, logits)
         with n = the number of steps the reference would have run.  defer: everything is enqueued, the arg-max arrays are
         written to pinned memory by a kernel (cube_copy_to_pinned) and a handle for `_decode_finish` is returned instead, so
         that the caller can featurise and enqueue the NEXT batch before it waits for this one."""
@@ -285,6 +286,15 @@ class Lemmatizer:
         a.ld_x, a.col_ctx, a.col_emb = ld_x, 0, lay.xd_emb
         a.out_char, a.out_case, a.ld_out = out[0].data_ptr(), out[1].data_ptr(), out.shape[2]
         a.eol, a.done, a.n_done = self._eol, flags.data_ptr(), flags[B:].data_ptr()
+        if sampling is not None:
+            pick = torch.empty(B, dtype=torch.int32, device=dev)
+            V = self._eol + 1
+            n_ws = lib.cube_sample_workspace_bytes(0, B, V)
+            draw_ws = torch.empty(n_ws, dtype=torch.uint8, device=dev) if n_ws else None
+            draw = hip.SampleArgs(q.data_ptr() + 4 * lay.q_char, 0, ld_q, B, V, None, None, None, None, None, sampling.temperature,
+                                  min(sampling.top_k, 0x7fffffff), sampling.top_p, sampling.min_p, pick.data_ptr(), None)
+            uniforms = None   # drawn for CHECK_EVERY steps at a time
+            self._live += [pick, draw_ws]
 
         # start frame through the decoder with a zero state (lemmatizer.py:128-131)
         cur = 0
@@ -303,6 +313,15 @@ class Lemmatizer:
                 logits[s - 1].copy_(q[:B * ld_q].view(B, ld_q)[:, lay.q_char:lay.q_char + lay.n_char + lay.n_case])
             if fused:
                 cur = 1 - cur   # context and the chosen character's embedding go into the NEXT step's input row
+            if sampling is not None and s > 0:
+                k = (s - 1) % self.CHECK_EVERY
+                if k == 0:
+                    uniforms = sampling.uniforms(self.CHECK_EVERY, B, dev)
+                    if keep_logits:
+                        ed.setdefault("uniforms", []).append(uniforms)
+                draw.u = uniforms[k].data_ptr()
+                hip.check(lib.cube_sample_rows(ctypes.byref(draw), lo(draw_ws), n_ws, st), "cube_sample_rows")
+                a.pick = pick.data_ptr()
             a.x, a.x_lo = X[cur].hi.data_ptr(), lo(X[cur].lo)
             a.step, a.attend = s, int(s < limit)
             hip.check(lib.cube_lemma_attend(ctypes.byref(a), st), "cube_lemma_attend")
@@ -359,14 +378,14 @@ class Lemmatizer:
         return logits[:, :, :self._lay.n_char], logits[:, :, self._lay.n_char:]
 
     @hip.on_device
-    def decode_batch(self, X):
-        """-> (chars int32 [B, n], cases int32 [B, n]) arg-max sequences (NumPy), no logits kept."""
+    def decode_batch(self, X, sampling=None):
+        """-> (chars int32 [B, n], cases int32 [B, n]) arg-max (or, with `sampling`, drawn) sequences (NumPy), no logits kept."""
         self._require_gpu()
-        oc, ok, _, _ = self._decode(self._encode(X), max_steps=self.max_steps)
+        oc, ok, _, _ = self._decode(self._encode(X), max_steps=self.max_steps, sampling=sampling)
         return oc, ok
 
     @hip.on_device
-    def _decode_batches(self, batches, collate):
+    def _decode_batches(self, batches, collate, sampling=None):
         """batches: iterable of lists of items for `collate`.  Yields (index, lemma strings) per batch, in order, with the
         host work of neighbouring batches (collate of the next, strings of the previous) under the device's decode."""
         def finish(k, h):
@@ -378,7 +397,7 @@ class Lemmatizer:
             batch = collate.collate_fn(items, targets=False) if isinstance(collate, Word2TargetCollate) else collate.collate_fn(items)
             batch.pop("y_char", None)
             batch.pop("y_case", None)
-            h = self._decode(self._encode(batch), max_steps=self.max_steps, defer=True)
+            h = self._decode(self._encode(batch), max_steps=self.max_steps, defer=True, sampling=sampling)
             if pending is not None:
                 yield finish(*pending)
             pending = (k, h)
@@ -482,8 +501,10 @@ class Lemmatizer:
         return doc
 
     @hip.on_device
-    def process(self, doc, collate, batch_size=4, num_workers=4, merge=True, max_words=8192):
+    def process(self, doc, collate, batch_size=4, num_workers=4, merge=True, max_words=8192, sampling=None):
         """reference: lemmatizer.py:185-231.  `num_workers` is accepted and ignored.
+        sampling (no counterpart in the reference): a `networks.sampling.Sampling`; the lemmas are drawn instead of decoded
+        greedily -- alternatives for an ambiguous word, one call each.
         merge (no counterpart in the reference, results unchanged): the reference's in-order batches of
         `batch_size` words whose longest word has the same length (same S, hence the same pad positions
         for every word in them) run together as one device batch of up to `max_words` words; words do not
@@ -500,7 +521,7 @@ class Lemmatizer:
         else:
             device_batches = [list(range(a, min(a + batch_size, n))) for a in starts]
         all_lemmas = [None] * n
-        for b, lemmas in self._decode_batches(([dataset[i] for i in ids] for ids in device_batches), collate):
+        for b, lemmas in self._decode_batches(([dataset[i] for i in ids] for ids in device_batches), collate, sampling):
             for i, lemma in zip(device_batches[b], lemmas):
                 all_lemmas[i] = lemma
         i = 0

@@ -85,10 +85,13 @@ class LMHelperHF:
     model: a name / local directory for `transformers.AutoTokenizer` / `AutoModel` as in the reference (lm.py:122-129;
     offline only a local directory can work), or omit it and pass the two objects: `splitter(word)['input_ids']` =
     [start] + pieces + [end] (lm.py:155), `encoder(ids, return_dict=True)['hidden_states']` = K tensors
-    [sentences, pieces, E] (lm.py:178-179)."""
+    [sentences, pieces, E] (lm.py:178-179).
+
+    fp8 (no counterpart in the reference): the encoder's nn.Linear layers run in 8-bit floating point (networks/fp8.py); the encoder
+    is changed in place."""
     START, PAD, END = 0, 1, 2   # lm.py:147-149
 
-    def __init__(self, device="cuda:0", model=None, splitter=None, encoder=None):
+    def __init__(self, device="cuda:0", model=None, splitter=None, encoder=None, fp8=False):
         import torch
         from cube_amd import hip
         self._device = torch.device(device)
@@ -104,6 +107,10 @@ class LMHelperHF:
         self._xlmr = encoder
         self._xlmr.eval()
         self._xlmr.to(self._device)
+        if fp8:
+            from cube_amd.networks.fp8 import quantise_linears
+            with torch.cuda.device(self._device):
+                quantise_linears(self._xlmr)
         with torch.no_grad():
             tmp = self._xlmr(torch.tensor([[100]], device=self._device), return_dict=True)  # lm.py:133-135
         hs = tmp["hidden_states"]
