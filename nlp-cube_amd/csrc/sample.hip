@@ -22,6 +22,8 @@
 //   half    16-bit logits have 65536 values: a workgroup counts every value of a row (or of a slice of it) in LDS, and everything
 //           is decided from the counts, with one exponential for each value that occurs;
 //   long    f32: slices of a row meet in a histogram and in a list of the few logits that can still decide.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/cube_hip.h"
 
@@ -1553,12 +1555,14 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
   return CUBE_OK;
 }
 
-constexpr int HALF_V = 8192;  // 16-bit rows longer than this are counted by value
+// 16-bit rows longer than this are counted by value (top-p, us: bf16 64 x 16000 16 against 19, 256 x 32000 19 against 33;  f16 has eight
+// times as many values to an octave, so it pays later: 256 x 32000 44 against 33)
+template <class T> constexpr int half_v() { return std::is_same<T, bf16_t>::value ? 16000 : MID_V; }
 
 template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStream_t st) {
   if (a.V <= SHORT_V) return launch_short<T>(a, S, st);
   if constexpr (sizeof(T) == 2) {
-    if (a.V > HALF_V) return launch_half<T>(a, S, (HalfSlice*)ws, st);
+    if (a.V > half_v<T>()) return launch_half<T>(a, S, (HalfSlice*)ws, st);
   } else {
     if (a.V > MID_V) return launch_long(a, S, (LongRow*)ws, st);
   }
@@ -1571,7 +1575,7 @@ template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStr
 extern "C" size_t cube_sample_workspace_bytes(int type, int M, int V) {
   if (M <= 0 || V <= 0 || V > CUBE_SAMPLE_MAX_V) return 0;
   if (type == CUBE_T_F32) return V > MID_V ? sizeof(LongRow) * (size_t)(M < ROWS_AT_ONCE ? M : ROWS_AT_ONCE) : 0;
-  if (V <= HALF_V) return 0;
+  if (V <= (type == CUBE_T_BF16 ? half_v<bf16_t>() : half_v<_Float16>())) return 0;
   const HalfPlan p = half_plan(M, V);
   return p.slices > 1 ? sizeof(HalfSlice) * (size_t)p.slices * p.rows : 0;
 }
