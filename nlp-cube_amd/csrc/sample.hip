@@ -710,22 +710,36 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
 
 // ---- half: 16-bit logits by the counts of their values ----------------------------------------------------------------------
 // A slice's counts: one 32-bit word per magnitude (the 15 bits without the sign), the number of its logits in the low half and
-// of its negative ones in the high half; a slice has at most 65528 logits, so neither runs over.  Groups of 128 magnitudes (an
-// octave of bf16).  In the candidates' order group g comes 255 - g-th for positive values, falling inside, and 256 + g-th for
-// negative ones, rising.
+// of its negative ones in the high half; a slice has at most 65528 logits, so neither runs over.  Groups of 64 * E magnitudes, E
+// to a lane: an octave of bf16, half an octave of f16 (quarters of that took 65 us where these take 38, 1 x 250002: a row then has 130 groups).
+// In the candidates' order group g comes GROUPS - 1 - g-th for positive values, falling inside, and GROUPS + g-th for negative
+// ones, rising.
 constexpr int HWG = 1024;
-constexpr int MAGS = 32768, GROUP = 128, GROUPS = MAGS / GROUP;
+constexpr int MAGS = 32768;
+constexpr int MAX_GROUPS = 256;
 constexpr int HALF_GRANULES = 8191;  // of 8 logits, per slice
+
+template <class T> struct Half;
+template <> struct Half<bf16_t> { static constexpr uint32_t INF = 0x7f80; static constexpr int E = 2; };
+template <> struct Half<_Float16> { static constexpr uint32_t INF = 0x7c00; static constexpr int E = 8; };
+template <class T> constexpr int half_groups() { return MAGS / (64 * Half<T>::E); }
+template <class T> __device__ __forceinline__ float half_value(uint32_t raw) { return as_float(__builtin_bit_cast(T, (uint16_t)raw)); }
 
 struct HalfSlice {  // of the workspace: the counts of the groups that `has` marks
   uint32_t count[MAGS];
-  uint64_t has[GROUPS / 64];
+  uint64_t has[MAX_GROUPS / 64];
 };
 
-template <class T> struct Half;
-template <> struct Half<bf16_t> { static constexpr uint32_t INF = 0x7f80; };
-template <> struct Half<_Float16> { static constexpr uint32_t INF = 0x7c00; };
-template <class T> __device__ __forceinline__ float half_value(uint32_t raw) { return as_float(__builtin_bit_cast(T, (uint16_t)raw)); }
+// E neighbouring words
+template <int E> struct Words { uint32_t v[E]; };
+__device__ __forceinline__ Words<2> load_words(const uint32_t* p, Words<2>) {
+  const uint2 c = *(const uint2*)p;
+  return {{c.x, c.y}};
+}
+__device__ __forceinline__ Words<8> load_words(const uint32_t* p, Words<8>) {
+  const uint4 a = *(const uint4*)p, b = *(const uint4*)(p + 4);
+  return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
 
 // the raw 16-byte granules of a row; f(word) for the two logits of each 32-bit word, whole granules only, and g(raw) for the rest
 template <class T, class F, class G> __device__ __forceinline__ void half_words(const Row<T>& row, int lo, int hi, F f, G g) {
@@ -749,121 +763,159 @@ template <class T> __device__ void count_half(uint32_t* count, const Row<T>& row
   half_words(row, lo, hi, [&](uint32_t w) { one(w & 0xffffu); one(w >> 16); }, one);
   __syncthreads();
 }
+// marks of the groups that have a logit, a wave its own run of groups: into part (LDS), then has[0 .. GROUPS / 64); f(group, words) for
+// each marked one
+template <class T, class F> __device__ void mark_half(const uint32_t* count, uint32_t* part, uint64_t* has, F f) {
+  constexpr int E = Half<T>::E, G = half_groups<T>() / (HWG / 64), WAVES = 64 / G;  // groups of a wave, waves of a word of `has`
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t mask = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int group = wave * G + g;
+    const Words<E> c = load_words(count + (group * 64 + lane) * E, Words<E>{});
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) any |= c.v[i];
+    if (__ballot(any != 0)) {
+      mask |= 1u << g;
+      f(group, c);
+    }
+  }
+  if (lane == 0) part[wave] = mask;
+  __syncthreads();
+  if (threadIdx.x < half_groups<T>() / 64) {
+    uint64_t h = 0;
+    for (int i = 0; i < WAVES; ++i) h |= (uint64_t)part[WAVES * threadIdx.x + i] << (G * i);
+    has[threadIdx.x] = h;
+  }
+}
 
 template <class T>
 __global__ __launch_bounds__(HWG) void half_count_kernel(cube_sample_args a, int r0, HalfSlice* ws, int per) {
   extern __shared__ __attribute__((aligned(16))) uint32_t count[];
-  const int r = r0 + blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ uint32_t part[HWG / 64];
+  constexpr int E = Half<T>::E;
+  const int r = r0 + blockIdx.y, lane = threadIdx.x & 63;
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   HalfSlice& out = ws[(size_t)blockIdx.y * gridDim.x + blockIdx.x];
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   count_half(count, row, lo, hi);
-  __shared__ uint32_t any[HWG / 64];
-  constexpr int G = GROUPS / (HWG / 64);  // a wave's groups
-  uint32_t mask = 0;
+  mark_half<T>(count, part, out.has, [&](int group, const Words<E>& c) {
+    uint32_t* to = out.count + (group * 64 + lane) * E;
+    if constexpr (E == 2) {
+      *(uint2*)to = make_uint2(c.v[0], c.v[1]);
+    } else {
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int at = (wave * G + g) * (GROUP / 2) + lane;
-    const uint2 c = ((const uint2*)count)[at];
-    if (__ballot((c.x | c.y) != 0)) {
-      mask |= 1u << g;
-      ((uint2*)out.count)[at] = c;
+      for (int i = 0; i < E; i += 4) *(uint4*)(to + i) = make_uint4(c.v[i], c.v[i + 1], c.v[i + 2], c.v[i + 3]);
     }
-  }
-  static_assert(G == 16, "four waves' masks make one word of `has`");
-  if (lane == 0) any[wave] = mask;
-  __syncthreads();
-  if (threadIdx.x < GROUPS / 64) {
-    uint64_t h = 0;
-    for (int i = 0; i < 4; ++i) h |= (uint64_t)any[4 * threadIdx.x + i] << (16 * i);
-    out.has[threadIdx.x] = h;
-  }
+  });
 }
 
 struct HalfScratch {  // in LDS
-  uint64_t weight[2 * GROUPS];  // by order; after prefix_half: running sums
-  uint32_t count[2 * GROUPS];
-  uint64_t has[GROUPS / 64];
+  uint64_t weight[2 * MAX_GROUPS];  // by order; after prefix_half: running sums
+  uint32_t count[2 * MAX_GROUPS];
+  uint64_t has[MAX_GROUPS / 64];
   uint64_t heavy;
   uint32_t raw, tie, ties, slice;
   float prob;
   uint32_t part[HWG / 64];
 };
 
-// Counts of the two neighbouring magnitudes 2 * lane, 2 * lane + 1 of a group: all and negative.  From LDS, or summed over the slices
-// of the workspace (and kept in LDS for the groups of the first SLOTS marks: a search comes back to a group).
-struct Pair2 { uint32_t all[2], neg[2]; };
-struct LdsCounts {
+// Counts of a lane's E neighbouring magnitudes of a group: all and negative.  From LDS, or summed over the slices of the workspace
+// (and kept in LDS for the groups of the first SLOTS marks: a search comes back to a group).
+template <int E> struct Counts { uint32_t all[E], neg[E]; };
+template <class T> struct LdsCounts {
+  static constexpr int E = Half<T>::E;
   const uint32_t* count;
-  __device__ __forceinline__ Pair2 load(int g) const {
-    const uint2 c = ((const uint2*)count)[g * (GROUP / 2) + (threadIdx.x & 63)];
-    return {{c.x & 0xffffu, c.y & 0xffffu}, {c.x >> 16, c.y >> 16}};
+  __device__ __forceinline__ Counts<E> load(int g) const {
+    const Words<E> c = load_words(count + (g * 64 + (threadIdx.x & 63)) * E, Words<E>{});
+    Counts<E> r;
+#pragma unroll
+    for (int i = 0; i < E; ++i) { r.all[i] = c.v[i] & 0xffffu; r.neg[i] = c.v[i] >> 16; }
+    return r;
   }
-  __device__ __forceinline__ Pair2 again(const HalfScratch&, int g) const { return load(g); }
-  __device__ __forceinline__ void keep(const HalfScratch&, int, const Pair2&) const {}
+  __device__ __forceinline__ Counts<E> again(const HalfScratch&, int g) const { return load(g); }
+  __device__ __forceinline__ void keep(const HalfScratch&, int, const Counts<E>&) const {}
 };
 constexpr int HALF_SLICES = 96;  // of a row, at most: 65 cover 2^22 logits
-constexpr int SLOTS = 128;
-struct SliceCounts {
+constexpr int KEPT_BYTES = 128 * 1024;
+template <class T> struct SliceCounts {
+  static constexpr int E = Half<T>::E, SLOTS = KEPT_BYTES / (64 * E * 8), BATCH = 32 / E;
   const HalfSlice* slice; int n;
-  const uint64_t (*has)[GROUPS / 64];  // of every slice, in LDS
-  uint4* kept;                         // [SLOTS][64], in LDS
+  const uint64_t (*has)[MAX_GROUPS / 64];  // of every slice, in LDS
+  uint32_t* kept;                          // [SLOTS][2 * E][64], in LDS
   __device__ __forceinline__ int slot(const HalfScratch& s, int g) const {  // marked groups before g
     int r = 0;
     for (int i = 0; i < (g >> 6); ++i) r += __popcll(s.has[i]);
     return r + __popcll(s.has[g >> 6] & ((1ull << (g & 63)) - 1));
   }
-  __device__ __forceinline__ Pair2 load(int g) const {
-    const int lane = threadIdx.x & 63, at = g * (GROUP / 2) + lane;
-    Pair2 r = {{0, 0}, {0, 0}};
+  __device__ __forceinline__ Counts<E> load(int g) const {
+    const int lane = threadIdx.x & 63, at = (g * 64 + lane) * E;
+    Counts<E> r;
+#pragma unroll
+    for (int i = 0; i < E; ++i) r.all[i] = r.neg[i] = 0;
     for (int i0 = 0; i0 < n; i0 += 64) {
       uint64_t left = __ballot(i0 + lane < n && ((has[i0 + lane < n ? i0 + lane : i0][g >> 6] >> (g & 63)) & 1));
-      while (left) {  // sixteen slices' loads at a time
-        uint2 c[16];
+      while (left) {  // several slices' loads at a time
+        Words<E> c[BATCH];
 #pragma unroll
-        for (int u = 0; u < 16; ++u) {
-          c[u] = make_uint2(0, 0);
+        for (int u = 0; u < BATCH; ++u) {
+          c[u] = {};
           if (left) {
-            c[u] = ((const uint2*)slice[i0 + __ffsll((long long)left) - 1].count)[at];
+            c[u] = load_words(slice[i0 + __ffsll((long long)left) - 1].count + at, Words<E>{});
             left &= left - 1;
           }
         }
 #pragma unroll
-        for (int u = 0; u < 16; ++u) {
-          r.all[0] += c[u].x & 0xffffu; r.neg[0] += c[u].x >> 16; r.all[1] += c[u].y & 0xffffu; r.neg[1] += c[u].y >> 16;
-        }
+        for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+          for (int i = 0; i < E; ++i) { r.all[i] += c[u].v[i] & 0xffffu; r.neg[i] += c[u].v[i] >> 16; }
       }
     }
     return r;
   }
-  __device__ __forceinline__ void keep(const HalfScratch& s, int g, const Pair2& c) const {
+  __device__ __forceinline__ void keep(const HalfScratch& s, int g, const Counts<E>& c) const {
     const int at = slot(s, g);
-    if (at < SLOTS) kept[at * 64 + (threadIdx.x & 63)] = make_uint4(c.all[0], c.all[1], c.neg[0], c.neg[1]);
+    if (at >= SLOTS) return;
+    uint32_t* to = kept + at * 2 * E * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int i = 0; i < E; ++i) { to[2 * i * 64] = c.all[i]; to[(2 * i + 1) * 64] = c.neg[i]; }
   }
-  __device__ __forceinline__ Pair2 again(const HalfScratch& s, int g) const {
+  __device__ __forceinline__ Counts<E> again(const HalfScratch& s, int g) const {
     const int at = slot(s, g);
     if (at >= SLOTS) return load(g);
-    const uint4 c = kept[at * 64 + (threadIdx.x & 63)];
-    return {{c.x, c.y}, {c.z, c.w}};
+    const uint32_t* from = kept + at * 2 * E * 64 + (threadIdx.x & 63);
+    Counts<E> r;
+#pragma unroll
+    for (int i = 0; i < E; ++i) { r.all[i] = from[2 * i * 64]; r.neg[i] = from[(2 * i + 1) * 64]; }
+    return r;
   }
 };
+template <class T> __device__ __forceinline__ uint32_t half_raw(int g, bool neg, int i) {
+  return (uint32_t)((g * 64 + ((int)threadIdx.x & 63)) * Half<T>::E + i) | (neg ? 0x8000u : 0u);
+}
 // the candidates among them: negative counts for `neg` (below the infinity), positive ones else (up to it; zero takes both signs)
-template <class T> __device__ __forceinline__ void valid2(int g, bool neg, const Pair2& p, uint32_t (&c)[2]) {
+template <class T> __device__ __forceinline__ void valid(int g, bool neg, const Counts<Half<T>::E>& p, uint32_t (&c)[Half<T>::E]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t mag = (uint32_t)(g * GROUP + 2 * (threadIdx.x & 63) + i);
+  for (int i = 0; i < Half<T>::E; ++i) {
+    const uint32_t mag = half_raw<T>(g, false, i);
     if (neg) c[i] = mag != 0 && mag < Half<T>::INF ? p.neg[i] : 0;
     else c[i] = mag == 0 ? p.all[i] : mag <= Half<T>::INF ? p.all[i] - p.neg[i] : 0;
   }
 }
-__device__ __forceinline__ uint32_t half_raw(int g, bool neg, int i) {
-  return (uint32_t)(g * GROUP + 2 * ((int)threadIdx.x & 63) + i) | (neg ? 0x8000u : 0u);
+template <int E> __device__ __forceinline__ uint32_t sum_of(const uint32_t (&c)[E]) {
+  uint32_t s = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) s += c[i];
+  return s;
 }
-__device__ __forceinline__ int group_of(int order) { return order < GROUPS ? GROUPS - 1 - order : order - GROUPS; }
+template <class T> __device__ __forceinline__ int group_of(int order) {
+  return order < half_groups<T>() ? half_groups<T>() - 1 - order : order - half_groups<T>();
+}
 
 // One wave: counts and weights by order become running sums
-__device__ __forceinline__ void prefix_half(HalfScratch& s) {
-  constexpr int R = 2 * GROUPS / 64;
+template <class T> __device__ __forceinline__ void prefix_half(HalfScratch& s) {
+  constexpr int R = 2 * half_groups<T>() / 64;
   const int lane = threadIdx.x & 63;
   uint32_t c[R], cs = 0;
   uint64_t w[R], ws = 0;
@@ -889,37 +941,39 @@ struct Spot { uint32_t raw, tie, ties; uint64_t before, one; __device__ uint64_t
 // One wave: the value at which the running count (BY_COUNT) or weight passes target (the total does); before, one: weights
 template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfScratch& s, const C& counts, const Weigher& w, uint64_t target) {
   const int lane = threadIdx.x & 63;
-  constexpr int R = 2 * GROUPS / 64;
+  constexpr int E = Half<T>::E, R = 2 * half_groups<T>() / 64;
   // 64 running sums, R apart, then the R between them
   auto sum = [&](int i) { return BY_COUNT ? (uint64_t)s.count[i] : s.weight[i]; };
   int order = R * (__ffsll(__ballot(target < sum(lane * R + R - 1))) - 1);
   order += __ffsll(__ballot(lane < R && target < sum(order + (lane < R ? lane : 0)))) - 1;
   uint64_t bc = order > 0 ? s.count[order - 1] : 0, bw = order > 0 ? s.weight[order - 1] : 0;
-  const bool neg = order >= GROUPS;
-  const int g = group_of(order);
-  uint32_t c[2];
-  valid2<T>(g, neg, counts.again(s, g), c);
-  uint64_t v[2];
+  const bool neg = order >= half_groups<T>();
+  const int g = group_of<T>(order);
+  uint32_t c[E];
+  valid<T>(g, neg, counts.again(s, g), c);
+  uint64_t v[E], sw = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) v[i] = c[i] ? (uint64_t)c[i] * w.of(half_value<T>(half_raw(g, neg, i))) : 0;
+  for (int i = 0; i < E; ++i) {
+    v[i] = c[i] ? (uint64_t)c[i] * w.of(half_value<T>(half_raw<T>(g, neg, i))) : 0;
+    sw += v[i];
+  }
   // in falling order: negative values as they lie, positive ones from the other end
-  const uint32_t sc = c[0] + c[1], ic = wave_scan(sc);
-  const uint64_t sw = v[0] + v[1], iw = wave_scan(sw);
+  const uint32_t sc = sum_of(c), ic = wave_scan(sc);
+  const uint64_t iw = wave_scan(sw);
   bc += neg ? ic - sc : lane_value(ic, 63) - ic;
   bw += neg ? iw - sw : lane_value(iw, 63) - iw;
   Spot out = {0, 0, 0, 0, 0};
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = neg ? j : 1 - j;
-    const uint32_t ci = i ? c[1] : c[0];
-    const uint64_t vi = i ? v[1] : v[0];
+  for (int j = 0; j < E; ++j) {
+    const uint32_t ci = neg ? c[j] : c[E - 1 - j];
+    const uint64_t vi = neg ? v[j] : v[E - 1 - j];
     const uint64_t here = BY_COUNT ? bc : bw, mine = BY_COUNT ? ci : vi;
     if (here <= target && target < here + mine) {
-      out.raw = half_raw(g, neg, i);
-      out.one = vi / ci;
-      out.tie = (uint32_t)((target - here) / (BY_COUNT ? 1 : out.one));
+      out.raw = half_raw<T>(g, neg, neg ? j : E - 1 - j);
       out.ties = ci;
       out.before = bw;
+      out.one = vi;   // (of all of them; divided below)
+      out.tie = BY_COUNT ? (uint32_t)(target - here) : 0;
     }
     bc += ci;
     bw += vi;
@@ -929,14 +983,15 @@ template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfS
   out.tie = lane_value(out.tie, owner);
   out.ties = lane_value(out.ties, owner);
   out.before = lane_value(out.before, owner);
-  out.one = lane_value(out.one, owner);
+  out.one = w.of(half_value<T>(out.raw));
+  if (!BY_COUNT) out.tie = (uint32_t)((target - out.before) / out.one);
   return out;
 }
 
 // The workgroup's decision for a row from its counts (s.has filled): s.raw, s.tie, s.ties, s.prob; false for an empty row.
 template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C& counts, const Settings& st, int V, int S) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int R = 2 * GROUPS / 64;
+  constexpr int E = Half<T>::E, GROUPS = half_groups<T>(), R = 2 * GROUPS / 64;
   for (int i = threadIdx.x; i < 2 * GROUPS; i += HWG) { s.weight[i] = 0; s.count[i] = 0; }
   if (threadIdx.x == 0) s.heavy = 0;
   __syncthreads();
@@ -948,12 +1003,12 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
         if (turn++ % (HWG / 64) == wave) f(64 * word + __ffsll((long long)left) - 1);
   };
   groups([&](int g) {
-    const Pair2 p = counts.load(g);
+    const Counts<E> p = counts.load(g);
     counts.keep(s, g, p);
-    uint32_t pos[2], neg[2];
-    valid2<T>(g, false, p, pos);
-    valid2<T>(g, true, p, neg);
-    const uint32_t np = wave_sum(pos[0] + pos[1]), nn = wave_sum(neg[0] + neg[1]);
+    uint32_t pos[E], neg[E];
+    valid<T>(g, false, p, pos);
+    valid<T>(g, true, p, neg);
+    const uint32_t np = wave_sum(sum_of(pos)), nn = wave_sum(sum_of(neg));
     if (lane == 0) { s.count[GROUPS - 1 - g] = np; s.count[GROUPS + g] = nn; }
   });
   __syncthreads();
@@ -964,25 +1019,31 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
   const unsigned long long some = __ballot(first < 2 * GROUPS);
   if (!some) return false;
   const int order = (int)lane_value(first, __ffsll(some) - 1);
-  uint32_t c[2];
-  valid2<T>(group_of(order), order >= GROUPS, counts.again(s, group_of(order)), c);
-  const unsigned long long hit = __ballot((c[0] | c[1]) != 0);
-  const int at = order < GROUPS ? 63 - __clzll((long long)hit) : __ffsll(hit) - 1;
-  const uint32_t mine = half_raw(group_of(order), order >= GROUPS, order < GROUPS ? (c[1] ? 1 : 0) : (c[0] ? 0 : 1));
+  const bool below = order >= GROUPS;
+  uint32_t c[E], mine = 0;
+  valid<T>(group_of<T>(order), below, counts.again(s, group_of<T>(order)), c);
+#pragma unroll
+  for (int j = 0; j < E; ++j) {  // of a lane's own the largest: the first of the negative ones, the last of the others
+    const int i = below ? E - 1 - j : j;
+    mine = (below ? c[E - 1 - j] : c[j]) ? half_raw<T>(group_of<T>(order), below, i) : mine;
+  }
+  const unsigned long long hit = __ballot(sum_of(c) != 0);
+  const int at = below ? __ffsll(hit) - 1 : 63 - __clzll((long long)hit);
   const Weigher w(st, half_value<T>(lane_value(mine, at)), S);
   const bool greedy = st.greedy();
   if (!greedy) {
     groups([&](int g) {
-      const Pair2 p = counts.again(s, g);
+      const Counts<E> p = counts.again(s, g);
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
-        uint32_t c[2];
-        valid2<T>(g, side != 0, p, c);
-        if (!__ballot((c[0] | c[1]) != 0)) continue;
+        uint32_t c[E];
+        valid<T>(g, side != 0, p, c);
+        if (!__ballot(sum_of(c) != 0)) continue;
         uint64_t sum = 0, heavy = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const double x = w.x(half_value<T>(half_raw(g, side != 0, i)));
+        for (int i = 0; i < E; ++i) {
+          if (!__ballot(c[i] != 0)) continue;
+          const double x = w.x(half_value<T>(half_raw<T>(g, side != 0, i)));
           const uint64_t v = c[i] ? (uint64_t)c[i] * w.at(x) : 0;
           sum += v;
           if (x >= w.floor_x) heavy += v;
@@ -998,7 +1059,7 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
     __syncthreads();
   }
   if (wave == 0) {
-    prefix_half(s);
+    prefix_half<T>(s);
     Spot at;
     float prob = 1.0f;
     if (greedy) {
@@ -1084,17 +1145,17 @@ template <class T> __device__ void find_half(HalfScratch& s, const Row<T>& row, 
 // the counts of a row's slices -> its token
 template <class T>
 __global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, int r0, const HalfSlice* ws, int slices, int per, int S) {
-  extern __shared__ __attribute__((aligned(16))) uint4 kept[];  // [SLOTS][64]
+  extern __shared__ __attribute__((aligned(16))) uint32_t kept[];
   __shared__ HalfScratch s;
+  __shared__ uint64_t has[HALF_SLICES][MAX_GROUPS / 64];
+  constexpr int WORDS = half_groups<T>() / 64, GROUP = 64 * Half<T>::E;
   const int r = r0 + blockIdx.x, lane = threadIdx.x & 63;
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const Settings st(a, r);
-  __shared__ uint64_t has[HALF_SLICES][GROUPS / 64];
-  const SliceCounts counts = {ws + (size_t)blockIdx.x * slices, slices, has, kept};
-  if ((int)threadIdx.x < slices * (GROUPS / 64)) has[threadIdx.x / (GROUPS / 64)][threadIdx.x % (GROUPS / 64)] =
-      counts.slice[threadIdx.x / (GROUPS / 64)].has[threadIdx.x % (GROUPS / 64)];
+  const SliceCounts<T> counts = {ws + (size_t)blockIdx.x * slices, slices, has, kept};
+  if ((int)threadIdx.x < slices * WORDS) has[threadIdx.x / WORDS][threadIdx.x % WORDS] = counts.slice[threadIdx.x / WORDS].has[threadIdx.x % WORDS];
   __syncthreads();
-  if (threadIdx.x < GROUPS / 64) {
+  if (threadIdx.x < WORDS) {
     uint64_t h = 0;
     for (int i = 0; i < slices; ++i) h |= has[i][threadIdx.x];
     s.has[threadIdx.x] = h;
@@ -1135,25 +1196,12 @@ template <class T>
 __global__ __launch_bounds__(HWG) void half_row_kernel(cube_sample_args a, int S) {
   extern __shared__ __attribute__((aligned(16))) uint32_t count[];
   HalfScratch& s = *(HalfScratch*)(count + MAGS);
-  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = blockIdx.x;
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const Settings st(a, r);
   count_half(count, row, 0, row.granules);
-  constexpr int G = GROUPS / (HWG / 64);
-  uint32_t mask = 0;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const uint2 c = ((const uint2*)count)[(wave * G + g) * (GROUP / 2) + lane];
-    if (__ballot((c.x | c.y) != 0)) mask |= 1u << g;
-  }
-  if (lane == 0) s.part[wave] = mask;
-  __syncthreads();
-  if (threadIdx.x < GROUPS / 64) {
-    uint64_t h = 0;
-    for (int i = 0; i < 4; ++i) h |= (uint64_t)s.part[4 * threadIdx.x + i] << (16 * i);
-    s.has[threadIdx.x] = h;
-  }
-  if (!decide_half<T>(s, LdsCounts{count}, st, a.V, S)) {
+  mark_half<T>(count, s.part, s.has, [](int, const Words<Half<T>::E>&) {});
+  if (!decide_half<T>(s, LdsCounts<T>{count}, st, a.V, S)) {
     if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
@@ -1543,7 +1591,7 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
     return CUBE_OK;
   }
   static CubeLdsReservation lds, lds2;
-  constexpr size_t kept = 16 * 64 * SLOTS + 16;  // (16: always past the size that needs no reservation)
+  constexpr size_t kept = KEPT_BYTES;
   if (!lds.ensure((const void*)half_count_kernel<T>, bytes) || !lds2.ensure((const void*)half_choose_kernel<T>, kept))
     CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
   for (int r0 = 0; r0 < a.M; r0 += p.rows) {
