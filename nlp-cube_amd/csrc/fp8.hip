@@ -23,7 +23,9 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int BLK = 128;       // columns per scale
-constexpr int MAX_K = 1 << 24;  // column indices stay far inside 32 bits
+constexpr int MAX_K = 1 << 24;  // column indices stay far inside 32 bits,
+constexpr int MAX_MN = 1 << 30;  // and rounded-up row and output counts inside them;
+constexpr long long MAX_LD = 1LL << 40;  // distances of rows in bytes inside 64
 
 __device__ __forceinline__ float load_val(const float* p) { return *p; }
 __device__ __forceinline__ float load_val(const _Float16* p) { return (float)*p; }
@@ -235,7 +237,8 @@ __device__ __forceinline__ Frag16 widen(i32x8 q, uint32_t e) {
 // EXACT.  The 8-bit matrix instructions align the products of 8 neighbouring columns to their largest and keep 13 bits below
 // it before they reach the fp32 accumulator (measured, the scaled and the unscaled form alike: 1.5e-5 of the result's 2-norm on
 // normal data, whatever K): a hundredth of a bf16 step, but too coarse for an fp32 result.  For fp32 outputs the codes are
-// widened to bf16 on their way from LDS, the conversion applying the block's scale, and multiplied at half the rate.
+// widened to bf16 on their way from LDS, the conversion applying the block's scale, and multiplied at half the rate: exactly for
+// values from 2^-133 to below 2^128 (what is smaller rounds to a multiple of 2^-133, and 2^128 is infinite, as it is in fp32).
 template <bool EXACT> struct Operand;
 template <> struct Operand<false> {
   i32x8 q; uint32_t e;
@@ -730,14 +733,24 @@ size_t quant_bytes(int M, int K) {
   return q + (size_t)((kblocks(K) + 3) / 4) * M * 4;
 }
 
+// whether two matrices share bytes: address, bytes from row to row, bytes of a row, rows (windows of one buffer side by side do not)
+bool overlap(const void* a, long long pa, long long wa, int na, const void* b, long long pb, long long wb, int nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  const __int128 x1 = (__int128)pa * (na - 1) + wa + x, y1 = (__int128)pb * (nb - 1) + wb + y;
+  if (x >= y1 || y >= x1) return false;
+  if (pa != pb) return true;
+  const long long d = y >= x ? (long long)((y - x) % (uintptr_t)pa) : (pa - (long long)((x - y) % (uintptr_t)pa)) % pa;
+  return d < wa || d + wb > pa;
+}
+
 // what cube_gemm_fp8 and cube_linear_fp8 check alike
 int check_args(const cube_fp8_args* a, const char* who) {
-  if (a->M < 0 || a->N < 0 || a->K < 1 || a->K > MAX_K) CUBE_FAIL(CUBE_ERR_ARG, "%s: M=%d N=%d K=%d", who, a->M, a->N, a->K);
+  if (a->M < 0 || a->N < 0 || a->M > MAX_MN || a->N > MAX_MN || a->K < 1 || a->K > MAX_K) CUBE_FAIL(CUBE_ERR_ARG, "%s: M=%d N=%d K=%d", who, a->M, a->N, a->K);
   if (a->M == 0 || a->N == 0) return CUBE_OK;
   if (!a->A || !a->W || !a->W_scale || !a->out) CUBE_FAIL(CUBE_ERR_ARG, "%s: null A / W / W_scale / out", who);
   if (a->out_type < CUBE_T_F32 || a->out_type > CUBE_T_F16) CUBE_FAIL(CUBE_ERR_ARG, "%s: out_type=%d", who, a->out_type);
   if (a->act < CUBE_FP8_NONE || a->act > CUBE_FP8_RELU) CUBE_FAIL(CUBE_ERR_ARG, "%s: act=%d", who, a->act);
-  if (a->ldw < (long long)kblocks(a->K) * BLK || a->lds_w < a->N || a->ldo < a->N)
+  if (a->ldw < (long long)kblocks(a->K) * BLK || a->lds_w < a->N || a->ldo < a->N || a->ldo > MAX_LD)
     CUBE_FAIL(CUBE_ERR_ARG, "%s: ldw=%lld (>= %lld), lds_w=%d (>= N=%d), ldo=%lld (>= N)", who, a->ldw, (long long)kblocks(a->K) * BLK,
               a->lds_w, a->N, a->ldo);
   if (a->ldw > MAX_K) CUBE_FAIL(CUBE_ERR_ARG, "%s: ldw=%lld is over %d", who, a->ldw, MAX_K);
@@ -763,11 +776,11 @@ Fp8Params params(const cube_fp8_args* a) {
 extern "C" int cube_quant_fp8(const void* x, int x_type, long long ld_x, int M, int K, void* q, long long ld_q, uint32_t* scale,
                               int ld_s, void* stream) {
   CUBE_ENTRY();
-  if (M < 0 || K < 1 || K > MAX_K) CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: M=%d K=%d", M, K);
+  if (M < 0 || M > MAX_MN || K < 1 || K > MAX_K) CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: M=%d K=%d", M, K);
   if (M == 0) return CUBE_OK;
   if (!x || !q || !scale) CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: null x / q / scale");
   if (x_type < CUBE_T_F32 || x_type > CUBE_T_F16) CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: x_type=%d", x_type);
-  if (ld_x < K || ld_q < (long long)kblocks(K) * BLK || ld_s < M)
+  if (ld_x < K || ld_x > MAX_LD || ld_q > MAX_LD || ld_q < (long long)kblocks(K) * BLK || ld_s < M)
     CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: ld_x=%lld (>= K=%d), ld_q=%lld (>= %lld), ld_s=%d (>= M=%d)", ld_x, K, ld_q,
               (long long)kblocks(K) * BLK, ld_s, M);
   if (((uintptr_t)q & 15) || ld_q % 16) CUBE_FAIL(CUBE_ERR_ALIGN, "cube_quant_fp8: rows of q are not 16-byte aligned");
@@ -787,12 +800,14 @@ extern "C" int cube_gemm_fp8(const cube_fp8_args* a, void* stream) {
               a->lds_a, a->M);
   if (((uintptr_t)a->A & 15) || a->lda % 16 || ((uintptr_t)a->A_scale & 3))
     CUBE_FAIL(CUBE_ERR_ALIGN, "cube_gemm_fp8: rows of A are not 16-byte aligned, or A_scale not 4-byte aligned");
+  if (overlap(a->A, a->lda, (long long)kblocks(a->K) * BLK, a->M, a->out, a->ldo * type_size(a->out_type), (long long)a->N * type_size(a->out_type), a->M))
+    CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: out overlaps A");
   Fp8Params p = params(a);
   return launch_gemm(p, (hipStream_t)stream);
 }
 
 extern "C" size_t cube_linear_fp8_workspace_bytes(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > MAX_K || fused(M, K)) return 0;
+  if (M <= 0 || M > MAX_MN || N <= 0 || K <= 0 || K > MAX_K || fused(M, K)) return 0;
   return quant_bytes(M, K);
 }
 
@@ -803,11 +818,13 @@ extern "C" int cube_linear_fp8(const cube_fp8_args* a, void* ws, size_t ws_bytes
   const int rc = check_args(a, "cube_linear_fp8");
   if (rc) return rc;
   if (a->M == 0 || a->N == 0) return CUBE_OK;
-  if (a->lda < a->K) CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: lda=%lld < K=%d", a->lda, a->K);
+  if (a->lda < a->K || a->lda > MAX_LD) CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: lda=%lld (>= K=%d)", a->lda, a->K);
   if ((uintptr_t)a->A % type_size(a->a_type)) CUBE_FAIL(CUBE_ERR_ALIGN, "cube_linear_fp8: A is not aligned to its type");
   const size_t need = cube_linear_fp8_workspace_bytes(a->M, a->N, a->K);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: workspace of %zu bytes (need %zu, 16-byte aligned)", ws_bytes, need);
+  const long long es = type_size(a->a_type), eo = type_size(a->out_type);
+  if (overlap(a->A, a->lda * es, a->K * es, a->M, a->out, a->ldo * eo, a->N * eo, a->M)) CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: out overlaps A");
   Fp8Params p = params(a);
   hipStream_t st = (hipStream_t)stream;
   if (!need) {

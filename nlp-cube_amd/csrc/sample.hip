@@ -1603,8 +1603,8 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
   return CUBE_OK;
 }
 
-// 16-bit rows longer than this are counted by value (top-p, us: bf16 64 x 16000 16 against 19, 256 x 32000 19 against 33;  f16 has eight
-// times as many values to an octave, so it pays later: 256 x 32000 44 against 33)
+// 16-bit rows longer than this are counted by value (us: bf16 64 x 16000, top-p 16 against 19; bf16 256 x 32000 19 against 33).  f16
+// has eight times as many values to an octave: 256 x 32000, top-p 31 against 33, but top-k 33 against 17 and 1 x 20000 24 against 16.
 template <class T> constexpr int half_v() { return std::is_same<T, bf16_t>::value ? 16000 : MID_V; }
 
 template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStream_t st) {

@@ -389,9 +389,9 @@ class Fp8Rows:
         """The values the rows stand for, f32 [rows, columns]."""
         import torch
         kb = self.q.shape[1] // FP8_BLOCK
-        e = self.scale.t().contiguous().view(torch.uint8)[:, :kb].to(torch.int32) - 127
+        e = self.scale.t().reshape(-1).view(torch.uint8).reshape(self.rows, 4 * self.scale.shape[0])[:, :kb].to(torch.int32) - 127
         v = self.q.view(torch.float8_e4m3fn).float().reshape(self.rows, kb, FP8_BLOCK)
-        return torch.ldexp(v, e[:, :, None]).reshape(self.rows, -1)[:, :self.columns]
+        return torch.ldexp(v, e[:, :, None]).reshape(self.rows, kb * FP8_BLOCK)[:, :self.columns]
 
 
 def quant_fp8(x):
@@ -509,7 +509,7 @@ def sample_rows(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             ptrs.append(_vector("sample_rows", name, x, M, dtype, dev))
             scalars.append(0)
         else:
-            if not x >= 0 or (name in ("top_p", "min_p") and x > 1.0) or (name == "top_k" and int(x) != x):
+            if not x >= 0 or (name in ("top_p", "min_p") and x > 1.0) or (name == "top_k" and x % 1):
                 raise ValueError("sample_rows: %s=%r" % (name, x))
             ptrs.append(None)
             scalars.append(min(int(x), 0x7fffffff) if name == "top_k" else x)

@@ -11,7 +11,7 @@ class Sampling:
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=None):
         if not temperature >= 0:
             raise ValueError("temperature must be 0 (greedy) or more, got %r" % (temperature,))
-        if not (int(top_k) == top_k and top_k >= 0):
+        if not (top_k >= 0 and top_k % 1 == 0):
             raise ValueError("top_k must be a whole number, 0 for no limit, got %r" % (top_k,))
         if not 0 <= top_p <= 1 or not 0 <= min_p <= 1:
             raise ValueError("top_p and min_p lie in 0..1, got %r, %r" % (top_p, min_p))

@@ -209,6 +209,27 @@ def test_gemm_scales_span_the_whole_range(dev):
     np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("M", [5, 40, 300])
+def test_gemm_of_every_code_and_scale_byte(dev, M):
+    """Every magnitude of e4m3 at scale bytes over the range, times 1 or 3 * 2^-9 at a scale that brings the product back near 1: 16-bit
+    outputs are the product rounded once at every byte; fp32 outputs are exact for values from 2^-133 (byte 3 on) to below 2^128."""
+    mags = oo.e4m3_values()[1:127]
+    for t in ("bf16", "f32"):
+        for be in ((3, 4, 60, 127, 200, 246) if t == "f32" else (0, 1, 2, 3, 60, 127, 200, 247, 253, 254)):
+            bw = min(max(254 - be, 3), 246)
+            v, wv = np.zeros((M, 128)), np.zeros((40, 128))
+            v[:, 9] = np.resize(mags, M)
+            wv[:, 9] = np.where(np.arange(40) % 2, 3 * 2.0 ** -9, 1.0)
+            a, w = rows_from(v, np.full((M, 1), be), 128, dev), rows_from(wv, np.full((40, 1), bw), 128, dev)
+            got = hip.gemm_fp8(a, w, out_dtype=TYPES[t])
+            want = np.outer(v[:, 9], wv[:, 9]) * 2.0 ** (be + bw - 254.0)
+            assert torch.equal(got.cpu(), torch.from_numpy(want).float().to(TYPES[t])), (t, be)
+    big = torch.full((M, 128), 3.3e38, device=dev)            # rounds to 2^128: infinite in fp32, finite times a small weight in 16 bits
+    w = hip.quant_fp8(torch.full((4, 128), 2.0 ** -60, device=dev))
+    assert bool((hip.linear_fp8(big, w) == float("inf")).all())
+    assert bool((hip.linear_fp8(big, w, out_dtype=torch.bfloat16) == 2.0 ** 75).all())
+
+
 def test_gemm_nan_stays_in_its_row_and_column(dev):
     rng = np.random.default_rng(3)
     a, w = integer_rows(rng, 40, 300, dev), integer_rows(rng, 50, 300, dev)
@@ -346,6 +367,37 @@ def test_two_graphs_replayed_in_turn(dev):
         torch.cuda.synchronize()
         for e, o in zip(eager, outs):
             assert torch.equal(e, o)
+
+
+def test_two_streams_at_once(dev):
+    """The same entry points on two streams with nothing between them, few and many rows: every result is the one of its own inputs."""
+    w = hip.quant_fp8(torch.randn(500, 900, device=dev))
+    xs = [torch.randn(m, 900, device=dev) for m in (2, 45, 300, 2000)]
+    want = [hip.linear_fp8(x, w, act="tanh") for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for turn in range(6):
+        for i, x in enumerate(xs):
+            with torch.cuda.stream(streams[(turn + i) % 2]):
+                got.append((i, hip.linear_fp8(x, w, act="tanh")))
+    for s in streams:
+        s.synchronize()
+    for i, g in got:
+        assert torch.equal(g, want[i])
+
+
+def test_out_beside_and_over_the_input(dev):
+    """Windows of one buffer: side by side is a call like any other, over one another is refused."""
+    for M in (3, 30, 100):
+        w = hip.quant_fp8(torch.randn(64, 200, device=dev))
+        buf = torch.randn(M, 300, device=dev)
+        want = hip.linear_fp8(buf[:, :200].clone(), w)
+        keep = buf.clone()
+        hip.linear_fp8(buf[:, :200], w, out=buf[:, 230:294])
+        assert torch.equal(buf[:, 230:294], want) and torch.equal(buf[:, :230], keep[:, :230]) and torch.equal(buf[:, 294:], keep[:, 294:])
+        with pytest.raises(hip.CubeHipError, match="overlaps"):
+            hip.linear_fp8(buf[:, :200], w, out=buf[:, 199:263])
 
 
 def test_refusals_on_tensors(dev):

@@ -228,9 +228,47 @@ def test_streams_graphs_and_repeats(dev, M, V):
             assert torch.equal(e[0], o[0]) and torch.equal(e[1], o[1])
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_the_longest_row(dev, t):
+    """2^22 logits, the most a row may have; one more is refused."""
+    V = 1 << 22
+    z, u = logits(2, V, t, dev, seed=9)
+    for s in (dict(), dict(k=50, p=0.9), dict(p=0.6), dict(m=0.01, T=0.7)):
+        check(z, u, **s)
+    with pytest.raises(hip.CubeHipError):
+        hip.sample_rows(torch.zeros(1, V + 1, dtype=TYPES[t], device=dev), u[:1])
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V,k", [(102, 101), (9000, 8999), (32768, 20000), (100000, 30000), (100000, 99999)])
+def test_limits_near_the_row(dev, V, k, t):
+    """A top-k of thousands, where the kept set is longer than any list the kernels sort."""
+    z, u = logits(4, V, t, dev, seed=V + k)
+    check(z, u, k=k)
+    check(z, u, k=k, p=0.9, T=2.0)
+
+
+def test_two_streams_at_once(dev):
+    """Calls of every form on two streams with nothing between them."""
+    cases = [logits(M, V, t, dev, seed=11) + (kw,) for M, V, t in ((500, 102, "f32"), (20, 5000, "bf16"), (8, 60000, "f32"), (8, 60000, "bf16"), (4, 60000, "f16"))
+             for kw in (dict(top_p=0.9), dict(top_k=40))]
+    want = [hip.sample_rows(z, u, **kw) for z, u, kw in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for turn in range(5):
+        for i, (z, u, kw) in enumerate(cases):
+            with torch.cuda.stream(streams[(turn + i) % 2]):
+                got.append((i, hip.sample_rows(z, u, **kw)))
+    for s in streams:
+        s.synchronize()
+    for i, (token, prob) in got:
+        assert torch.equal(token, want[i][0]) and torch.equal(prob, want[i][1])
+
+
 def test_refusals_on_tensors(dev):
     z, u = logits(4, 50, "f32", dev)
-    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=1.5), dict(top_p=1.1), dict(top_p=-0.1), dict(min_p=2.0),
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=1.5), dict(top_k=float("inf")), dict(top_p=1.1), dict(top_p=-0.1), dict(min_p=2.0),
                 dict(top_k=torch.zeros(4, device=dev)), dict(top_p=torch.zeros(3, device=dev)), dict(min_p=torch.zeros(4)),
                 dict(temperature=torch.zeros(8, device=dev)[::2])):
         with pytest.raises(ValueError):

@@ -82,6 +82,24 @@ def test_sample_rows_refuses_a_workspace_that_is_short():
         _err(lib.cube_sample_rows(ctypes.byref(a), ws, n, None))
 
 
+def test_outputs_over_inputs_and_sizes_past_the_limits_are_refused():
+    lib = hip.load()
+    far = P + (1 << 32)
+    assert "overlaps" in _err(lib.cube_gemm_fp8(ctypes.byref(_fp8()), None))              # out = A
+    assert "overlaps" in _err(lib.cube_gemm_fp8(ctypes.byref(_fp8(out=P + 7 * 256 + 254, A=P)), None))   # the last row's last byte
+    x = _fp8(a_type=0, lda=200, A_scale=None, out_type=0, ldo=200)
+    for out in (P, P + 4 * 199, P + 4 * (200 * 7 + 199), P - 4 * 15):                     # windows of one row distance that meet
+        x.out = out
+        assert "overlaps" in _err(lib.cube_linear_fp8(ctypes.byref(x), far, 1 << 20, None))
+    for kw in (dict(M=(1 << 30) + 1, lds_a=(1 << 30) + 1), dict(N=(1 << 30) + 1, lds_w=(1 << 30) + 1, ldo=1 << 31), dict(ldo=(1 << 40) + 1), dict(ldw=(1 << 24) + 16),
+               dict(lda=(1 << 24) + 16)):
+        assert "overlaps" not in _err(lib.cube_gemm_fp8(ctypes.byref(_fp8(out=far, **kw)), None))
+    assert "lda" in _err(lib.cube_linear_fp8(ctypes.byref(_fp8(a_type=0, lda=(1 << 40) + 1, out=far)), far, 1 << 20, None))
+    big = (1 << 30) + 1
+    _err(lib.cube_quant_fp8(P, 0, 200, big, 200, far, 256, far, big, None))
+    assert lib.cube_linear_fp8_workspace_bytes(big, 16, 200) == 0
+
+
 def test_null_structures_are_refused():
     lib = hip.load()
     _err(lib.cube_gemm_fp8(None, None))
@@ -135,6 +153,24 @@ def test_rows_stand_for_what_the_oracle_says():
     v, eb = oo.unpack(q, s, 256)
     np.testing.assert_array_equal(eb, e)
     np.testing.assert_array_equal(got, oo.rows_value(v, eb).astype(np.float32))
+
+
+@pytest.mark.parametrize("rows,kb", [(3, 1), (1, 1), (1, 5), (5, 4), (5, 6), (0, 2)])
+def test_rows_of_any_number_of_scale_words(rows, kb):
+    """Fp8Rows.float where the scales are one word a row, one row, or none."""
+    rng = np.random.default_rng(rows + kb)
+    v = rng.choice(oo.e4m3_values()[:127], (rows, kb * 128))
+    e = rng.integers(100, 150, (rows, kb))
+    q, s = oo.pack(v, e)
+    got = hip.Fp8Rows(torch.from_numpy(q), torch.from_numpy(s), kb * 128).float().numpy()
+    np.testing.assert_array_equal(got, oo.rows_value(v, e).astype(np.float32))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 1.5, -1])
+def test_sampling_refuses_a_limit_that_is_no_count(bad):
+    from cube_amd.networks.sampling import Sampling
+    with pytest.raises(ValueError):
+        Sampling(top_k=bad)
 
 
 def test_oracle_sampler_against_enumeration():
