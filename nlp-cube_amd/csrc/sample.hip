@@ -48,24 +48,24 @@ template <class T> struct Granule { static constexpr int N = 16 / sizeof(T); }; 
 
 // The 16-byte granules of a row, counted from the aligned address at or before its first logit: granule j holds the logits
 // j*N - lead .. j*N - lead + N - 1.  Whole ones are loaded at once; the first and the last element by element, so that nothing
-// outside the row is read.  out: keys, 0 for what lies outside.
+// outside the row is read.  What lies outside comes as -inf, no candidate.
 template <class T> struct Row {
   const T* at; int V, lead, granules;
   __device__ Row(const T* row, int v) : at(row), V(v) {
     lead = (int)(((uintptr_t)row & 15) / sizeof(T));
     granules = (V + lead + Granule<T>::N - 1) / Granule<T>::N;
   }
-  __device__ __forceinline__ void keys(int j, uint32_t (&out)[Granule<T>::N]) const {
+  __device__ __forceinline__ void values(int j, float (&out)[Granule<T>::N]) const {
     constexpr int N = Granule<T>::N;
     typedef T vec __attribute__((ext_vector_type(N)));
     const int i0 = j * N - lead;
     if (i0 >= 0 && i0 + N <= V) {
       const vec v = *(const vec*)(at + i0);
 #pragma unroll
-      for (int i = 0; i < N; ++i) out[i] = key_of(as_float(v[i]));
+      for (int i = 0; i < N; ++i) out[i] = as_float(v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) out[i] = i0 + i >= 0 && i0 + i < V ? key_of(as_float(at[i0 + i])) : 0u;
+      for (int i = 0; i < N; ++i) out[i] = i0 + i >= 0 && i0 + i < V ? as_float(at[i0 + i]) : -INFINITY;
     }
   }
 };
@@ -96,32 +96,35 @@ struct Settings {
 };
 
 struct Weigher {
-  double inv_t, floor_x;  // 1 / T, ln(min-p)
-  float top; int S;       // largest logit
-  __device__ Weigher(const Settings& s, float best, int bits) : top(best), S(bits) {
-    inv_t = 1.0 / (double)s.temp;
-    floor_x = s.m > 0.0f ? log(s.m < 1.0f ? (double)s.m : 1.0) : -INFINITY;
+  double top, per_t, floor_x;  // largest logit, log2(e) / T, log2(min-p)
+  int S;
+  // An infinite logit beside an infinite largest one has weight 1 and every other none: the largest finite double in place of the
+  // infinity makes their differences infinite and -1.8e308, and power() ends the range on both sides.
+  __device__ Weigher(const Settings& s, float best, int bits) : S(bits) {
+    top = fmin((double)best, 1.7976931348623157e308);
+    per_t = fmax(1.4426950408889634 / (double)s.temp, 1e-290);
+    floor_x = s.m > 0.0f ? log2(s.m < 1.0f ? (double)s.m : 1.0) : -INFINITY;
   }
-  __device__ __forceinline__ double x(float v) const { return v == top ? 0.0 : ((double)v - (double)top) * inv_t; }
-  // 2^shift * exp(x), x <= 0: 2^(n + f) with |f| <= 1/2, 2^f by the series of exp(f ln 2) to the 11th power (the 12th is below
-  // 2^-47 of the value).  NaN (0 * inf: an infinite temperature beside an infinite logit) counts as -1100, nothing.
+  __device__ __forceinline__ double x(float v) const { return ((double)v - top) * per_t; }  // log2 of the weight
+  // 2^(x + shift): x = n + f with |f| <= 1/2 (adding 1.5 * 2^52 rounds x to n and leaves n in the low bits), 2^f = 1 + f * P(f),
+  // P of the 9th degree through (2^f - 1) / f at the Chebyshev nodes (2^-50 of the value), n + shift added to the exponent bits.
+  // What is no candidate (NaN, -inf) comes out at 2^-960, as nothing.
   __device__ __forceinline__ double power(double x, int shift) const {
-    const double y = fmax(x, -1100.0) * 1.4426950408889634;
-    const double n = rint(y);
-    const double f = (y - n) * 0.6931471805599453;
-    double e = 1.0 / 39916800.0;
-    e = fma(e, f, 1.0 / 3628800.0);
-    e = fma(e, f, 1.0 / 362880.0);
-    e = fma(e, f, 1.0 / 40320.0);
-    e = fma(e, f, 1.0 / 5040.0);
-    e = fma(e, f, 1.0 / 720.0);
-    e = fma(e, f, 1.0 / 120.0);
-    e = fma(e, f, 1.0 / 24.0);
-    e = fma(e, f, 1.0 / 6.0);
-    e = fma(e, f, 0.5);
+    const double y = fmin(fmax(x, -960.0), 0.0);
+    const double t = y + 6755399441055744.0;
+    const double f = y - (t - 6755399441055744.0);
+    double e = 7.070977866508139e-09;
+    e = fma(e, f, 1.0205905413765595e-07);
+    e = fma(e, f, 1.3215451633221434e-06);
+    e = fma(e, f, 1.5252672924850737e-05);
+    e = fma(e, f, 0.00015403530424776529);
+    e = fma(e, f, 0.0013333558200794592);
+    e = fma(e, f, 0.009618129107618665);
+    e = fma(e, f, 0.05550410866465167);
+    e = fma(e, f, 0.24022650695910075);
+    e = fma(e, f, 0.6931471805599462);
     e = fma(e, f, 1.0);
-    e = fma(e, f, 1.0);
-    return ldexp(e, (int)n + shift);
+    return __hiloint2double(__double2hiint(e) + ((__double2loint(t) + shift) << 20), __double2loint(e));
   }
   // to an integer: at 2^52 a double's last place is 1, and its low bits are the sum (S <= 46)
   __device__ __forceinline__ uint64_t at(double x) const {
@@ -514,11 +517,29 @@ __device__ void place_few(Few& f, const Weigher& w, uint64_t before, uint64_t ta
 // Equal steps of the logit below the largest one, 32 wide in all (32 T for temperatures above 1): in the region that matters a bin
 // then holds few logits whatever their scale.  Falls monotonically with the key, so bins are in the candidates' order.
 struct Steps {
-  float top, scale, last;
-  __device__ Steps(float best, float temp, int bins) : top(best), last((float)(bins - 1)) { scale = (float)(bins / 32) / (temp > 1.0f ? temp : 1.0f); }
-  __device__ __forceinline__ int operator()(uint32_t key) const {
-    const float v = value_of(key);
-    return v == top ? 0 : (int)fminf((top - v) * scale, last);  // (inf and NaN: the last bin)
+  float top, scale; uint32_t last;
+  __device__ Steps(float best, float temp, int bins) : top(best), last((uint32_t)bins - 1) { scale = (float)(bins / 32) / (temp > 1.0f ? temp : 1.0f); }
+  __device__ __forceinline__ int operator()(float v) const {
+    uint32_t b;  // the conversion ends at 2^32 - 1 and takes NaN (an infinite logit below an infinite largest one) to 0: as an instruction, since in C++ both are undefined
+    asm("v_cvt_u32_f32 %0, %1" : "=v"(b) : "v"((top - v) * scale));
+    return (int)(b < last ? b : last);
+  }
+  __device__ __forceinline__ int operator()(uint32_t key) const { return (*this)(value_of(key)); }
+};
+// A span of bins as a span of logits, a little wider (2^-20 of the numbers it is computed from, where their roundings take 2^-22): two
+// comparisons tell nearly all logits outside it, and the bins of the others are computed.
+struct Span {
+  float lo, hi; int from, to;
+  __device__ Span(const Steps& step, int from_, int to_) : from(from_), to(to_) {
+    const float slack = fabsf(step.top) * 9.6e-7f, least = step.top - (float)(to + 1) / step.scale * 1.000001f - slack;
+    const float most = step.top - (float)from / step.scale * 0.999999f + slack;
+    lo = to == (int)step.last || !(least >= -INFINITY) ? -INFINITY : least;  // (infinities: the span may come out empty-handed as NaN)
+    hi = from == 0 || !(most >= -INFINITY) ? INFINITY : most;
+  }
+  __device__ __forceinline__ bool near(float v) const { return v >= lo && v <= hi; }  // false for NaN
+  __device__ __forceinline__ bool has(const Steps& step, float v) const {
+    const int b = step(v);
+    return v > -INFINITY && b >= from && b <= to;
   }
 };
 
@@ -535,20 +556,37 @@ template <int WG, int BINS, class G> __device__ Found find_up(Scratch& s, const 
 // ---- mid: one workgroup a row, keys in LDS ----------------------------------------------------------------------------------
 constexpr int MID_V = 32768;
 
-// every thread four neighbouring keys at a time; n4: a multiple of four
-template <int WG> struct LdsKeys {
-  const uint32_t* keys; int n4;
-  template <class F> __device__ __forceinline__ void operator()(F f) const {
+// every thread four neighbouring logits at a time; n4: a multiple of four
+template <int WG> struct LdsValues {
+  const float* at; int n4;
+  template <class F> __device__ __forceinline__ void values(F f) const {
     for (int i = 4 * (int)threadIdx.x; i < n4; i += 4 * WG) {
-      const uint4 k = *(const uint4*)&keys[i];
-      f(k.x); f(k.y); f(k.z); f(k.w);
+      const f32x4 v = *(const f32x4*)&at[i];
+      f(v[0]); f(v[1]); f(v[2]); f(v[3]);
     }
   }
-  template <class F> __device__ __forceinline__ void with_index(F f) const {
+  template <class F> __device__ __forceinline__ void operator()(F f) const {
+    values([&](float v) { f(key_of(v)); });
+  }
+  // f(value, index) for those in the span
+  template <class F> __device__ __forceinline__ void inside(const Steps& step, const Span& span, F f) const {
     for (int i = 4 * (int)threadIdx.x; i < n4; i += 4 * WG) {
-      const uint4 k = *(const uint4*)&keys[i];
-      f(k.x, i); f(k.y, i + 1); f(k.z, i + 2); f(k.w, i + 3);
+      const f32x4 v = *(const f32x4*)&at[i];
+      if (span.near(v[0]) || span.near(v[1]) || span.near(v[2]) || span.near(v[3])) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (span.has(step, v[e])) f(v[e], i + e);
+      }
     }
+  }
+};
+// The weights of many logits into a histogram over steps; MIN_P: and the sum of those that min-p keeps
+template <bool MIN_P> struct Gather {
+  const Weigher& w; const Steps& step; uint64_t* hist; uint64_t& heavy;
+  __device__ __forceinline__ void operator()(float v) const {
+    const double x = w.x(v);
+    const uint64_t one = w.at(x);
+    if (one) atomicAdd((unsigned long long*)&hist[step(v)], (unsigned long long)one);  // (none for what is no candidate)
+    if (MIN_P && x >= w.floor_x) heavy += one;
   }
 };
 
@@ -566,7 +604,7 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
   };
   if (st.limited(V)) {
     clear();
-    keys([&](uint32_t k) { if (k) atomicAdd((unsigned long long*)&s.high[step(k)], 1ull); });
+    keys.values([&](float v) { if (v > -INFINITY) atomicAdd((unsigned long long*)&s.high[step(v)], 1ull); });
     __syncthreads();
     const Runs r = scan_up<WG, BINS>(s, get);
     if ((uint64_t)st.k < r.total || r.total <= FEW) {
@@ -576,7 +614,7 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
         if (at.before + s.high[at.bin] > FEW) return false;
         bin = at.bin;
       }
-      keys.with_index([&](uint32_t k, int i) { if (k && step(k) <= (int)bin) append(f, entry_of(k, (uint32_t)(i - lead))); });
+      keys.inside(step, Span(step, 0, (int)bin), [&](float v, int i) { append(f, entry_of(key_of(v), (uint32_t)(i - lead))); });
       __syncthreads();
       sort_few<WG>(f);
       if (threadIdx.x < 64) {
@@ -594,20 +632,14 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
   }
   clear();
   uint64_t heavy = 0;  // weight of those that min-p keeps
-  keys([&](uint32_t k) {
-    if (k) {
-      const double x = w.x(value_of(k));
-      const uint64_t v = w.at(x);
-      if (v) atomicAdd((unsigned long long*)&s.high[step(k)], (unsigned long long)v);
-      if (x >= w.floor_x) heavy += v;
-    }
-  });
+  if (st.m > 0.0f) keys.values(Gather<true>{w, step, s.high, heavy});
+  else keys.values(Gather<false>{w, step, s.high, heavy});
   __syncthreads();
   const Runs r = scan_up<WG, BINS>(s, get);
   // the place in which the running weight passes a target: the members of its bin, sorted
   auto place = [&](uint64_t target) {
     const Found at = find_up<WG, BINS>(s, r, target, get);
-    keys.with_index([&](uint32_t k, int i) { if (k && step(k) == (int)at.bin) append(f, entry_of(k, (uint32_t)(i - lead))); });
+    keys.inside(step, Span(step, (int)at.bin, (int)at.bin), [&](float v, int i) { append(f, entry_of(key_of(v), (uint32_t)(i - lead))); });
     __syncthreads();
     if (f.n > FEW) return false;
     sort_few<WG>(f);
@@ -641,27 +673,27 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Scratch& s = *(Scratch*)smem;
   Few& few = *(Few*)(smem + sizeof(Scratch));
-  uint32_t* keys = (uint32_t*)(smem + sizeof(Scratch) + sizeof(Few));
+  float* keys = (float*)(smem + sizeof(Scratch) + sizeof(Few));
   constexpr int N = Granule<T>::N;
   const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const Settings st(a, r);
-  uint32_t best = 0;
+  float largest = -INFINITY;
   for (int j = threadIdx.x; j < row.granules; j += WG) {
-    uint32_t k[N];
-    row.keys(j, k);
+    float v[N];
+    row.values(j, v);
 #pragma unroll
-    for (int i = 0; i < N; i += 4) *(uint4*)&keys[j * N + i] = make_uint4(k[i], k[i + 1], k[i + 2], k[i + 3]);
+    for (int i = 0; i < N; i += 4) *(f32x4*)&keys[j * N + i] = (f32x4){v[i], v[i + 1], v[i + 2], v[i + 3]};
 #pragma unroll
-    for (int i = 0; i < N; ++i) best = k[i] > best ? k[i] : best;
+    for (int i = 0; i < N; ++i) largest = fmaxf(largest, v[i]);  // (NaN is passed over)
   }
-  best = block_max<WG>(s, best);  // its barriers also make the keys visible
+  const uint32_t best = block_max<WG>(s, key_of(largest));  // its barriers also make the logits visible
   if (best == 0) {
     if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
   const int n4 = row.granules * N;
-  const LdsKeys<WG> each = {keys, n4};
+  const LdsValues<WG> each = {keys, n4};
   Choice c = {best, 0, 0};
   float prob = 1.0f;
   if (!st.greedy()) {
@@ -674,16 +706,18 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
     c = decide<WG>(s, each, st, w, a.V);
     prob = w.prob(value_of(c.key), c.kept);
   }
-  // the c.tie-th key equal to c.key in order of index: each wave counts its span (256 keys a step), the owner walks its own
+  // the c.tie-th logit equal to that of c.key in order of index: each wave counts its span (256 a step), the owner walks its own
+  const float chosen = value_of(c.key);
   const int steps = (n4 + 255) / 256, per = (steps + WG / 64 - 1) / (WG / 64);
   const int lo = wave * per, hi = lo + per < steps ? lo + per : steps;
-  auto ties4 = [&](int step, uint32_t (&k)[4]) {  // this lane's four keys of a step: how many are equal
+  auto ties4 = [&](int step, float (&k)[4]) {  // this lane's four of a step: how many are equal
     const int i = step * 256 + 4 * lane;
-    const uint4 v = i < n4 ? *(const uint4*)&keys[i] : make_uint4(0, 0, 0, 0);
-    k[0] = v.x; k[1] = v.y; k[2] = v.z; k[3] = v.w;
-    return (v.x == c.key) + (v.y == c.key) + (v.z == c.key) + (v.w == c.key);
+    const f32x4 v = i < n4 ? *(const f32x4*)&keys[i] : (f32x4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    k[0] = v[0]; k[1] = v[1]; k[2] = v[2]; k[3] = v[3];
+    return (v[0] == chosen) + (v[1] == chosen) + (v[2] == chosen) + (v[3] == chosen);
   };
-  uint32_t mine = 0, k[4];
+  uint32_t mine = 0;
+  float k[4];
   for (int i = lo; i < hi; ++i) mine += ties4(i, k);
   mine = wave_sum(mine);
   if (lane == 0) s.part32[wave] = mine;
@@ -698,7 +732,7 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
       uint32_t at = before + incl - n;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (k[e] == c.key) {
+        if (k[e] == chosen) {
           if (at == c.tie) { a.token[r] = i * 256 + 4 * lane + e - row.lead; if (a.prob) a.prob[r] = prob; }
           ++at;
         }
@@ -1240,15 +1274,15 @@ __global__ __launch_bounds__(LWG) void long_top_kernel(cube_sample_args a, int r
   if (blockIdx.x == 0 && threadIdx.x == 0) { l.heavy = 0; l.listed = 0; }
   const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
-  uint32_t best = 0;
+  float largest = -INFINITY;
 #pragma unroll 4
   for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-    uint32_t k[4];
-    row.keys(j, k);
+    float v[4];
+    row.values(j, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) best = k[i] > best ? k[i] : best;
+    for (int i = 0; i < 4; ++i) largest = fmaxf(largest, v[i]);
   }
-  best = wave_max(best);
+  uint32_t best = wave_max(key_of(largest));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = best;
   __syncthreads();
   if (threadIdx.x < 64) {
@@ -1270,34 +1304,26 @@ __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int 
   const Steps step(value_of(best), st.temp, LONG_BINS);
   const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
-  if (st.limited(a.V)) {
+  auto all = [&](auto f) {
 #pragma unroll 2
     for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-      uint32_t k[4];
-      row.keys(j, k);
+      float v[4];
+      row.values(j, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) if (k[i]) atomicAdd((unsigned long long*)&hist[step(k[i])], 1ull);
+      for (int i = 0; i < 4; ++i) f(v[i]);
     }
+  };
+  if (st.limited(a.V)) {
+    all([&](float v) { if (v > -INFINITY) atomicAdd((unsigned long long*)&hist[step(v)], 1ull); });
   } else {
     const Weigher w(st, value_of(best), S);
     uint64_t heavy = 0;
-#pragma unroll 2
-    for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-      uint32_t k[4];
-      row.keys(j, k);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (k[i]) {
-          const double x = w.x(value_of(k[i]));
-          const uint64_t v = w.at(x);
-          if (v) atomicAdd((unsigned long long*)&hist[step(k[i])], (unsigned long long)v);
-          if (x >= w.floor_x) heavy += v;
-        }
-      }
-    }
     if (st.m > 0.0f) {
+      all(Gather<true>{w, step, hist, heavy});
       heavy = wave_sum(heavy);
       if ((threadIdx.x & 63) == 0 && heavy) atomicAdd((unsigned long long*)&l.heavy, (unsigned long long)heavy);
+    } else {
+      all(Gather<false>{w, step, hist, heavy});
     }
   }
   __syncthreads();
@@ -1356,15 +1382,22 @@ __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int 
   }
   const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
+  const float largest = value_of(best);
+  const Span span(step, from, to), last(step, end < 0 ? from : end, end < 0 ? to : end);
+#pragma unroll 2
   for (int j0 = lo; j0 < hi; j0 += LWG) {
     const int j = j0 + threadIdx.x;
-    uint32_t k[4] = {0, 0, 0, 0}, n = 0;
+    float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (j < hi) row.values(j, v);
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) some |= span.near(v[i]) | last.near(v[i]);
+    if (__ballot(some) == 0) continue;
+    uint32_t n = 0;
     bool in[4];
-    if (j < hi) row.keys(j, k);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int b = step(k[i]);
-      in[i] = k[i] && ((b >= from && b <= to) || b == end) && (!st.greedy() || k[i] == best);
+      in[i] = (span.has(step, v[i]) || last.has(step, v[i])) && (!st.greedy() || v[i] == largest);
       n += in[i];
     }
     if (__ballot(n != 0) == 0) continue;
@@ -1375,7 +1408,7 @@ __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (in[i]) {
-        if (at < LIST) l.list[at] = entry_of(k[i], (uint32_t)(j * 4 + i - row.lead));
+        if (at < LIST) l.list[at] = entry_of(key_of(v[i]), (uint32_t)(j * 4 + i - row.lead));
         ++at;
       }
   }
@@ -1392,10 +1425,10 @@ struct RowKeys {
   const Row<float>& row;
   template <class F> __device__ __forceinline__ void operator()(F f) const {
     for (int j = threadIdx.x; j < row.granules; j += LWG) {
-      uint32_t k[4];
-      row.keys(j, k);
+      float v[4];
+      row.values(j, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f(k[i]);
+      for (int i = 0; i < 4; ++i) f(key_of(v[i]));
     }
   }
 };
@@ -1500,10 +1533,10 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
     };
     if (whole) {
       for (int j = threadIdx.x; j < row.granules; j += LWG) {
-        uint32_t k[4];
-        row.keys(j, k);
+        float v[4];
+        row.values(j, v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (k[i] == c.key) add((uint32_t)(j * 4 + i - row.lead));
+        for (int i = 0; i < 4; ++i) if (key_of(v[i]) == c.key) add((uint32_t)(j * 4 + i - row.lead));
       }
     } else {
       for (int i = threadIdx.x; i < n; i += LWG) if ((uint32_t)(list[i] >> 32) == c.key) add(~(uint32_t)list[i]);
