@@ -392,15 +392,12 @@ __global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, i
     const int i = lane + 64 * e;
     key[e] = i < V ? key_of(as_float(row[i])) : 0u;
     best = key[e] > best ? key[e] : best;
-    s_key[wave][i] = key[e];
   }
   best = wave_max(best);
   if (best == 0) {
     if (lane == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
   if (st.greedy()) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -411,10 +408,20 @@ __global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, i
       }
     }
   }
-  // places: before an equal key of its own 64 come those of lower lanes, of earlier 64s all, of later 64s none
+  // places: before an equal key of its own 64 come those of lower lanes, of earlier 64s all, of later 64s none.  A key of 16 bits has
+  // room for its lane below them, so that none are equal.  Others are counted as if none were, and put right where two then have one
+  // place (8192 x 102 f32: 12.6 us, 15.9 with the lanes compared in every step; 22 where all logits are equal).
   int place[E];
+  uint32_t plain[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) place[e] = 0;
+  for (int e = 0; e < E; ++e) {
+    place[e] = 0;
+    plain[e] = key[e];
+    if (sizeof(T) == 2 && key[e]) key[e] = (key[e] & ~255u) | (255u - (lane + 64 * e));
+    s_key[wave][lane + 64 * e] = key[e];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   const int n4 = (V + 3) / 4;
 #pragma unroll
   for (int c = 0; c < E; ++c) {
@@ -422,15 +429,28 @@ __global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, i
       const uint4 o = *(const uint4*)&s_key[wave][4 * q];
       const uint32_t other[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = 4 * (q - 16 * c) + i;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t mine = e > c ? key[e] : e < c ? key[e] + 1 : key[e] + (at >= lane ? 1u : 0u);
-          place[e] += other[i] >= mine ? 1 : 0;
-        }
+        for (int e = 0; e < E; ++e) place[e] += other[i] >= key[e] + (e > c ? 0u : 1u) ? 1 : 0;
+    }
+  }
+  if constexpr (sizeof(T) == 4) {
+    bool twice = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) if (key[e]) s_order[wave][place[e]] = lane + 64 * e;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < E; ++e) twice |= key[e] && s_order[wave][place[e]] != (uint32_t)(lane + 64 * e);
+    if (__ballot(twice)) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+#pragma unroll 4
+        for (int i = 0; i < 64; ++i) place[e] += i < lane && s_key[wave][64 * e + i] == key[e] ? 1 : 0;
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -442,7 +462,7 @@ __global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, i
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int e = 0; e < E; ++e)
-    if (key[e]) { s_sorted[wave][place[e]] = key[e]; s_order[wave][place[e]] = lane + 64 * e; }
+    if (key[e]) { s_sorted[wave][place[e]] = plain[e]; s_order[wave][place[e]] = lane + 64 * e; }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 
