@@ -284,7 +284,13 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void gemm_fp8_kernel(const Fp8Pa
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0, "every wave issues whole pieces");
   constexpr int ROWS = (BM + BN) * BLK, STAGE = ROWS + (BM + BN) * 4;
   constexpr int LOADS = PA + PB + PS;                    // a wave's loads per stage
-  constexpr int PER = (LOADS + TM - 1) / TM;             // of them, with each row tile's products
+  // EARLY: a step's barrier and first fragment reads come under the last products of the step before it.  With 8 row tiles a wave, where
+  // a workgroup has the CU for itself, that takes 2 to 4 % off (8192x4096x4096 131 -> 128 us, 8192x8192x8192 425 -> 415); with fewer,
+  // where another workgroup covers them, it costs 2 % (2048x2048x2048 15.0 -> 15.9 us, 8192x500x768 f32 13.8 -> 14.2).
+  constexpr bool EARLY = TM >= 8;
+  constexpr int SLOTS = EARLY ? TM / 2 + 1 : TM;         // row tiles whose products loads go out with
+  constexpr int PER = (LOADS + SLOTS - 1) / SLOTS;
+  static_assert(!EARLY || KS == 1, "the barriers of wave groups along K are counted for the other form");
   extern __shared__ __attribute__((aligned(16))) unsigned char all_smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave / NW, wid = wave % NW;
@@ -356,58 +362,111 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void gemm_fp8_kernel(const Fp8Pa
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = KS == 1 || kg == 0 ? bias[j] : (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-#pragma unroll
-  for (int k = 0; k < ST - 1; ++k)
-    if (k < steps) fill(k);
   // this lane's two chunks of a row of a fragment
   const int o0 = l15 * BLK + ((g ^ (l15 >> 1)) << 4), o1 = l15 * BLK + (((g + 4) ^ (l15 >> 1)) << 4);
-  // One step.  MORE: with the loads of stage k + ST - 1, which go out between the products (all at once in front of them they held
-  // up the fragment reads); no branch inside, so that they stay there.
   auto meet = [&] {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  auto step = [&](int k, auto MORE) {
+  // fragment and scale word of one of a stage's tiles of 16 rows
+  auto frag = [&](const unsigned char* cur, int tile) {
+    return __builtin_shufflevector(*(const i32x4*)(cur + tile * 16 * BLK + o0), *(const i32x4*)(cur + tile * 16 * BLK + o1), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto scale = [&](const unsigned char* cur, int k, int tile) { return *(const uint32_t*)(cur + ROWS + (tile * 16 + l15) * 4) >> (8 * ((first + k) & 3)); };
+  // One step.  CONT: loads of stage k + ST - 1 between the products (all at once in front of them they held up the fragment reads).
+  // EARLY: the step's first fragments are in registers already; when its last row tile's fragment has been read, the wait and the
+  // barrier of the next step come -- all waves are then done with this step's stage -- and the last products cover the reads of the
+  // next fragments.  START: the first loads of stage k + ST behind that barrier; NEXT: there is a next step.
+  i32x8 wq[TN], next;
+  uint32_t we[TN], ea[TM];
+  auto begin = [&](int k) {
     const unsigned char* cur = smem + (k % ST) * STAGE;
-    meet();
-    const int shift = 8 * ((first + k) & 3);
-    auto frag = [&](int tile) {  // of the stage's tiles of 16 rows
-      const i32x4 lo = *(const i32x4*)(cur + tile * 16 * BLK + o0), hi = *(const i32x4*)(cur + tile * 16 * BLK + o1);
-      return (i32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    };
-    auto scale = [&](int tile) { return *(const uint32_t*)(cur + ROWS + (tile * 16 + l15) * 4) >> shift; };
+#pragma unroll
+    for (int i = 0; i < TM; ++i) ea[i] = scale(cur, k, wm * TM + i);
+    next = frag(cur, wm * TM);
+  };
+  auto weight = [&](int k, int j) {
+    const unsigned char* cur = smem + (k % ST) * STAGE;
+    wq[j] = frag(cur, BM / 16 + wn * TN + j);
+    we[j] = scale(cur, k, BM / 16 + wn * TN + j);
+  };
+  auto step = [&](int k, auto CONT, auto START, auto NEXT) {
+    const unsigned char* cur = smem + (k % ST) * STAGE;
+    if constexpr (!EARLY) {
+      meet();
+      begin(k);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) weight(k, j);
+    }
     Operand<EXACT> w[TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) w[j] = Operand<EXACT>(frag(BM / 16 + wn * TN + j), scale(BM / 16 + wn * TN + j));
-    uint32_t ea[TM];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) ea[i] = scale(wm * TM + i);
-    i32x8 next = frag(wm * TM);
+    for (int j = 0; j < TN; ++j) w[j] = Operand<EXACT>(wq[j], we[j]);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {  // a row tile's fragment is read while the one before it is multiplied
       const Operand<EXACT> a(next, ea[i]);
-      if (i + 1 < TM) next = frag(wm * TM + i + 1);
-      if constexpr (decltype(MORE)::value) {
+      if (i + 1 < TM) next = frag(cur, wm * TM + i + 1);
+      if constexpr (decltype(CONT)::value) {
 #pragma unroll
-        for (int u = i * PER; u < (i + 1) * PER && u < LOADS; ++u) load(k + ST - 1, u);
+        for (int u = (i + EARLY) * PER; u < (i + EARLY + 1) * PER && u < LOADS; ++u) load(k + ST - 1, u);
+      }
+      if (EARLY && i == TM - 1) {
+        if constexpr (decltype(NEXT)::value) {
+          // step k + 1 has landed once no more loads are open than the later stages'; the barrier says so for every wave's pieces
+          if constexpr (decltype(CONT)::value) wait_vm<(ST - 2) * LOADS>();
+          else wait_vm<0>();
+          meet();
+          begin(k + 1);
+        }
+        if constexpr (decltype(START)::value) {
+#pragma unroll
+          for (int u = 0; u < PER && u < LOADS; ++u) load(k + ST, u);
+        }
       }
       if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);  // the compiler would put the read right in front of its use
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mma(w[j], a, acc[i][j]);
+      for (int j = 0; j < TN; ++j) {
+        acc[i][j] = mma(w[j], a, acc[i][j]);
+        if constexpr (decltype(NEXT)::value) {
+          if (i == TM - 1) weight(k + 1, j);
+        }
+      }
       if constexpr (!EXACT) __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // step k has landed once no more loads are open than the later stages'; the barrier in the step says so for every wave's pieces, and
-  // that all waves are done with the stage that is filled next
+#pragma unroll
+  for (int k = 0; k < ST - 1; ++k)
+    if (k < steps) fill(k);
   int k = 0;
-  for (; k < steps - (ST - 1); ++k) {
-    wait_vm<(ST - 2) * LOADS>();
-    step(k, std::true_type{});
-  }
-  for (; k < steps; ++k) {
-    wait_vm<0>();
-    step(k, std::false_type{});
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  if constexpr (EARLY) {
+    if (steps >= ST) {
+#pragma unroll
+      for (int u = 0; u < PER && u < LOADS; ++u) load(ST - 1, u);
+      wait_vm<(ST - 2) * LOADS + (PER < LOADS ? PER : LOADS)>();
+    } else {
+      wait_vm<0>();
+    }
+    meet();
+    begin(0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) weight(0, j);
+    for (; k + ST < steps; ++k) step(k, yes, yes, yes);
+    if (k + ST == steps) step(k++, yes, no, yes);
+    for (; k + 1 < steps; ++k) step(k, no, no, yes);
+    step(k, no, no, no);
+  } else {
+    // step k has landed once no more loads are open than the later stages'; the barrier in the step says so for every wave's pieces,
+    // and that all waves are done with the stage that is filled next
+    for (; k < steps - (ST - 1); ++k) {
+      wait_vm<(ST - 2) * LOADS>();
+      step(k, yes, no, no);
+    }
+    for (; k < steps; ++k) {
+      wait_vm<0>();
+      step(k, no, no, no);
+    }
   }
   if constexpr (KS > 1) {
     for (; k < per; ++k) meet();  // a group with fewer steps comes to as many barriers
