@@ -707,14 +707,19 @@ inline int kblocks(int K) { return (K - 1) / BLK + 1; }
 
 template <class T> int launch_quant(const void* x, long long ld_x, int M, int K, void* q, long long ld_q, uint32_t* scale, int ld_s,
                                     hipStream_t st) {
-  const long long blocks = (long long)((kblocks(K) + 3) / 4) * ((M + Q_ROWS - 1) / Q_ROWS);
-  if (blocks > 0x7fffffffLL) CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: %d x %d values are too many for one launch", M, K);
-  const dim3 grid((unsigned)blocks);
+  const int quads = (kblocks(K) + 3) / 4;
   // 16-byte loads where every row starts on a 16-byte boundary
   const bool vec = ((uintptr_t)x & 15) == 0 && (ld_x * (long long)sizeof(T)) % 16 == 0;
-  if (vec) hipLaunchKernelGGL((quant_kernel<T, true>), grid, dim3(256), 0, st, (const T*)x, ld_x, M, K, (uint8_t*)q, ld_q, scale, ld_s);
-  else hipLaunchKernelGGL((quant_kernel<T, false>), grid, dim3(256), 0, st, (const T*)x, ld_x, M, K, (uint8_t*)q, ld_q, scale, ld_s);
-  CUBE_CHECK_LAUNCH("cube_quant_fp8");
+  const int part = (1 << 23) / quads * Q_ROWS;  // rows of a launch: fewer than 2^32 threads (K <= 2^24: at most 2^15 quads)
+  for (long long r0 = 0; r0 < M; r0 += part) {
+    const int n = (int)(M - r0 < part ? M - r0 : part);
+    const dim3 grid((unsigned)quads * ((n + Q_ROWS - 1) / Q_ROWS));
+    const T* from = (const T*)x + r0 * ld_x;
+    uint8_t* to = (uint8_t*)q + r0 * ld_q;
+    if (vec) hipLaunchKernelGGL((quant_kernel<T, true>), grid, dim3(256), 0, st, from, ld_x, n, K, to, ld_q, scale + r0, ld_s);
+    else hipLaunchKernelGGL((quant_kernel<T, false>), grid, dim3(256), 0, st, from, ld_x, n, K, to, ld_q, scale + r0, ld_s);
+    CUBE_CHECK_LAUNCH("cube_quant_fp8");
+  }
   return CUBE_OK;
 }
 int quant_any(const void* x, int type, long long ld_x, int M, int K, void* q, long long ld_q, uint32_t* scale, int ld_s, hipStream_t st) {

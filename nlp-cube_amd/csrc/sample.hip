@@ -540,7 +540,8 @@ struct Steps {
   float top, scale; uint32_t last;
   __device__ Steps(float best, float temp, int bins) : top(best), last((uint32_t)bins - 1) { scale = (float)(bins / 32) / (temp > 1.0f ? temp : 1.0f); }
   __device__ __forceinline__ int operator()(float v) const {
-    uint32_t b;  // the conversion ends at 2^32 - 1 and takes NaN (an infinite logit below an infinite largest one) to 0: as an instruction, since in C++ both are undefined
+    uint32_t b;  // the conversion ends at 2^32 - 1 and takes NaN (an infinite logit beside an infinite largest one)
+                 // to 0: as an instruction, since in C++ both are undefined
     asm("v_cvt_u32_f32 %0, %1" : "=v"(b) : "v"((top - v) * scale));
     return (int)(b < last ? b : last);
   }
@@ -1591,22 +1592,40 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 
-template <class T> int launch_short(const cube_sample_args& a, int S, hipStream_t st) {
-  const dim3 grid((a.M + 3) / 4), block(256);
-  if (a.V <= 64) hipLaunchKernelGGL((sample_short_kernel<T, 1>), grid, block, 0, st, a, S);
-  else if (a.V <= 128) hipLaunchKernelGGL((sample_short_kernel<T, 2>), grid, block, 0, st, a, S);
-  else hipLaunchKernelGGL((sample_short_kernel<T, 4>), grid, block, 0, st, a, S);
-  CUBE_CHECK_LAUNCH("cube_sample_rows");
+// A launch has fewer than 2^32 threads: where every row has a wave or a workgroup, rows go in parts of 2^21.
+template <class T, class F> int in_parts(const cube_sample_args& all, F f) {
+  constexpr int PART = 1 << 21;
+  for (long long r0 = 0; r0 < all.M; r0 += PART) {
+    cube_sample_args a = all;
+    a.M = (int)(all.M - r0 < PART ? all.M - r0 : PART);
+    a.logits = (const T*)all.logits + r0 * all.ld;
+    a.u += r0;
+    a.token += r0;
+    if (a.prob) a.prob += r0;
+    if (a.temperature) a.temperature += r0;
+    if (a.top_k) a.top_k += r0;
+    if (a.top_p) a.top_p += r0;
+    if (a.min_p) a.min_p += r0;
+    f(a);
+    CUBE_CHECK_LAUNCH("cube_sample_rows");
+  }
   return CUBE_OK;
 }
 
-template <class T, int WG> int launch_mid(const cube_sample_args& a, int S, hipStream_t st) {
+template <class T> int launch_short(const cube_sample_args& all, int S, hipStream_t st) {
+  return in_parts<T>(all, [&](const cube_sample_args& a) {
+    const dim3 grid((a.M + 3) / 4), block(256);
+    if (a.V <= 64) hipLaunchKernelGGL((sample_short_kernel<T, 1>), grid, block, 0, st, a, S);
+    else if (a.V <= 128) hipLaunchKernelGGL((sample_short_kernel<T, 2>), grid, block, 0, st, a, S);
+    else hipLaunchKernelGGL((sample_short_kernel<T, 4>), grid, block, 0, st, a, S);
+  });
+}
+
+template <class T, int WG> int launch_mid(const cube_sample_args& all, int S, hipStream_t st) {
   static CubeLdsReservation lds;
-  const size_t bytes = sizeof(Scratch) + sizeof(Few) + 4 * (size_t)((a.V + 2 * Granule<T>::N + 3) / 4 * 4);
+  const size_t bytes = sizeof(Scratch) + sizeof(Few) + 4 * (size_t)((all.V + 2 * Granule<T>::N + 3) / 4 * 4);
   if (!lds.ensure((const void*)sample_mid_kernel<T, WG>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
-  hipLaunchKernelGGL((sample_mid_kernel<T, WG>), dim3(a.M), dim3(WG), bytes, st, a, S);
-  CUBE_CHECK_LAUNCH("cube_sample_rows");
-  return CUBE_OK;
+  return in_parts<T>(all, [&](const cube_sample_args& a) { hipLaunchKernelGGL((sample_mid_kernel<T, WG>), dim3(a.M), dim3(WG), bytes, st, a, S); });
 }
 
 int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
@@ -1658,9 +1677,7 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
     static CubeLdsReservation lds;
     constexpr size_t all = bytes + sizeof(HalfScratch);
     if (!lds.ensure((const void*)half_row_kernel<T>, all)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
-    hipLaunchKernelGGL((half_row_kernel<T>), dim3(a.M), dim3(HWG), all, st, a, S);
-    CUBE_CHECK_LAUNCH("cube_sample_rows");
-    return CUBE_OK;
+    return in_parts<T>(a, [&](const cube_sample_args& part) { hipLaunchKernelGGL((half_row_kernel<T>), dim3(part.M), dim3(HWG), all, st, part, S); });
   }
   static CubeLdsReservation lds, lds2;
   constexpr size_t kept = KEPT_BYTES;

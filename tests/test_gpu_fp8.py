@@ -129,6 +129,16 @@ def test_quant_of_strided_rows(dev, t, col, pad):
     assert torch.equal(a.q, b.q) and torch.equal(a.scale, b.scale)
 
 
+def test_quant_of_more_rows_than_a_launch_has_threads_for(dev):
+    """2^28 rows of one column and a few: bytes and scales of the first and last rows, and of those around every 2^27th."""
+    M = (1 << 28) + 37
+    x = torch.arange(M, device=dev, dtype=torch.int32).remainder_(1000).add_(1).half()[:, None]
+    rows = hip.quant_fp8(x)
+    for r in (0, (1 << 27) - 9, (1 << 27) + 3, (1 << 28) - 20, M - 17):
+        part = hip.quant_fp8(x[r:r + 17])
+        assert torch.equal(rows.q[r:r + 17], part.q) and torch.equal(rows.scale[:, r:r + 17], part.scale)
+
+
 def test_quant_writes_nothing_behind_its_rows(dev):
     """Through the C ABI with wider leading dimensions: the bytes between the rows and behind the last one stay."""
     x = torch.randn(5, 200, device=dev)

@@ -248,6 +248,19 @@ def test_limits_near_the_row(dev, V, k, t):
     check(z, u, k=k, p=0.9, T=2.0)
 
 
+@pytest.mark.parametrize("M,V", [(70_000_001, 2), (17_000_003, 257)])
+def test_more_rows_than_a_launch_has_threads_for(dev, M, V):
+    """The arg-max and a draw of two candidates in rows spread over tens of millions, settings and random numbers per row."""
+    z = torch.full((M, V), -50.0, dtype=torch.bfloat16, device=dev)
+    at = torch.arange(M, device=dev) % V
+    z[torch.arange(M, device=dev), at] = 2.0
+    u = torch.full((M,), 0.5, dtype=torch.float64, device=dev)
+    T = torch.ones(M, device=dev)
+    T[::2] = 0.0
+    token, prob = hip.sample_rows(z, u, temperature=T)
+    assert torch.equal(token.long(), at) and bool((prob == 1).all())
+
+
 def test_two_streams_at_once(dev):
     """Calls of every form on two streams with nothing between them."""
     cases = [logits(M, V, t, dev, seed=11) + (kw,) for M, V, t in ((500, 102, "f32"), (20, 5000, "bf16"), (8, 60000, "f32"), (8, 60000, "bf16"), (4, 60000, "f16"))
