@@ -21,7 +21,7 @@
 //           that matters are sorted;
 //   half    16-bit logits have 65536 values: a workgroup counts every value of a row (or of a slice of it) in LDS, and everything
 //           is decided from the counts, with one exponential for each value that occurs;
-//   long    f32: slices of a row meet in a histogram and in a list of the few logits that can still decide.
+//   long    f32 and few f16 rows: slices of a row meet in a histogram and in a list of the few logits that can still decide.
 #include <type_traits>
 
 #include "common.h"
@@ -766,7 +766,8 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
 // ---- half: 16-bit logits by the counts of their values ----------------------------------------------------------------------
 // A slice's counts: one 32-bit word per magnitude (the 15 bits without the sign), the number of its logits in the low half and
 // of its negative ones in the high half; a slice has at most 65528 logits, so neither runs over.  Groups of 64 * E magnitudes, E
-// to a lane: an octave of bf16, half an octave of f16 (quarters of that took 65 us where these take 38, 1 x 250002: a row then has 130 groups).
+// to a lane: an octave of bf16, half an octave of f16 (quarters of that, 128 x 250002: 88 us, these 60:
+// a row then has 130 groups).
 // In the candidates' order group g comes GROUPS - 1 - g-th for positive values, falling inside, and GROUPS + g-th for negative
 // ones, rising.
 constexpr int HWG = 1024;
@@ -1283,7 +1284,7 @@ __global__ __launch_bounds__(HWG) void half_row_kernel(cube_sample_args a, int S
   find_half(s, row, 0, row.granules, s.raw, s.tie, s.ties, &a.token[r]);
 }
 
-// ---- long: f32 rows in slices side by side -----------------------------------------------------------------------------------
+// ---- long: f32 rows (and few f16 ones) in slices side by side ------------------------------------------------------------------
 // 1 largest key of every slice, and the row's histogram cleared;  2 histogram over steps of the logit: counts for a top-k row,
 // weights for another;  3 the bins in which the targets can fall are known: their logits into the row's list;  4 one workgroup
 // decides from the list and the histogram.  A list that runs over (very many equal logits) sends the fourth launch over the
@@ -1306,21 +1307,22 @@ __device__ __forceinline__ uint32_t row_top(const LongRow& l, int slices, Scratc
   return block_max<LWG>(s, (int)threadIdx.x < slices ? l.top[threadIdx.x] : 0u);
 }
 
-__global__ __launch_bounds__(LWG) void long_top_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
+template <class T> __global__ __launch_bounds__(LWG) void long_top_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
   __shared__ uint32_t part[LWG / 64];
+  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y, slices = gridDim.x;
   LongRow& l = rows[blockIdx.y];
   for (int b = blockIdx.x * LWG + threadIdx.x; b < LONG_BINS; b += slices * LWG) l.hist[b] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) { l.heavy = 0; l.listed = 0; }
-  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   float largest = -INFINITY;
 #pragma unroll 4
   for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-    float v[4];
+    float v[N];
     row.values(j, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) largest = fmaxf(largest, v[i]);
+    for (int i = 0; i < N; ++i) largest = fmaxf(largest, v[i]);
   }
   uint32_t best = wave_max(key_of(largest));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = best;
@@ -1331,9 +1333,10 @@ __global__ __launch_bounds__(LWG) void long_top_kernel(cube_sample_args a, int r
   }
 }
 
-__global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int r0, LongRow* rows, int per, int S) {
+template <class T> __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int r0, LongRow* rows, int per, int S) {
   __shared__ uint64_t hist[LONG_BINS];
   __shared__ Scratch s;
+  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y;
   LongRow& l = rows[blockIdx.y];
   const Settings st(a, r);
@@ -1342,15 +1345,15 @@ __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int 
   for (int b = threadIdx.x; b < LONG_BINS; b += LWG) hist[b] = 0;
   __syncthreads();
   const Steps step(value_of(best), st.temp, LONG_BINS);
-  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   auto all = [&](auto f) {
 #pragma unroll 2
     for (int j = lo + threadIdx.x; j < hi; j += LWG) {
-      float v[4];
+      float v[N];
       row.values(j, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f(v[i]);
+      for (int i = 0; i < N; ++i) f(v[i]);
     }
   };
   if (st.limited(a.V)) {
@@ -1397,8 +1400,9 @@ template <class G> __device__ Open open_bins(Scratch& s, const Runs& r, const Se
   return o;
 }
 
-__global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
+template <class T> __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
   __shared__ Scratch s;
+  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y, lane = threadIdx.x & 63;
   LongRow& l = rows[blockIdx.y];
   const Settings st(a, r);
@@ -1420,23 +1424,25 @@ __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int 
       if (o.ends) end = (int)o.end.bin;
     }
   }
-  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   const float largest = value_of(best);
   const Span span(step, from, to), last(step, end < 0 ? from : end, end < 0 ? to : end);
 #pragma unroll 2
   for (int j0 = lo; j0 < hi; j0 += LWG) {
     const int j = j0 + threadIdx.x;
-    float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = -INFINITY;
     if (j < hi) row.values(j, v);
     bool some = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) some |= span.near(v[i]) | last.near(v[i]);
+    for (int i = 0; i < N; ++i) some |= span.near(v[i]) | last.near(v[i]);
     if (__ballot(some) == 0) continue;
     uint32_t n = 0;
-    bool in[4];
+    bool in[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       in[i] = (span.has(step, v[i]) || last.has(step, v[i])) && (!st.greedy() || v[i] == largest);
       n += in[i];
     }
@@ -1446,9 +1452,9 @@ __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int 
     if (lane == 63) base = atomicAdd(&l.listed, incl);
     uint32_t at = lane_value(base, 63) + incl - n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
       if (in[i]) {
-        if (at < LIST) l.list[at] = entry_of(key_of(v[i]), (uint32_t)(j * 4 + i - row.lead));
+        if (at < LIST) l.list[at] = entry_of(key_of(v[i]), (uint32_t)(j * N + i - row.lead));
         ++at;
       }
   }
@@ -1461,14 +1467,15 @@ struct ListKeys {
     for (int i = threadIdx.x; i < n; i += LWG) f((uint32_t)(list[i] >> 32));
   }
 };
-struct RowKeys {
-  const Row<float>& row;
+template <class T> struct RowKeys {
+  const Row<T>& row;
   template <class F> __device__ __forceinline__ void operator()(F f) const {
+    constexpr int N = Granule<T>::N;
     for (int j = threadIdx.x; j < row.granules; j += LWG) {
-      float v[4];
+      float v[N];
       row.values(j, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f(key_of(v[i]));
+      for (int i = 0; i < N; ++i) f(key_of(v[i]));
     }
   }
 };
@@ -1483,11 +1490,12 @@ template <class E> __device__ Place search(Scratch& s, E each, const Weigher& w,
   return refine<LWG, D1, false>(s, each, w, f.bin, f.before, target);
 }
 
-__global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, int r0, LongRow* rows, int slices, int S) {
+template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, int r0, LongRow* rows, int slices, int S) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Scratch& s = *(Scratch*)smem;
   Few& few = *(Few*)(smem + sizeof(Scratch));
   uint64_t* list = (uint64_t*)(smem + sizeof(Scratch) + sizeof(Few));
+  constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.x;
   LongRow& l = rows[blockIdx.x];
   const Settings st(a, r);
@@ -1496,7 +1504,7 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
     if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
-  const Row<float> row((const float*)a.logits + (size_t)r * a.ld, a.V);
+  const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const bool whole = l.listed > LIST;  // the list ran over: decide from the row itself
   const int n = whole ? 0 : (int)l.listed;
   for (int i = threadIdx.x; i < n; i += LWG) list[i] = l.list[i];
@@ -1507,7 +1515,7 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
   if (!st.greedy()) {
     const Weigher w(st, value_of(best), S);
     if (whole) {
-      c = decide<LWG>(s, RowKeys{row}, st, w, a.V);
+      c = decide<LWG>(s, RowKeys<T>{row}, st, w, a.V);
     } else if (st.limited(a.V)) {
       if (n <= FEW) {
         for (int i = threadIdx.x; i < n; i += LWG) few.entry[i] = list[i];
@@ -1573,10 +1581,10 @@ __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, in
     };
     if (whole) {
       for (int j = threadIdx.x; j < row.granules; j += LWG) {
-        float v[4];
+        float v[N];
         row.values(j, v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (key_of(v[i]) == c.key) add((uint32_t)(j * 4 + i - row.lead));
+        for (int i = 0; i < N; ++i) if (key_of(v[i]) == c.key) add((uint32_t)(j * N + i - row.lead));
       }
     } else {
       for (int i = threadIdx.x; i < n; i += LWG) if ((uint32_t)(list[i] >> 32) == c.key) add(~(uint32_t)list[i]);
@@ -1628,11 +1636,11 @@ template <class T, int WG> int launch_mid(const cube_sample_args& all, int S, hi
   return in_parts<T>(all, [&](const cube_sample_args& a) { hipLaunchKernelGGL((sample_mid_kernel<T, WG>), dim3(a.M), dim3(WG), bytes, st, a, S); });
 }
 
-int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
+template <class T> int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
   static CubeLdsReservation lds;
   const size_t bytes = sizeof(Scratch) + sizeof(Few) + 8 * LIST;
-  if (!lds.ensure((const void*)long_choose_kernel, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
-  const int granules = (a.V + 2 * 4 - 2) / 4;  // of a row that starts inside a granule
+  if (!lds.ensure((const void*)long_choose_kernel<T>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
+  const int granules = (a.V + 2 * Granule<T>::N - 2) / Granule<T>::N;  // of a row that starts inside a granule
   for (int r0 = 0; r0 < a.M; r0 += ROWS_AT_ONCE) {
     const int n = a.M - r0 < ROWS_AT_ONCE ? a.M - r0 : ROWS_AT_ONCE;
     // slices of one granule a thread at least, about two workgroups a CU over all rows
@@ -1642,10 +1650,10 @@ int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
     slices = slices < MAX_SLICES ? slices : MAX_SLICES;
     const int per = (granules + slices - 1) / slices;
     const dim3 grid(slices, n);
-    hipLaunchKernelGGL(long_top_kernel, grid, dim3(LWG), 0, st, a, r0, ws, per);
-    hipLaunchKernelGGL(long_hist_kernel, grid, dim3(LWG), 0, st, a, r0, ws, per, S);
-    hipLaunchKernelGGL(long_list_kernel, grid, dim3(LWG), 0, st, a, r0, ws, per);
-    hipLaunchKernelGGL(long_choose_kernel, dim3(n), dim3(LWG), bytes, st, a, r0, ws, slices, S);
+    hipLaunchKernelGGL((long_top_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
+    hipLaunchKernelGGL((long_hist_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per, S);
+    hipLaunchKernelGGL((long_list_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
+    hipLaunchKernelGGL((long_choose_kernel<T>), dim3(n), dim3(LWG), bytes, st, a, r0, ws, slices, S);
     CUBE_CHECK_LAUNCH("cube_sample_rows");
   }
   return CUBE_OK;
@@ -1696,12 +1704,21 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
 // has eight times as many values to an octave: 256 x 32000, top-p 31 against 33, but top-k 33 against 17 and 1 x 20000 24 against 16.
 template <class T> constexpr int half_v() { return std::is_same<T, bf16_t>::value ? 16000 : MID_V; }
 
+// Rows that go through slices, histogram and list: f32 beyond what a workgroup holds; of f16 up to 32 rows of 2^23 logits in all, while
+// counting by value costs more (us, plain and top-p: 1 x 250002 20 and 25 against 36 and 39;  32 x 40000 25 and 29 against 34 and 36;
+// 32 x 250002 49 and 52 against 48 and 51;  64 x 40000 33 and 39 against 28 and 30).  bf16 has too many equal values for the list
+// (1 x 250002, top-p 30 against 22).
+bool sliced(int type, int M, int V) {
+  return V > MID_V && (type == CUBE_T_F32 || (type == CUBE_T_F16 && M <= 32 && (long long)M * V <= 1 << 23));
+}
+
 template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStream_t st) {
   if (a.V <= SHORT_V) return launch_short<T>(a, S, st);
+  if constexpr (!std::is_same<T, bf16_t>::value) {
+    if (sliced(a.type, a.M, a.V)) return launch_long<T>(a, S, (LongRow*)ws, st);
+  }
   if constexpr (sizeof(T) == 2) {
     if (a.V > half_v<T>()) return launch_half<T>(a, S, (HalfSlice*)ws, st);
-  } else {
-    if (a.V > MID_V) return launch_long(a, S, (LongRow*)ws, st);
   }
   // 256 threads keep several rows on a CU; above 4096 logits a row's own passes are what takes time
   return a.V <= 4096 ? launch_mid<T, 256>(a, S, st) : launch_mid<T, 1024>(a, S, st);
@@ -1711,7 +1728,7 @@ template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStr
 
 extern "C" size_t cube_sample_workspace_bytes(int type, int M, int V) {
   if (M <= 0 || V <= 0 || V > CUBE_SAMPLE_MAX_V) return 0;
-  if (type == CUBE_T_F32) return V > MID_V ? sizeof(LongRow) * (size_t)(M < ROWS_AT_ONCE ? M : ROWS_AT_ONCE) : 0;
+  if (type == CUBE_T_F32 || sliced(type, M, V)) return V > MID_V ? sizeof(LongRow) * (size_t)(M < ROWS_AT_ONCE ? M : ROWS_AT_ONCE) : 0;
   if (V <= (type == CUBE_T_BF16 ? half_v<bf16_t>() : half_v<_Float16>())) return 0;
   const HalfPlan p = half_plan(M, V);
   return p.slices > 1 ? sizeof(HalfSlice) * (size_t)p.slices * p.rows : 0;

@@ -248,6 +248,20 @@ def test_limits_near_the_row(dev, V, k, t):
     check(z, u, k=k, p=0.9, T=2.0)
 
 
+@pytest.mark.parametrize("M,V", [(32, 33000), (33, 33000), (32, 262144), (32, 262145), (60, 33000)])
+def test_f16_rows_around_the_change_of_form(dev, M, V):
+    """Few f16 rows go another way than many: the same tokens from both, for the same rows."""
+    z, u = logits(64, V, "f16", dev, seed=21)
+    for s in (dict(), dict(top_k=30, top_p=0.9), dict(top_p=0.7), dict(min_p=0.02)):
+        many, few = hip.sample_rows(z, u, **s), hip.sample_rows(z[:M], u[:M], **s)
+        assert torch.equal(few[0], many[0][:M])
+        np.testing.assert_allclose(few[1].cpu(), many[1][:M].cpu(), rtol=2.0 ** -22)
+    check(z[:2], u[:2], p=0.8)
+    flat = torch.zeros(M, V, dtype=torch.float16, device=dev)       # one value: the list runs over
+    check(flat[:2], u[:2], p=0.5)
+    assert torch.equal(hip.sample_rows(flat, u[:M], top_p=0.5)[0], hip.sample_rows(flat.repeat(3, 1), u[:M].repeat(3), top_p=0.5)[0][:M])
+
+
 @pytest.mark.parametrize("M,V", [(70_000_001, 2), (17_000_003, 257)])
 def test_more_rows_than_a_launch_has_threads_for(dev, M, V):
     """The arg-max and a draw of two candidates in rows spread over tens of millions, settings and random numbers per row."""
