@@ -449,9 +449,10 @@ int cube_linear_fp8(const cube_fp8_args* args, void* ws, size_t ws_bytes, void* 
  * kept candidate at which the running sum of w exceeds u times the kept sum (u in [0, 1), one per row, clamped to it);
  * prob (may be NULL) = its w over that sum.  temperature <= 0 or NaN: the arg-max, prob 1.  A row without candidates: token
  * -1, prob 0.  NaN logits are no candidates; +inf logits share the whole weight.
- * temperature / top_k / top_p / min_p: device arrays of M, or NULL for the scalar beside each.  Weights are added in 64-bit
- * fixed point: the token does not depend on how the row is split.  V <= CUBE_SAMPLE_MAX_V; token and prob share no byte with an
- * input.                                                                                                                  */
+ * temperature / top_k / top_p / min_p: device arrays of M, or NULL for the scalar beside each.  Weights are added as integers: the
+ * token does not depend on how the row is split.  They are exponentials to 2^-50 of themselves, cut to a whole 2^-62 of the largest
+ * (V <= 256: rounded to 2^-46), so a border lies within 2^-48 + V * 2^-62 (2^-39) of the total from where it would exactly.
+ * V <= CUBE_SAMPLE_MAX_V; token and prob share no byte with an input.                                                      */
 #define CUBE_SAMPLE_MAX_V (1 << 22)
 typedef struct cube_sample_args {
   const void* logits; int type; long long ld; int M; int V;

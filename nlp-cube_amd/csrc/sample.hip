@@ -6,14 +6,16 @@
 //   w_i >= m (the largest weight is 1).  All three are prefixes of the one order, so the kept set is the shortest of them.
 //   token = the first candidate whose running sum exceeds u * (sum of the kept set);  prob = its w / that sum.
 //
-// A long row is never sorted: every decision is "the first position where the running count or weight passes a target", and a
-// radix search over the sortable bits of the logit finds it -- a histogram of count or weight over the top bits, the bin in which
-// the target falls, the next bits inside that bin; at the last bits all members of a bin are equal and share one weight.
+// A long row is never sorted: every decision is "the first position where the running count or weight passes a target".  A histogram
+// in the candidates' order (equal steps of the logit, or the values of a 16-bit type) has the running sums; the few logits of the bin
+// in which the target falls are sorted.  Where they are not few, a radix search over the sortable bits of the logit goes on inside
+// it: at the last bits all members of a bin are equal and share one weight.
 //
-// Weights are 64-bit fixed point, w * 2^S rounded, with S such that V of them cannot overflow: integer sums do not depend on
-// their order, so a row gives the same token however it is divided among lanes and workgroups (and by whatever order its
-// atomics come in), and at 2^-41 or finer they decide as 64-bit floating point would (a 32-bit running sum over a large
-// vocabulary is off by more than the distance between two neighbouring tokens' borders).
+// Weights are integers, w * 2^62 cut off, and their sums have 96 bits: sums of integers do not depend on their order, so a row gives
+// the same token however it is divided among lanes and workgroups (and by whatever order its atomics come in).  V cut weights are off
+// by less than V * 2^-62 of the largest, 2^-40 for the longest row (64-bit sums leave a weight 62 - log2 V bits, and put a flat tail of
+// 2^22 logits off by up to 2^-19 of the mass, hundreds of tokens' shares; they take 64 x 32003 25 us where these take 28, 128 x 250002
+// f32 110 where these take 120).  Up to 256 logits, w * 2^46 rounded and sums of 64 bits do: 256 * 2^-47 = 2^-39.
 //
 // Forms, by the length and type of a row (sizes measured at the entry point below):
 //   short   up to 256 logits: one wave sorts the row by counting;
@@ -70,6 +72,71 @@ template <class T> struct Row {
   }
 };
 
+// ---- sums of weights ------------------------------------------------------------------------------------------------------
+
+struct Sum {  // 96 bits
+  uint64_t lo; uint32_t hi;
+  Sum() = default;
+  __device__ __forceinline__ constexpr Sum(uint64_t l, uint32_t h = 0) : lo(l), hi(h) {}
+};
+// word by word with the carry: comparisons of 64 bits take more than the additions
+__device__ __forceinline__ uint64_t add64(uint64_t a, uint64_t b, uint32_t& carry) {
+  uint32_t c;
+  const uint32_t l = __builtin_addc((uint32_t)a, (uint32_t)b, 0u, &c);
+  const uint32_t h = __builtin_addc((uint32_t)(a >> 32), (uint32_t)(b >> 32), c, &carry);
+  return (uint64_t)h << 32 | l;
+}
+__device__ __forceinline__ Sum operator+(Sum a, Sum b) {
+  uint32_t c;
+  const uint64_t l = add64(a.lo, b.lo, c);
+  return {l, a.hi + b.hi + c};
+}
+__device__ __forceinline__ Sum subtract(Sum a, Sum b, uint32_t& borrow) {
+  uint32_t c, d;
+  const uint32_t l = __builtin_subc((uint32_t)a.lo, (uint32_t)b.lo, 0u, &c);
+  const uint32_t h = __builtin_subc((uint32_t)(a.lo >> 32), (uint32_t)(b.lo >> 32), c, &d);
+  const uint32_t t = __builtin_subc(a.hi, b.hi, d, &borrow);
+  return {(uint64_t)h << 32 | l, t};
+}
+__device__ __forceinline__ Sum operator-(Sum a, Sum b) { uint32_t c; return subtract(a, b, c); }
+__device__ __forceinline__ bool operator<(Sum a, Sum b) { uint32_t c; subtract(a, b, c); return c != 0; }
+__device__ __forceinline__ Sum& operator+=(Sum& a, Sum b) { return a = a + b; }
+__device__ __forceinline__ bool operator<=(Sum a, Sum b) { return !(b < a); }
+__device__ __forceinline__ bool operator==(Sum a, Sum b) { return a.lo == b.lo && a.hi == b.hi; }
+__device__ __forceinline__ uint64_t choose(bool c, uint64_t a, uint64_t b) { return c ? a : b; }
+__device__ __forceinline__ Sum choose(bool c, Sum a, Sum b) { return {c ? a.lo : b.lo, c ? a.hi : b.hi}; }  // (c ? a : b of structures is one of two addresses)
+template <class V> __device__ __forceinline__ V smaller(V a, V b) { return choose(b < a, b, a); }
+__device__ __forceinline__ Sum times(uint32_t n, uint64_t w) {
+  const uint64_t p = (uint64_t)n * (uint32_t)w, q = (uint64_t)n * (uint32_t)(w >> 32) + (p >> 32);
+  return {(q << 32) | (uint32_t)p, (uint32_t)(q >> 32)};
+}
+__device__ __forceinline__ double to_double(uint64_t s) { return (double)s; }
+__device__ __forceinline__ double to_double(Sum s) { return fma((double)s.hi, 18446744073709551616.0, (double)s.lo); }
+// the whole part of 0 <= d < 2^96
+template <class V> __device__ __forceinline__ V whole(double d);
+template <> __device__ __forceinline__ uint64_t whole<uint64_t>(double d) { return (uint64_t)d; }
+template <> __device__ __forceinline__ Sum whole<Sum>(double d) {
+  const uint32_t hi = (uint32_t)(d * 5.421010862427522e-20);  // 2^-64
+  return {(uint64_t)fma((double)hi, -18446744073709551616.0, d), hi};
+}
+// d / one, where that is a number of logits
+__device__ __forceinline__ uint32_t quotient(Sum d, uint64_t one) {
+  uint32_t q = (uint32_t)(to_double(d) / (double)one);
+  if (d < times(q, one)) --q;
+  else if (times(q + 1, one) <= d) ++q;
+  return q;
+}
+// a sum that many threads add to: the 64 bits, and what was carried out of them
+__device__ __forceinline__ void add_to(uint64_t* lo, uint32_t* hi, uint64_t w) {
+  const uint64_t old = atomicAdd((unsigned long long*)lo, (unsigned long long)w);
+  if (old + w < old) atomicAdd(hi, 1u);
+}
+__device__ __forceinline__ void add_to(uint64_t* lo, uint32_t* hi, Sum w) {
+  uint32_t c;
+  add64(atomicAdd((unsigned long long*)lo, (unsigned long long)w.lo), w.lo, c);
+  if (w.hi + c) atomicAdd(hi, w.hi + c);
+}
+
 // ---- settings and weights -------------------------------------------------------------------------------------------------
 
 struct Settings {
@@ -85,31 +152,30 @@ struct Settings {
   __device__ bool greedy() const { return !(temp > 0.0f); }
   __device__ bool limited(int V) const { return k > 0 && k < V; }
   // first position whose running sum passes this target ends the top-p set of a total
-  __device__ uint64_t goal(uint64_t total) const {
-    const double g = ceil((p > 0.0f ? (double)p : 0.0) * (double)total);
-    return g >= 1.0 ? (uint64_t)g - 1 : 0;
+  template <class V> __device__ V goal(V total) const {
+    const double g = ceil((p > 0.0f ? (double)p : 0.0) * to_double(total));
+    return choose(g >= 1.0, whole<V>(g) - V(1), V(0));
   }
-  __device__ uint64_t draw(uint64_t kept) const {
-    const uint64_t t = (uint64_t)(u * (double)kept);
-    return t < kept ? t : kept - 1;
+  template <class V> __device__ V draw(V kept) const {
+    const V t = whole<V>(u * to_double(kept));
+    return choose(t < kept, t, kept - V(1));
   }
 };
 
 struct Weigher {
   double top, per_t, floor_x;  // largest logit, log2(e) / T, log2(min-p)
-  int S;
   // An infinite logit beside an infinite largest one has weight 1 and every other none: the largest finite double in place of the
-  // infinity makes their differences infinite and -1.8e308, and power() ends the range on both sides.
-  __device__ Weigher(const Settings& s, float best, int bits) : S(bits) {
+  // infinity makes their differences infinite and -1.8e308, and parts() ends the range on both sides.
+  __device__ Weigher(const Settings& s, float best) {
     top = fmin((double)best, 1.7976931348623157e308);
     per_t = fmax(1.4426950408889634 / (double)s.temp, 1e-290);
     floor_x = s.m > 0.0f ? log2(s.m < 1.0f ? (double)s.m : 1.0) : -INFINITY;
   }
   __device__ __forceinline__ double x(float v) const { return ((double)v - top) * per_t; }  // log2 of the weight
-  // 2^(x + shift): x = n + f with |f| <= 1/2 (adding 1.5 * 2^52 rounds x to n and leaves n in the low bits), 2^f = 1 + f * P(f),
-  // P of the 9th degree through (2^f - 1) / f at the Chebyshev nodes (2^-50 of the value), n + shift added to the exponent bits.
-  // What is no candidate (NaN, -inf) comes out at 2^-960, as nothing.
-  __device__ __forceinline__ double power(double x, int shift) const {
+  // 2^x = e * 2^n: x = n + f with |f| <= 1/2 (adding 1.5 * 2^52 rounds x to n and leaves n in the low bits), e = 2^f = 1 + f * P(f),
+  // P of the 9th degree through (2^f - 1) / f at the Chebyshev nodes (2^-50 of the value).  What is no candidate (NaN, -inf) comes
+  // out at 2^-960, as nothing.
+  __device__ __forceinline__ double parts(double x, int& n) const {
     const double y = fmin(fmax(x, -960.0), 0.0);
     const double t = y + 6755399441055744.0;
     const double f = y - (t - 6755399441055744.0);
@@ -124,15 +190,32 @@ struct Weigher {
     e = fma(e, f, 0.24022650695910075);
     e = fma(e, f, 0.6931471805599462);
     e = fma(e, f, 1.0);
-    return __hiloint2double(__double2hiint(e) + ((__double2loint(t) + shift) << 20), __double2loint(e));
+    n = __double2loint(t);
+    return e;
   }
-  // to an integer: at 2^52 a double's last place is 1, and its low bits are the sum (S <= 46)
+  __device__ __forceinline__ double power(double x, int shift) const {  // 2^(x + shift): added to the exponent bits
+    int n;
+    const double e = parts(x, n);
+    return __hiloint2double(__double2hiint(e) + ((n + shift) << 20), __double2loint(e));
+  }
+  // 2^(x + 62) cut off: the fraction of e with its leading 1 in bit 62, moved down by what is missing to the exponent 62 (rounded
+  // through two additions of large powers of two the middle form took 3 % more time)
   __device__ __forceinline__ uint64_t at(double x) const {
-    return (uint64_t)__double_as_longlong(power(x, S) + 4503599627370496.0) & 0xfffffffffffffull;
+    int n;
+    const double e = parts(x, n);
+    const uint32_t hi = (uint32_t)__double2hiint(e), lo = (uint32_t)__double2loint(e);
+    const uint64_t f = ((uint64_t)((__builtin_amdgcn_alignbit(hi, lo, 22) & 0x3fffffffu) | 0x40000000u) << 32) | (lo << 10);
+    const int down = 1023 - n - (int)(hi >> 20);
+    return f >> (down < 63 ? down : 63);
   }
   __device__ __forceinline__ uint64_t of(float v) const { return at(x(v)); }
   __device__ __forceinline__ uint64_t operator()(uint32_t key) const { return of(value_of(key)); }
-  __device__ __forceinline__ float prob(float v, uint64_t kept) const { return (float)(power(x(v), S) / (double)kept); }
+  // the same for sums of up to 256 weights in 64 bits, 2^(x + 46) rounded: at 2^52 a double's last place is 1, and its low bits are the sum
+  __device__ __forceinline__ uint64_t few(double x) const {
+    return (uint64_t)__double_as_longlong(power(x, 46) + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ float prob(float v, Sum kept) const { return (float)(power(x(v), 62) / to_double(kept)); }
+  __device__ __forceinline__ float prob(float v, uint64_t kept) const { return (float)(power(x(v), 46) / (double)kept); }
 };
 
 // ---- wave and workgroup helpers -------------------------------------------------------------------------------------------
@@ -145,6 +228,7 @@ template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t from_lane(uint
 template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t from_lane(uint64_t v) {
   return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)v) | ((uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32);
 }
+template <int CTRL, int ROWS> __device__ __forceinline__ Sum from_lane(Sum v) { return {from_lane<CTRL, ROWS>(v.lo), from_lane<CTRL, ROWS>(v.hi)}; }
 template <class V> __device__ __forceinline__ V wave_scan(V v) {  // inclusive
   v += from_lane<0x111, 0xf>(v);
   v += from_lane<0x112, 0xf>(v);
@@ -158,8 +242,10 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (u
 __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
   return (uint64_t)lane_value((uint32_t)v, lane) | ((uint64_t)lane_value((uint32_t)(v >> 32), lane) << 32);
 }
+__device__ __forceinline__ Sum lane_value(Sum v, int lane) { return {lane_value(v.lo, lane), lane_value(v.hi, lane)}; }
 template <class V> __device__ __forceinline__ V wave_sum(V v) { return lane_value(wave_scan(v), 63); }
-template <class V> __device__ __forceinline__ V larger(V a, V b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <class V> __device__ __forceinline__ V larger(V a, V b) { return choose(b < a, a, b); }
 template <class V> __device__ __forceinline__ V wave_max(V v) {
   v = larger(v, from_lane<0x111, 0xf>(v));
   v = larger(v, from_lane<0x112, 0xf>(v));
@@ -173,15 +259,20 @@ template <class V> __device__ __forceinline__ V wave_max(V v) {
 constexpr int D1 = 11, D2 = 10;  // bits of the first two digits of a key within a workgroup; the third has the rest
 constexpr int LOW_BINS = 1 << D2;
 
-struct Scratch {  // of a workgroup, in LDS
-  uint64_t high[1 << D1];   // first digit
+struct alignas(16) Scratch {  // of a workgroup, in LDS
+  uint64_t high[1 << D1];   // first digit, or steps of the logit
   uint64_t low[LOW_BINS];   // second digit (64-bit sums), third digit (twice as many 32-bit counts)
-  uint64_t part[16];
+  Sum part[16];
+  Sum before, in;
   uint32_t part32[16];
-  uint64_t before;
   uint32_t bin;
+  // What sums of weights carry out of 64 bits lies in the other array: `low` is idle while `high` is filled, and a thread takes its bins
+  // of `high` into registers (hold) before `low` is filled.
+  __device__ uint32_t* high_carry() { return (uint32_t*)low; }
+  __device__ uint32_t* low_carry() { return (uint32_t*)high; }
 };
 static_assert(sizeof(Scratch) % 16 == 0, "keys behind it are read 16 bytes at a time");
+static_assert(sizeof(Scratch::low) >= (4 << D1) && sizeof(Scratch::high) >= 4 * LOW_BINS, "room for the carries");
 
 template <int WG> __device__ uint32_t block_max(Scratch& s, uint32_t v) {
   v = wave_max(v);
@@ -192,180 +283,213 @@ template <int WG> __device__ uint32_t block_max(Scratch& s, uint32_t v) {
   __syncthreads();
   return v;
 }
-template <int WG> __device__ uint64_t block_sum(Scratch& s, uint64_t v) {
+// the running sums (inclusive) of a workgroup's waves, lane l: waves 0 .. l
+template <int WG, class V> __device__ __forceinline__ V over_waves(const V* part) {
+  static_assert(WG / 64 <= 16, "one row of lanes");
+  const int lane = threadIdx.x & 63;
+  V v = part[lane < WG / 64 ? lane : 0];
+  v = choose(lane < WG / 64, v, V(0));
+  v += from_lane<0x111, 0xf>(v);
+  v += from_lane<0x112, 0xf>(v);
+  if constexpr (WG / 64 > 4) {
+    v += from_lane<0x114, 0xf>(v);
+    v += from_lane<0x118, 0xf>(v);
+  }
+  return v;
+}
+template <int WG> __device__ Sum block_sum(Scratch& s, Sum v) {
   v = wave_sum(v);
   if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int i = 0; i < WG / 64; ++i) v += s.part[i];
+  v = over_waves<WG>(s.part);
   __syncthreads();
-  return v;
+  return lane_value(v, WG / 64 - 1);
 }
 
-// Bins from the top one down, a run of neighbours per thread: what lies before this thread's run, and in it.
-struct Runs { uint64_t before, sum, total; };
-template <int WG, int BINS, class G> __device__ Runs scan_bins(Scratch& s, G get) {
+// A histogram's bins in the candidates' order in registers, a run of neighbours per thread: what is in each, what lies before the run,
+// in it, and in all.  UP: the order is from the first bin up, else from the last one down.
+template <class V, int C> struct Held { V v[C]; V before, sum, total; };
+template <bool UP, int BINS> __device__ __forceinline__ int bin_at(int place) { return UP ? place : BINS - 1 - place; }
+template <int WG, int BINS, bool UP, class G> __device__ auto hold(Scratch& s, G get) {
   static_assert(BINS % WG == 0, "whole runs");
   constexpr int C = BINS / WG;
-  Runs r;
-  r.sum = 0;
+  typedef decltype(get(0)) V;
+  Held<V, C> r;
+  r.sum = V(0);
 #pragma unroll
-  for (int c = 0; c < C; ++c) r.sum += get(BINS - 1 - (int)threadIdx.x * C - c);
-  const uint64_t incl = wave_scan(r.sum);
-  if ((threadIdx.x & 63) == 63) s.part[threadIdx.x >> 6] = incl;
+  for (int c = 0; c < C; ++c) r.sum += r.v[c] = get(bin_at<UP, BINS>((int)threadIdx.x * C + c));
+  const V incl = wave_scan(r.sum);
+  V* part = (V*)s.part;
+  if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = incl;
   __syncthreads();
-  r.before = incl - r.sum;
-  r.total = 0;
-#pragma unroll
-  for (int i = 0; i < WG / 64; ++i) {
-    if (i < (int)(threadIdx.x >> 6)) r.before += s.part[i];
-    r.total += s.part[i];
-  }
+  const V waves = over_waves<WG>(part);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  r.before = lane_value(waves, wave) - part[wave] + (incl - r.sum);
+  r.total = lane_value(waves, WG / 64 - 1);
   __syncthreads();
   return r;
 }
-// the bin in which the running sum passes target - base (base + total > target), and base + what lies before it
-struct Found { uint32_t bin; uint64_t before; };
-template <int WG, int BINS, class G> __device__ Found find_bin(Scratch& s, const Runs& r, uint64_t base, uint64_t target, G get) {
-  constexpr int C = BINS / WG;
-  uint64_t before = base + r.before;
+// the bin in which the running sum passes target - base (base + total > target), base + what lies before it, and what is in it
+template <class V> struct Found { uint32_t bin; V before, in; };
+template <int WG, int BINS, bool UP, class V, int C> __device__ Found<V> find_bin(Scratch& s, const Held<V, C>& r, V base, V target) {
+  static_assert(C == BINS / WG, "");
+  V before = base + r.before;
   if (before <= target && target < before + r.sum) {
-    int b = BINS - 1 - (int)threadIdx.x * C;
-    for (int c = 0; c < C; ++c, --b) {
-      const uint64_t v = get(b);
-      if (target < before + v) break;
-      before += v;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (before <= target && target < before + r.v[c]) {
+        s.bin = (uint32_t)bin_at<UP, BINS>((int)threadIdx.x * C + c);
+        *(V*)&s.before = before;
+        *(V*)&s.in = r.v[c];
+      }
+      before += r.v[c];
     }
-    s.bin = b;
-    s.before = before;
   }
   __syncthreads();
-  const Found f = {s.bin, s.before};
+  const Found<V> f = {s.bin, *(const V*)&s.before, *(const V*)&s.in};
   __syncthreads();
   return f;
 }
 
 // Inside the bin `bin` of the first `DIG1` bits: the key at which the running count (COUNT) or weight passes `target`, the place of
 // the position among the logits equal to it, and how many those are.  each(f) calls f(key) for every logit of the bin at least.
-struct Place { uint32_t key, tie, ties; uint64_t before, one; __device__ uint64_t end() const { return before + (uint64_t)(tie + 1) * one; } };
-template <int WG, int DIG1, bool COUNT, class E>
-__device__ Place refine(Scratch& s, E each, const Weigher& w, uint32_t bin, uint64_t before, uint64_t target) {
+struct Place { uint32_t key, tie, ties; Sum before; uint64_t one; __device__ Sum end() const { return before + times(tie + 1, one); } };
+template <int WG, int DIG1, bool COUNT, class V, class E>
+__device__ Place refine(Scratch& s, E each, const Weigher& w, uint32_t bin, V before, V target) {
   constexpr int D3 = 32 - DIG1 - D2;
   static_assert((4 << D3) <= (int)sizeof(s.low), "the third digit's counts fit");
-  for (int b = threadIdx.x; b < LOW_BINS; b += WG) s.low[b] = 0;
+  static_assert(std::is_same<V, typename std::conditional<COUNT, uint64_t, Sum>::type>::value, "");
+  uint32_t* carry = s.low_carry();
+  for (int b = threadIdx.x; b < LOW_BINS; b += WG) { s.low[b] = 0; if (!COUNT) carry[b] = 0; }
   __syncthreads();
   each([&](uint32_t k) {
-    if (k >> (32 - DIG1) == bin) atomicAdd((unsigned long long*)&s.low[(k >> D3) & (LOW_BINS - 1)], (unsigned long long)(COUNT ? 1 : w(k)));
+    if (k >> (32 - DIG1) == bin) {
+      const uint32_t at = (k >> D3) & (LOW_BINS - 1);
+      if constexpr (COUNT) atomicAdd((unsigned long long*)&s.low[at], 1ull);
+      else add_to(&s.low[at], &carry[at], w(k));
+    }
   });
   __syncthreads();
-  auto second = [&](int b) { return s.low[b]; };
-  const Found f = find_bin<WG, LOW_BINS>(s, scan_bins<WG, LOW_BINS>(s, second), before, target, second);
+  const Found<V> f = find_bin<WG, LOW_BINS, false>(s, hold<WG, LOW_BINS, false>(s, [&](int b) {
+    if constexpr (COUNT) return s.low[b];
+    else return Sum(s.low[b], carry[b]);
+  }), before, target);
   const uint32_t prefix = (bin << D2) | f.bin;
   uint32_t* cnt = (uint32_t*)s.low;
   for (int b = threadIdx.x; b < (1 << D3); b += WG) cnt[b] = 0;
   __syncthreads();
   each([&](uint32_t k) { if (k >> D3 == prefix) atomicAdd(&cnt[k & ((1 << D3) - 1)], 1u); });
   __syncthreads();
-  auto third = [&](int b) { return cnt[b] ? (uint64_t)cnt[b] * (COUNT ? 1 : w((prefix << D3) | (uint32_t)b)) : 0; };
-  const Found h = find_bin<WG, 1 << D3>(s, scan_bins<WG, 1 << D3>(s, third), f.before, target, third);
+  const Found<V> h = find_bin<WG, 1 << D3, false>(s, hold<WG, 1 << D3, false>(s, [&](int b) {
+    if constexpr (COUNT) return (uint64_t)cnt[b];
+    else return times(cnt[b], cnt[b] ? w((prefix << D3) | (uint32_t)b) : 0);
+  }), f.before, target);
   Place at;
   at.key = (prefix << D3) | h.bin;
-  at.one = COUNT ? 1 : w(at.key);
-  at.before = h.before;
-  at.tie = (uint32_t)((target - h.before) / at.one);
   at.ties = cnt[h.bin];
+  if constexpr (COUNT) {
+    at.one = 1;
+    at.before = 0;
+    at.tie = (uint32_t)(target - h.before);
+  } else {
+    at.one = w(at.key);
+    at.before = h.before;
+    at.tie = quotient(target - h.before, at.one);
+  }
   __syncthreads();
   return at;
 }
 
 // A row's whole decision by one workgroup: which key, the how-manieth of the logits equal to it, and the kept sum.
-struct Choice { uint32_t key, tie; uint64_t kept; };
+struct Choice { uint32_t key, tie; Sum kept; };
 template <int WG, class E> __device__ Choice decide(Scratch& s, E each, const Settings& st, const Weigher& w, int V) {
-  auto first = [&](int b) { return s.high[b]; };
+  constexpr int BINS = 1 << D1;
   uint32_t least = 1;      // keys below it are outside the top-k set
-  uint64_t surplus = 0;    // weight of the logits equal to the last of the top-k set that are outside it
+  Sum surplus = 0;         // weight of the logits equal to the last of the top-k set that are outside it
   if (st.limited(V)) {
-    for (int b = threadIdx.x; b < (1 << D1); b += WG) s.high[b] = 0;
+    for (int b = threadIdx.x; b < BINS; b += WG) s.high[b] = 0;
     __syncthreads();
     each([&](uint32_t k) { if (k) atomicAdd((unsigned long long*)&s.high[k >> (32 - D1)], 1ull); });
     __syncthreads();
-    const Runs r = scan_bins<WG, 1 << D1>(s, first);
+    const auto r = hold<WG, BINS, false>(s, [&](int b) { return s.high[b]; });
     if ((uint64_t)st.k < r.total) {
       const uint64_t t = (uint64_t)st.k - 1;
-      const Found f = find_bin<WG, 1 << D1>(s, r, 0, t, first);
+      const Found<uint64_t> f = find_bin<WG, BINS, false>(s, r, (uint64_t)0, t);
       const Place at = refine<WG, D1, true>(s, each, w, f.bin, f.before, t);
       least = at.key;
-      surplus = (uint64_t)(at.ties - at.tie - 1) * w(at.key);
+      surplus = times(at.ties - at.tie - 1, w(at.key));
     }
   }
-  for (int b = threadIdx.x; b < (1 << D1); b += WG) s.high[b] = 0;
+  uint32_t* carry = s.high_carry();
+  for (int b = threadIdx.x; b < BINS; b += WG) { s.high[b] = 0; carry[b] = 0; }
   __syncthreads();
-  uint64_t heavy = 0;  // weight of those that min-p keeps
+  Sum heavy = 0;  // weight of those that min-p keeps
   each([&](uint32_t k) {
     if (k >= least) {
       const double x = w.x(value_of(k));
       const uint64_t v = w.at(x);
-      if (v) atomicAdd((unsigned long long*)&s.high[k >> (32 - D1)], (unsigned long long)v);
+      if (v) add_to(&s.high[k >> (32 - D1)], &carry[k >> (32 - D1)], v);
       if (x >= w.floor_x) heavy += v;
     }
   });
   __syncthreads();
-  const Runs r = scan_bins<WG, 1 << D1>(s, first);
-  const uint64_t total = r.total - surplus;
-  uint64_t kept = total;
+  const auto r = hold<WG, BINS, false>(s, [&](int b) { return Sum(s.high[b], carry[b]); });
+  const Sum total = r.total - surplus;
+  Sum kept = total;
   if (st.p < 1.0f) {
-    const uint64_t t = st.goal(total);
+    const Sum t = st.goal(total);
     if (t < total) {
-      const Found f = find_bin<WG, 1 << D1>(s, r, 0, t, first);
-      const uint64_t end = refine<WG, D1, false>(s, each, w, f.bin, f.before, t).end();
-      kept = end < kept ? end : kept;
+      const Found<Sum> f = find_bin<WG, BINS, false>(s, r, Sum(0), t);
+      const Sum end = refine<WG, D1, false>(s, each, w, f.bin, f.before, t).end();
+      kept = smaller(end, kept);
     }
   }
   if (st.m > 0.0f) {
     heavy = block_sum<WG>(s, heavy);
-    kept = heavy < kept ? heavy : kept;
+    kept = smaller(heavy, kept);
   }
-  const uint64_t t = st.draw(kept);
-  const Found f = find_bin<WG, 1 << D1>(s, r, 0, t, first);
+  const Sum t = st.draw(kept);
+  const Found<Sum> f = find_bin<WG, BINS, false>(s, r, Sum(0), t);
   const Place at = refine<WG, D1, false>(s, each, w, f.bin, f.before, t);
   return {at.key, at.tie, kept};
 }
 
 // One wave, candidates in order: lane l has the places l*E .. l*E + E - 1 (key 0 behind the last).  All that a row needs beyond its
-// first V is there, or st.k bounds it.  -> the chosen place
-template <int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Settings& st, const Weigher& w, int V, float& prob) {
+// first V is there, or st.k bounds it.  -> the chosen place.  W: the sums' type (uint64_t where the row has no more than these logits)
+template <class W, int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Settings& st, const Weigher& w, int V, float& prob) {
+  static_assert(E <= 4, "");
   const int lane = threadIdx.x & 63;
   const bool limited = st.limited(V);
-  uint64_t wt[E], run[E], sum = 0;
+  uint64_t wt[E];
+  W run[E], sum = W(0);
   double x[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     x[e] = w.x(value_of(q[e]));
-    wt[e] = q[e] && !(limited && lane * E + e >= st.k) ? w.at(x[e]) : 0;
+    wt[e] = q[e] && !(limited && lane * E + e >= st.k) ? (std::is_same<W, Sum>::value ? w.at(x[e]) : w.few(x[e])) : 0;
     sum += wt[e];
     run[e] = sum;
   }
-  const uint64_t incl = wave_scan(sum), before = incl - sum;
-  const uint64_t total = lane_value(incl, 63);
-  uint64_t kept = total;
-  const uint64_t goal = st.goal(total);
+  const W incl = wave_scan(sum), before = incl - sum;
+  const W total = lane_value(incl, 63);
+  W kept = total;
+  const W goal = st.goal(total);
   if (st.p < 1.0f || st.m > 0.0f) {
-    uint64_t mine = 0;  // running sum at the last place of this lane that stays
+    W mine = W(0);  // running sum at the last place of this lane that stays
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const uint64_t c = before + run[e];
+      const W c = before + run[e];
       const bool stays = wt[e] && (!(st.p < 1.0f) || c - wt[e] <= goal) && (!(st.m > 0.0f) || x[e] >= w.floor_x);
-      mine = stays ? c : mine;
+      mine = choose(stays, c, mine);
     }
     kept = wave_max(mine);
   }
-  const uint64_t t = st.draw(kept);
+  const W t = st.draw(kept);
   int at = 0;
   float pr = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const uint64_t c = before + run[e];
+    const W c = before + run[e];
     if (c - wt[e] <= t && t < c) { at = lane * E + e; pr = w.prob(value_of(q[e]), kept); }
   }
   const int owner = __ffsll(__ballot(before <= t && t < incl)) - 1;
@@ -378,7 +502,7 @@ template <int E> __device__ int choose_sorted(const uint32_t (&q)[E], const Sett
 // reads).  Then a lane holds E neighbouring places, and sums and searches are wave scans.
 constexpr int SHORT_V = 256;
 template <class T, int E>
-__global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, int S) {
+__global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a) {
   __shared__ __attribute__((aligned(16))) uint32_t s_key[4][64 * E];
   __shared__ uint32_t s_order[4][64 * E], s_sorted[4][64 * E];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, V = a.V;
@@ -469,9 +593,9 @@ __global__ __launch_bounds__(256) void sample_short_kernel(cube_sample_args a, i
   uint32_t q[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) q[e] = s_sorted[wave][lane * E + e];
-  const Weigher w(st, value_of(best), S);
+  const Weigher w(st, value_of(best));
   float prob;
-  const int at = choose_sorted<E>(q, st, w, V, prob);
+  const int at = choose_sorted<uint64_t>(q, st, w, V, prob);
   if (lane == 0) { a.token[r] = (int)s_order[wave][at]; if (a.prob) a.prob[r] = prob; }
 }
 
@@ -484,7 +608,7 @@ struct alignas(16) Few {  // in LDS
   uint32_t n;
   uint32_t key, index;
   float prob;
-  uint64_t end;
+  Sum end;
 };
 static_assert(sizeof(Few) % 16 == 0, "keys behind it are read 16 bytes at a time");
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
@@ -512,17 +636,18 @@ template <int WG> __device__ void sort_few(Few& f) {
 }
 // One wave: in the sorted entries, with `before` in front of them, the first place whose running weight exceeds target (there is
 // one) -> f.key, f.index, f.end (the running weight up to and with it)
-__device__ void place_few(Few& f, const Weigher& w, uint64_t before, uint64_t target) {
+__device__ void place_few(Few& f, const Weigher& w, Sum before, Sum target) {
   constexpr int E = FEW / 64;
   const int lane = threadIdx.x & 63;
-  uint64_t q[E], wt[E], sum = 0;
+  uint64_t q[E], wt[E];
+  Sum sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     q[e] = f.sorted[lane * E + e];
     wt[e] = q[e] ? w((uint32_t)(q[e] >> 32)) : 0;
     sum += wt[e];
   }
-  uint64_t c = before + wave_scan(sum) - sum;
+  Sum c = before + (wave_scan(sum) - sum);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (c <= target && target < c + wt[e]) {
@@ -564,27 +689,20 @@ struct Span {
   }
 };
 
-// Bins from the first one up, a run of neighbours per thread.
-template <int WG, int BINS, class G> __device__ Runs scan_up(Scratch& s, G get) {
-  return scan_bins<WG, BINS>(s, [&](int b) { return get(BINS - 1 - b); });
-}
-template <int WG, int BINS, class G> __device__ Found find_up(Scratch& s, const Runs& r, uint64_t target, G get) {
-  Found f = find_bin<WG, BINS>(s, r, 0, target, [&](int b) { return get(BINS - 1 - b); });
-  f.bin = BINS - 1 - f.bin;
-  return f;
-}
-
 // ---- mid: one workgroup a row, keys in LDS ----------------------------------------------------------------------------------
 constexpr int MID_V = 32768;
 
 // every thread four neighbouring logits at a time; n4: a multiple of four
 template <int WG> struct LdsValues {
   const float* at; int n4;
-  template <class F> __device__ __forceinline__ void values(F f) const {
+  template <class F> __device__ __forceinline__ void fours(F f) const {
     for (int i = 4 * (int)threadIdx.x; i < n4; i += 4 * WG) {
       const f32x4 v = *(const f32x4*)&at[i];
-      f(v[0]); f(v[1]); f(v[2]); f(v[3]);
+      f({v[0], v[1], v[2], v[3]});
     }
+  }
+  template <class F> __device__ __forceinline__ void values(F f) const {
+    fours([&](const float (&v)[4]) { f(v[0]); f(v[1]); f(v[2]); f(v[3]); });
   }
   template <class F> __device__ __forceinline__ void operator()(F f) const {
     values([&](float v) { f(key_of(v)); });
@@ -600,14 +718,32 @@ template <int WG> struct LdsValues {
     }
   }
 };
-// The weights of many logits into a histogram over steps; MIN_P: and the sum of those that min-p keeps
+// The weights of many logits into a histogram over steps; MIN_P: and the sum of those that min-p keeps.  N at a time: an addition that
+// says what was there before (for the carry) takes the LDS some hundred cycles, and these are on their way together.
 template <bool MIN_P> struct Gather {
-  const Weigher& w; const Steps& step; uint64_t* hist; uint64_t& heavy;
-  __device__ __forceinline__ void operator()(float v) const {
-    const double x = w.x(v);
-    const uint64_t one = w.at(x);
-    if (one) atomicAdd((unsigned long long*)&hist[step(v)], (unsigned long long)one);  // (none for what is no candidate)
-    if (MIN_P && x >= w.floor_x) heavy += one;
+  const Weigher& w; const Steps& step; uint64_t* hist; uint32_t* carry; Sum& heavy;
+  template <int N> __device__ __forceinline__ void operator()(const float (&v)[N]) const {
+    uint64_t one[N], old[N];
+    int b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double x = w.x(v[i]);
+      one[i] = w.at(x);
+      b[i] = step(v[i]);
+      if (MIN_P && x >= w.floor_x) heavy += one[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      old[i] = 0;
+      if (one[i]) old[i] = atomicAdd((unsigned long long*)&hist[b[i]], (unsigned long long)one[i]);  // (none for what is no candidate)
+    }
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) some |= old[i] + one[i] < old[i];
+    if (some) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) if (old[i] + one[i] < old[i]) atomicAdd(&carry[b[i]], 1u);
+    }
   }
 };
 
@@ -617,9 +753,9 @@ template <int WG, int BINS, class K>
 __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Settings& st, const Weigher& w, uint32_t best, int V) {
   static_assert(BINS <= (1 << D1) && BINS % WG == 0, "the histogram lies in Scratch::high");
   const Steps step(value_of(best), st.temp, BINS);
-  auto get = [&](int b) { return s.high[b]; };
+  uint32_t* carry = s.high_carry();
   auto clear = [&] {
-    for (int b = threadIdx.x; b < BINS; b += WG) s.high[b] = 0;
+    for (int b = threadIdx.x; b < BINS; b += WG) { s.high[b] = 0; carry[b] = 0; }
     if (threadIdx.x == 0) f.n = 0;
     __syncthreads();
   };
@@ -627,12 +763,12 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
     clear();
     keys.values([&](float v) { if (v > -INFINITY) atomicAdd((unsigned long long*)&s.high[step(v)], 1ull); });
     __syncthreads();
-    const Runs r = scan_up<WG, BINS>(s, get);
+    const auto r = hold<WG, BINS, true>(s, [&](int b) { return s.high[b]; });
     if ((uint64_t)st.k < r.total || r.total <= FEW) {
       uint32_t bin = BINS - 1;
       if ((uint64_t)st.k < r.total) {
-        const Found at = find_up<WG, BINS>(s, r, (uint64_t)st.k - 1, get);
-        if (at.before + s.high[at.bin] > FEW) return false;
+        const Found<uint64_t> at = find_bin<WG, BINS, true>(s, r, (uint64_t)0, (uint64_t)st.k - 1);
+        if (at.before + at.in > FEW) return false;
         bin = at.bin;
       }
       keys.inside(step, Span(step, 0, (int)bin), [&](float v, int i) { append(f, entry_of(key_of(v), (uint32_t)(i - lead))); });
@@ -643,7 +779,7 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
 #pragma unroll
         for (int e = 0; e < FEW / 64; ++e) q[e] = (uint32_t)(f.sorted[threadIdx.x * (FEW / 64) + e] >> 32);
         float prob;
-        const int at = choose_sorted<FEW / 64>(q, st, w, V, prob);
+        const int at = choose_sorted<Sum>(q, st, w, V, prob);
         if (threadIdx.x == 0) { f.index = ~(uint32_t)f.sorted[at]; f.prob = prob; }
       }
       __syncthreads();
@@ -652,14 +788,14 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
     // no more candidates than k: not limited
   }
   clear();
-  uint64_t heavy = 0;  // weight of those that min-p keeps
-  if (st.m > 0.0f) keys.values(Gather<true>{w, step, s.high, heavy});
-  else keys.values(Gather<false>{w, step, s.high, heavy});
+  Sum heavy = 0;  // weight of those that min-p keeps
+  if (st.m > 0.0f) keys.fours(Gather<true>{w, step, s.high, carry, heavy});
+  else keys.fours(Gather<false>{w, step, s.high, carry, heavy});
   __syncthreads();
-  const Runs r = scan_up<WG, BINS>(s, get);
+  const auto r = hold<WG, BINS, true>(s, [&](int b) { return Sum(s.high[b], carry[b]); });
   // the place in which the running weight passes a target: the members of its bin, sorted
-  auto place = [&](uint64_t target) {
-    const Found at = find_up<WG, BINS>(s, r, target, get);
+  auto place = [&](Sum target) {
+    const Found<Sum> at = find_bin<WG, BINS, true>(s, r, Sum(0), target);
     keys.inside(step, Span(step, (int)at.bin, (int)at.bin), [&](float v, int i) { append(f, entry_of(key_of(v), (uint32_t)(i - lead))); });
     __syncthreads();
     if (f.n > FEW) return false;
@@ -668,9 +804,9 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
     __syncthreads();
     return true;
   };
-  uint64_t kept = r.total;
+  Sum kept = r.total;
   if (st.p < 1.0f) {
-    const uint64_t t = st.goal(r.total);
+    const Sum t = st.goal(r.total);
     if (t < r.total) {
       if (!place(t)) return false;
       kept = f.end;
@@ -681,7 +817,7 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
   }
   if (st.m > 0.0f) {
     heavy = block_sum<WG>(s, heavy);
-    kept = heavy < kept ? heavy : kept;
+    kept = smaller(heavy, kept);
   }
   if (!place(st.draw(kept))) return false;
   if (threadIdx.x == 0) f.prob = w.prob(value_of(f.key), kept);
@@ -690,7 +826,7 @@ __device__ bool decide_few(Scratch& s, Few& f, const K& keys, int lead, const Se
 }
 
 template <class T, int WG>
-__global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int S) {
+__global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Scratch& s = *(Scratch*)smem;
   Few& few = *(Few*)(smem + sizeof(Scratch));
@@ -718,7 +854,7 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a, int 
   Choice c = {best, 0, 0};
   float prob = 1.0f;
   if (!st.greedy()) {
-    const Weigher w(st, value_of(best), S);
+    const Weigher w(st, value_of(best));
     if (decide_few<WG, WG == 256 ? 1024 : 2048>(s, few, each, row.lead, st, w, best, a.V)) {
       if (threadIdx.x == 0) { a.token[r] = (int)few.index; if (a.prob) a.prob[r] = few.prob; }
       return;
@@ -873,10 +1009,11 @@ __global__ __launch_bounds__(HWG) void half_count_kernel(cube_sample_args a, int
 }
 
 struct HalfScratch {  // in LDS
-  uint64_t weight[2 * MAX_GROUPS];  // by order; after prefix_half: running sums
+  Sum weight[2 * MAX_GROUPS];  // by order; after prefix_half: running sums
   uint32_t count[2 * MAX_GROUPS];
   uint64_t has[MAX_GROUPS / 64];
   uint64_t heavy;
+  uint32_t heavy_carry;
   uint32_t raw, tie, ties, slice;
   float prob;
   uint32_t part[HWG / 64];
@@ -979,7 +1116,7 @@ template <class T> __device__ __forceinline__ void prefix_half(HalfScratch& s) {
   constexpr int R = 2 * half_groups<T>() / 64;
   const int lane = threadIdx.x & 63;
   uint32_t c[R], cs = 0;
-  uint64_t w[R], ws = 0;
+  Sum w[R], ws = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     cs += s.count[lane * R + i];
@@ -998,43 +1135,42 @@ template <class T> __device__ __forceinline__ void prefix_half(HalfScratch& s) {
   __builtin_amdgcn_wave_barrier();
 }
 
-struct Spot { uint32_t raw, tie, ties; uint64_t before, one; __device__ uint64_t end() const { return before + (uint64_t)(tie + 1) * one; } };
+struct Spot { uint32_t raw, tie, ties; Sum before; uint64_t one; __device__ Sum end() const { return before + times(tie + 1, one); } };
 // One wave: the value at which the running count (BY_COUNT) or weight passes target (the total does); before, one: weights
-template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfScratch& s, const C& counts, const Weigher& w, uint64_t target) {
+template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfScratch& s, const C& counts, const Weigher& w, Sum target) {
   const int lane = threadIdx.x & 63;
   constexpr int E = Half<T>::E, R = 2 * half_groups<T>() / 64;
   // 64 running sums, R apart, then the R between them
-  auto sum = [&](int i) { return BY_COUNT ? (uint64_t)s.count[i] : s.weight[i]; };
+  auto sum = [&](int i) { return BY_COUNT ? Sum(s.count[i]) : s.weight[i]; };
   int order = R * (__ffsll(__ballot(target < sum(lane * R + R - 1))) - 1);
   order += __ffsll(__ballot(lane < R && target < sum(order + (lane < R ? lane : 0)))) - 1;
-  uint64_t bc = order > 0 ? s.count[order - 1] : 0, bw = order > 0 ? s.weight[order - 1] : 0;
+  Sum bc(order > 0 ? s.count[order - 1] : 0), bw = choose(order > 0, s.weight[order > 0 ? order - 1 : 0], Sum(0));
   const bool neg = order >= half_groups<T>();
   const int g = group_of<T>(order);
   uint32_t c[E];
   valid<T>(g, neg, counts.again(s, g), c);
-  uint64_t v[E], sw = 0;
+  Sum v[E], sw = 0;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    v[i] = c[i] ? (uint64_t)c[i] * w.of(half_value<T>(half_raw<T>(g, neg, i))) : 0;
+    v[i] = times(c[i], c[i] ? w.of(half_value<T>(half_raw<T>(g, neg, i))) : 0);
     sw += v[i];
   }
   // in falling order: negative values as they lie, positive ones from the other end
   const uint32_t sc = sum_of(c), ic = wave_scan(sc);
-  const uint64_t iw = wave_scan(sw);
+  const Sum iw = wave_scan(sw);
   bc += neg ? ic - sc : lane_value(ic, 63) - ic;
-  bw += neg ? iw - sw : lane_value(iw, 63) - iw;
+  bw += choose(neg, iw - sw, lane_value(iw, 63) - iw);
   Spot out = {0, 0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < E; ++j) {
     const uint32_t ci = neg ? c[j] : c[E - 1 - j];
-    const uint64_t vi = neg ? v[j] : v[E - 1 - j];
-    const uint64_t here = BY_COUNT ? bc : bw, mine = BY_COUNT ? ci : vi;
+    const Sum vi = choose(neg, v[j], v[E - 1 - j]);
+    const Sum here = choose(BY_COUNT, bc, bw), mine = choose(BY_COUNT, Sum(ci), vi);
     if (here <= target && target < here + mine) {
       out.raw = half_raw<T>(g, neg, neg ? j : E - 1 - j);
       out.ties = ci;
       out.before = bw;
-      out.one = vi;   // (of all of them; divided below)
-      out.tie = BY_COUNT ? (uint32_t)(target - here) : 0;
+      out.tie = BY_COUNT ? (uint32_t)(target - here).lo : 0;
     }
     bc += ci;
     bw += vi;
@@ -1045,16 +1181,16 @@ template <class T, bool BY_COUNT, class C> __device__ Spot spot_half(const HalfS
   out.ties = lane_value(out.ties, owner);
   out.before = lane_value(out.before, owner);
   out.one = w.of(half_value<T>(out.raw));
-  if (!BY_COUNT) out.tie = (uint32_t)((target - out.before) / out.one);
+  if (!BY_COUNT) out.tie = quotient(target - out.before, out.one);
   return out;
 }
 
 // The workgroup's decision for a row from its counts (s.has filled): s.raw, s.tie, s.ties, s.prob; false for an empty row.
-template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C& counts, const Settings& st, int V, int S) {
+template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C& counts, const Settings& st, int V) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr int E = Half<T>::E, GROUPS = half_groups<T>(), R = 2 * GROUPS / 64;
   for (int i = threadIdx.x; i < 2 * GROUPS; i += HWG) { s.weight[i] = 0; s.count[i] = 0; }
-  if (threadIdx.x == 0) s.heavy = 0;
+  if (threadIdx.x == 0) { s.heavy = 0; s.heavy_carry = 0; }
   __syncthreads();
   // the marked groups, the waves in turn: candidates of both signs
   auto groups = [&](auto f) {
@@ -1090,7 +1226,7 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
   }
   const unsigned long long hit = __ballot(sum_of(c) != 0);
   const int at = below ? __ffsll(hit) - 1 : 63 - __clzll((long long)hit);
-  const Weigher w(st, half_value<T>(lane_value(mine, at)), S);
+  const Weigher w(st, half_value<T>(lane_value(mine, at)));
   const bool greedy = st.greedy();
   if (!greedy) {
     groups([&](int g) {
@@ -1100,12 +1236,12 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
         uint32_t c[E];
         valid<T>(g, side != 0, p, c);
         if (!__ballot(sum_of(c) != 0)) continue;
-        uint64_t sum = 0, heavy = 0;
+        Sum sum = 0, heavy = 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           if (!__ballot(c[i] != 0)) continue;
           const double x = w.x(half_value<T>(half_raw<T>(g, side != 0, i)));
-          const uint64_t v = c[i] ? (uint64_t)c[i] * w.at(x) : 0;
+          const Sum v = times(c[i], w.at(x));
           sum += v;
           if (x >= w.floor_x) heavy += v;
         }
@@ -1113,7 +1249,7 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
         if (lane == 0) s.weight[side ? GROUPS + g : GROUPS - 1 - g] = sum;
         if (st.m > 0.0f) {
           heavy = wave_sum(heavy);
-          if (lane == 0 && heavy) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
+          if (lane == 0) add_to(&s.heavy, &s.heavy_carry, heavy);
         }
       }
     });
@@ -1124,19 +1260,22 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
     Spot at;
     float prob = 1.0f;
     if (greedy) {
-      at = spot_half<T, true>(s, counts, w, 0);
+      at = spot_half<T, true>(s, counts, w, Sum(0));
     } else {
-      uint64_t total = s.weight[2 * GROUPS - 1];
-      if (st.limited(V) && (uint32_t)st.k < s.count[2 * GROUPS - 1]) total = spot_half<T, true>(s, counts, w, (uint64_t)st.k - 1).end();
-      uint64_t kept = total;
+      Sum total = s.weight[2 * GROUPS - 1];
+      if (st.limited(V) && (uint32_t)st.k < s.count[2 * GROUPS - 1]) total = spot_half<T, true>(s, counts, w, Sum((uint64_t)st.k - 1)).end();
+      Sum kept = total;
       if (st.p < 1.0f) {
-        const uint64_t t = st.goal(total);
+        const Sum t = st.goal(total);
         if (t < total) {
-          const uint64_t end = spot_half<T, false>(s, counts, w, t).end();
-          kept = end < kept ? end : kept;
+          const Sum end = spot_half<T, false>(s, counts, w, t).end();
+          kept = smaller(end, kept);
         }
       }
-      if (st.m > 0.0f) kept = s.heavy < kept ? s.heavy : kept;
+      if (st.m > 0.0f) {
+        const Sum heavy(s.heavy, s.heavy_carry);
+        kept = smaller(heavy, kept);
+      }
       at = spot_half<T, false>(s, counts, w, st.draw(kept));
       prob = w.prob(half_value<T>(at.raw), kept);
     }
@@ -1219,7 +1358,7 @@ template <class T> __device__ void find_half(HalfScratch& s, const Row<T>& row, 
 
 // the counts of a row's slices -> its token
 template <class T>
-__global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, int r0, const HalfSlice* ws, int slices, int per, int S) {
+__global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, int r0, const HalfSlice* ws, int slices, int per) {
   extern __shared__ __attribute__((aligned(16))) uint32_t kept[];
   __shared__ HalfScratch s;
   __shared__ uint64_t has[HALF_SLICES][MAX_GROUPS / 64];
@@ -1235,7 +1374,7 @@ __global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, in
     for (int i = 0; i < slices; ++i) h |= has[i][threadIdx.x];
     s.has[threadIdx.x] = h;
   }
-  if (!decide_half<T>(s, counts, st, a.V, S)) {
+  if (!decide_half<T>(s, counts, st, a.V)) {
     if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
@@ -1268,7 +1407,7 @@ __global__ __launch_bounds__(HWG) void half_choose_kernel(cube_sample_args a, in
 
 // a row of one slice in one launch: the counts stay in LDS
 template <class T>
-__global__ __launch_bounds__(HWG) void half_row_kernel(cube_sample_args a, int S) {
+__global__ __launch_bounds__(HWG) void half_row_kernel(cube_sample_args a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t count[];
   HalfScratch& s = *(HalfScratch*)(count + MAGS);
   const int r = blockIdx.x;
@@ -1276,7 +1415,7 @@ __global__ __launch_bounds__(HWG) void half_row_kernel(cube_sample_args a, int S
   const Settings st(a, r);
   count_half(count, row, 0, row.granules);
   mark_half<T>(count, s.part, s.has, [](int, const Words<Half<T>::E>&) {});
-  if (!decide_half<T>(s, LdsCounts<T>{count}, st, a.V, S)) {
+  if (!decide_half<T>(s, LdsCounts<T>{count}, st, a.V)) {
     if (threadIdx.x == 0) { a.token[r] = -1; if (a.prob) a.prob[r] = 0.0f; }
     return;
   }
@@ -1298,9 +1437,12 @@ constexpr int MAX_SLICES = 256;
 struct LongRow {  // of the workspace
   uint64_t hist[LONG_BINS];
   uint64_t list[LIST];  // entries
+  uint32_t carry[LONG_BINS];  // out of hist
   uint64_t heavy;       // weight of those that min-p keeps
-  uint32_t top[MAX_SLICES];
+  uint32_t heavy_carry;
   uint32_t listed;
+  uint32_t top[MAX_SLICES];
+  __device__ Sum weight(int b) const { return {hist[b], carry[b]}; }
 };
 
 __device__ __forceinline__ uint32_t row_top(const LongRow& l, int slices, Scratch& s) {
@@ -1312,8 +1454,8 @@ template <class T> __global__ __launch_bounds__(LWG) void long_top_kernel(cube_s
   constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y, slices = gridDim.x;
   LongRow& l = rows[blockIdx.y];
-  for (int b = blockIdx.x * LWG + threadIdx.x; b < LONG_BINS; b += slices * LWG) l.hist[b] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) { l.heavy = 0; l.listed = 0; }
+  for (int b = blockIdx.x * LWG + threadIdx.x; b < LONG_BINS; b += slices * LWG) { l.hist[b] = 0; l.carry[b] = 0; }
+  if (blockIdx.x == 0 && threadIdx.x == 0) { l.heavy = 0; l.heavy_carry = 0; l.listed = 0; }
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
   const int lo = blockIdx.x * per, hi = lo + per < row.granules ? lo + per : row.granules;
   float largest = -INFINITY;
@@ -1333,7 +1475,7 @@ template <class T> __global__ __launch_bounds__(LWG) void long_top_kernel(cube_s
   }
 }
 
-template <class T> __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_sample_args a, int r0, LongRow* rows, int per, int S) {
+template <class T> __global__ __launch_bounds__(LWG, 8) void long_hist_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
   __shared__ uint64_t hist[LONG_BINS];
   __shared__ Scratch s;
   constexpr int N = Granule<T>::N;
@@ -1342,7 +1484,9 @@ template <class T> __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_
   const Settings st(a, r);
   const uint32_t best = row_top(l, gridDim.x, s);
   if (best == 0 || st.greedy()) return;
-  for (int b = threadIdx.x; b < LONG_BINS; b += LWG) hist[b] = 0;
+  uint32_t* carry = (uint32_t*)s.high;  // (row_top is done with it)
+  static_assert(sizeof(s.high) >= 4 * LONG_BINS, "room for the carries");
+  for (int b = threadIdx.x; b < LONG_BINS; b += LWG) { hist[b] = 0; carry[b] = 0; }
   __syncthreads();
   const Steps step(value_of(best), st.temp, LONG_BINS);
   const Row<T> row((const T*)a.logits + (size_t)r * a.ld, a.V);
@@ -1353,31 +1497,35 @@ template <class T> __global__ __launch_bounds__(LWG) void long_hist_kernel(cube_
       float v[N];
       row.values(j, v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f(v[i]);
+      for (int i = 0; i < N; i += 2) f({v[i], v[i + 1]});
     }
   };
   if (st.limited(a.V)) {
-    all([&](float v) { if (v > -INFINITY) atomicAdd((unsigned long long*)&hist[step(v)], 1ull); });
+    all([&](const float (&v)[2]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) if (v[i] > -INFINITY) atomicAdd((unsigned long long*)&hist[step(v[i])], 1ull);
+    });
   } else {
-    const Weigher w(st, value_of(best), S);
-    uint64_t heavy = 0;
+    const Weigher w(st, value_of(best));
+    Sum heavy = 0;
     if (st.m > 0.0f) {
-      all(Gather<true>{w, step, hist, heavy});
+      all(Gather<true>{w, step, hist, carry, heavy});
       heavy = wave_sum(heavy);
-      if ((threadIdx.x & 63) == 0 && heavy) atomicAdd((unsigned long long*)&l.heavy, (unsigned long long)heavy);
+      if ((threadIdx.x & 63) == 0) add_to(&l.heavy, &l.heavy_carry, heavy);
     } else {
-      all(Gather<false>{w, step, hist, heavy});
+      all(Gather<false>{w, step, hist, carry, heavy});
     }
   }
   __syncthreads();
   for (int b = threadIdx.x; b < LONG_BINS; b += LWG)
-    if (hist[b]) atomicAdd((unsigned long long*)&l.hist[b], (unsigned long long)hist[b]);
+    if (hist[b] | carry[b]) add_to(&l.hist[b], &l.carry[b], Sum(hist[b], carry[b]));
 }
 
 // What the histogram of a row without a top-k limit leaves open: the bin that ends the top-p set (if that can be the shortest
 // prefix), and the bins among which the drawn position lies.
-struct Open { bool ends; Found end; uint64_t goal, least, most; uint32_t from, to; };
-template <class G> __device__ Open open_bins(Scratch& s, const Runs& r, const Settings& st, uint64_t heavy, G get) {
+struct Open { bool ends; Found<Sum> end; Sum goal, least, most; uint32_t from, to; };
+typedef Held<Sum, LONG_BINS / LWG> LongHeld;
+__device__ Open open_bins(Scratch& s, const LongHeld& r, const Settings& st, Sum heavy) {
   Open o;
   o.ends = false;
   o.least = o.most = r.total;
@@ -1385,22 +1533,22 @@ template <class G> __device__ Open open_bins(Scratch& s, const Runs& r, const Se
     o.goal = st.goal(r.total);
     if (o.goal < r.total) {
       o.ends = true;
-      o.end = find_up<LWG, LONG_BINS>(s, r, o.goal, get);
-      o.least = o.goal + 1;  // the set's sum is at least the goal and at most the end of the bin
-      o.most = o.end.before + get(o.end.bin);
+      o.end = find_bin<LWG, LONG_BINS, true>(s, r, Sum(0), o.goal);
+      o.least = o.goal + Sum(1);  // the set's sum is at least the goal and at most the end of the bin
+      o.most = o.end.before + o.end.in;
     }
   }
   if (st.m > 0.0f) {
     if (heavy <= o.least) o.ends = false;
-    o.least = heavy < o.least ? heavy : o.least;
-    o.most = heavy < o.most ? heavy : o.most;
+    o.least = smaller(heavy, o.least);
+    o.most = smaller(heavy, o.most);
   }
-  o.from = find_up<LWG, LONG_BINS>(s, r, st.draw(o.least), get).bin;
-  o.to = o.least == o.most ? o.from : find_up<LWG, LONG_BINS>(s, r, st.draw(o.most), get).bin;
+  o.from = find_bin<LWG, LONG_BINS, true>(s, r, Sum(0), st.draw(o.least)).bin;
+  o.to = o.least == o.most ? o.from : find_bin<LWG, LONG_BINS, true>(s, r, Sum(0), st.draw(o.most)).bin;
   return o;
 }
 
-template <class T> __global__ __launch_bounds__(LWG) void long_list_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
+template <class T> __global__ __launch_bounds__(LWG, 8) void long_list_kernel(cube_sample_args a, int r0, LongRow* rows, int per) {
   __shared__ Scratch s;
   constexpr int N = Granule<T>::N;
   const int r = r0 + blockIdx.y, lane = threadIdx.x & 63;
@@ -1412,13 +1560,12 @@ template <class T> __global__ __launch_bounds__(LWG) void long_list_kernel(cube_
   // candidates in the bins from .. to and in the bin `end` are listed; of a greedy row those equal to the largest
   int from = 0, to = 0, end = -1;
   if (!st.greedy()) {
-    auto get = [&](int b) { return l.hist[b]; };
-    const Runs runs = scan_up<LWG, LONG_BINS>(s, get);
     if (st.limited(a.V)) {
+      const auto counts = hold<LWG, LONG_BINS, true>(s, [&](int b) { return l.hist[b]; });
       to = LONG_BINS - 1;
-      if ((uint64_t)st.k < runs.total) to = (int)find_up<LWG, LONG_BINS>(s, runs, (uint64_t)st.k - 1, get).bin;
+      if ((uint64_t)st.k < counts.total) to = (int)find_bin<LWG, LONG_BINS, true>(s, counts, (uint64_t)0, (uint64_t)st.k - 1).bin;
     } else {
-      const Open o = open_bins(s, runs, st, l.heavy, get);
+      const Open o = open_bins(s, hold<LWG, LONG_BINS, true>(s, [&](int b) { return l.weight(b); }), st, Sum(l.heavy, l.heavy_carry));
       from = (int)o.from;
       to = (int)o.to;
       if (o.ends) end = (int)o.end.bin;
@@ -1460,7 +1607,7 @@ template <class T> __global__ __launch_bounds__(LWG) void long_list_kernel(cube_
   }
 }
 
-// the listed logits of a row (of one bin only where `bin` is not negative), or all of a row's
+// the listed logits of a row, or all of a row's
 struct ListKeys {
   const uint64_t* list; int n;
   template <class F> __device__ __forceinline__ void operator()(F f) const {
@@ -1480,17 +1627,17 @@ template <class T> struct RowKeys {
   }
 };
 // the key at which the running weight passes target among the keys that each() gives, `before` in front of them
-template <class E> __device__ Place search(Scratch& s, E each, const Weigher& w, uint64_t before, uint64_t target) {
-  for (int b = threadIdx.x; b < (1 << D1); b += LWG) s.high[b] = 0;
+template <class E> __device__ Place search(Scratch& s, E each, const Weigher& w, Sum before, Sum target) {
+  uint32_t* carry = s.high_carry();
+  for (int b = threadIdx.x; b < (1 << D1); b += LWG) { s.high[b] = 0; carry[b] = 0; }
   __syncthreads();
-  each([&](uint32_t k) { atomicAdd((unsigned long long*)&s.high[k >> (32 - D1)], (unsigned long long)w(k)); });
+  each([&](uint32_t k) { add_to(&s.high[k >> (32 - D1)], &carry[k >> (32 - D1)], w(k)); });
   __syncthreads();
-  auto first = [&](int b) { return s.high[b]; };
-  const Found f = find_bin<LWG, 1 << D1>(s, scan_bins<LWG, 1 << D1>(s, first), before, target, first);
+  const Found<Sum> f = find_bin<LWG, 1 << D1, false>(s, hold<LWG, 1 << D1, false>(s, [&](int b) { return Sum(s.high[b], carry[b]); }), before, target);
   return refine<LWG, D1, false>(s, each, w, f.bin, f.before, target);
 }
 
-template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, int r0, LongRow* rows, int slices, int S) {
+template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cube_sample_args a, int r0, LongRow* rows, int slices) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   Scratch& s = *(Scratch*)smem;
   Few& few = *(Few*)(smem + sizeof(Scratch));
@@ -1513,7 +1660,7 @@ template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cub
   Choice c = {best, 0, 0};
   float prob = 1.0f;
   if (!st.greedy()) {
-    const Weigher w(st, value_of(best), S);
+    const Weigher w(st, value_of(best));
     if (whole) {
       c = decide<LWG>(s, RowKeys<T>{row}, st, w, a.V);
     } else if (st.limited(a.V)) {
@@ -1526,19 +1673,18 @@ template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cub
           uint32_t q[FEW / 64];
 #pragma unroll
           for (int e = 0; e < FEW / 64; ++e) q[e] = (uint32_t)(few.sorted[threadIdx.x * (FEW / 64) + e] >> 32);
-          const int at = choose_sorted<FEW / 64>(q, st, w, a.V, prob);
+          const int at = choose_sorted<Sum>(q, st, w, a.V, prob);
           if (threadIdx.x == 0) { a.token[r] = (int)~(uint32_t)few.sorted[at]; if (a.prob) a.prob[r] = prob; }
         }
         return;
       }
       c = decide<LWG>(s, ListKeys{list, n}, st, w, a.V);
     } else {
-      auto get = [&](int b) { return l.hist[b]; };
       const Steps step(value_of(best), st.temp, LONG_BINS);
-      const Runs runs = scan_up<LWG, LONG_BINS>(s, get);
-      const Open o = open_bins(s, runs, st, l.heavy, get);
+      const LongHeld runs = hold<LWG, LONG_BINS, true>(s, [&](int b) { return l.weight(b); });
+      const Open o = open_bins(s, runs, st, Sum(l.heavy, l.heavy_carry));
       // where the running weight passes a target, inside a bin of the list: a few members are sorted, more are searched
-      auto place = [&](const Found& at, uint64_t target, Place& out) {
+      auto place = [&](const Found<Sum>& at, Sum target, Place& out) {
         for (int i = threadIdx.x; i < n; i += LWG) if (step((uint32_t)(list[i] >> 32)) == (int)at.bin) append(few, list[i]);
         __syncthreads();
         if (few.n <= FEW) {
@@ -1552,17 +1698,17 @@ template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cub
         }, w, at.before, target);
         return false;
       };
-      uint64_t kept = o.most;
+      Sum kept = o.most;
       Place at;
       if (o.ends) {
-        const uint64_t end = place(o.end, o.goal, at) ? few.end : at.end();
-        kept = end < kept ? end : kept;
+        const Sum end = place(o.end, o.goal, at) ? few.end : at.end();
+        kept = smaller(end, kept);
         __syncthreads();
         if (threadIdx.x == 0) few.n = 0;
         __syncthreads();
       }
-      const uint64_t t = st.draw(kept);
-      if (place(find_up<LWG, LONG_BINS>(s, runs, t, get), t, at)) {
+      const Sum t = st.draw(kept);
+      if (place(find_bin<LWG, LONG_BINS, true>(s, runs, Sum(0), t), t, at)) {
         if (threadIdx.x == 0) { a.token[r] = (int)few.index; if (a.prob) a.prob[r] = w.prob(value_of(few.key), kept); }
         return;
       }
@@ -1590,8 +1736,7 @@ template <class T> __global__ __launch_bounds__(LWG) void long_choose_kernel(cub
       for (int i = threadIdx.x; i < n; i += LWG) if ((uint32_t)(list[i] >> 32) == c.key) add(~(uint32_t)list[i]);
     }
     __syncthreads();
-    auto get = [&](int b) { return s.high[b]; };
-    const Found f = find_bin<LWG, 2048>(s, scan_bins<LWG, 2048>(s, get), 0, left, get);
+    const auto f = find_bin<LWG, 2048, false>(s, hold<LWG, 2048, false>(s, [&](int b) { return s.high[b]; }), (uint64_t)0, (uint64_t)left);
     prefix = (prefix << 11) | (2047 - f.bin);
     left -= (uint32_t)f.before;
   }
@@ -1620,23 +1765,23 @@ template <class T, class F> int in_parts(const cube_sample_args& all, F f) {
   return CUBE_OK;
 }
 
-template <class T> int launch_short(const cube_sample_args& all, int S, hipStream_t st) {
+template <class T> int launch_short(const cube_sample_args& all, hipStream_t st) {
   return in_parts<T>(all, [&](const cube_sample_args& a) {
     const dim3 grid((a.M + 3) / 4), block(256);
-    if (a.V <= 64) hipLaunchKernelGGL((sample_short_kernel<T, 1>), grid, block, 0, st, a, S);
-    else if (a.V <= 128) hipLaunchKernelGGL((sample_short_kernel<T, 2>), grid, block, 0, st, a, S);
-    else hipLaunchKernelGGL((sample_short_kernel<T, 4>), grid, block, 0, st, a, S);
+    if (a.V <= 64) hipLaunchKernelGGL((sample_short_kernel<T, 1>), grid, block, 0, st, a);
+    else if (a.V <= 128) hipLaunchKernelGGL((sample_short_kernel<T, 2>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((sample_short_kernel<T, 4>), grid, block, 0, st, a);
   });
 }
 
-template <class T, int WG> int launch_mid(const cube_sample_args& all, int S, hipStream_t st) {
+template <class T, int WG> int launch_mid(const cube_sample_args& all, hipStream_t st) {
   static CubeLdsReservation lds;
   const size_t bytes = sizeof(Scratch) + sizeof(Few) + 4 * (size_t)((all.V + 2 * Granule<T>::N + 3) / 4 * 4);
   if (!lds.ensure((const void*)sample_mid_kernel<T, WG>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
-  return in_parts<T>(all, [&](const cube_sample_args& a) { hipLaunchKernelGGL((sample_mid_kernel<T, WG>), dim3(a.M), dim3(WG), bytes, st, a, S); });
+  return in_parts<T>(all, [&](const cube_sample_args& a) { hipLaunchKernelGGL((sample_mid_kernel<T, WG>), dim3(a.M), dim3(WG), bytes, st, a); });
 }
 
-template <class T> int launch_long(const cube_sample_args& a, int S, LongRow* ws, hipStream_t st) {
+template <class T> int launch_long(const cube_sample_args& a, LongRow* ws, hipStream_t st) {
   static CubeLdsReservation lds;
   const size_t bytes = sizeof(Scratch) + sizeof(Few) + 8 * LIST;
   if (!lds.ensure((const void*)long_choose_kernel<T>, bytes)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
@@ -1651,9 +1796,9 @@ template <class T> int launch_long(const cube_sample_args& a, int S, LongRow* ws
     const int per = (granules + slices - 1) / slices;
     const dim3 grid(slices, n);
     hipLaunchKernelGGL((long_top_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
-    hipLaunchKernelGGL((long_hist_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per, S);
+    hipLaunchKernelGGL((long_hist_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
     hipLaunchKernelGGL((long_list_kernel<T>), grid, dim3(LWG), 0, st, a, r0, ws, per);
-    hipLaunchKernelGGL((long_choose_kernel<T>), dim3(n), dim3(LWG), bytes, st, a, r0, ws, slices, S);
+    hipLaunchKernelGGL((long_choose_kernel<T>), dim3(n), dim3(LWG), bytes, st, a, r0, ws, slices);
     CUBE_CHECK_LAUNCH("cube_sample_rows");
   }
   return CUBE_OK;
@@ -1678,14 +1823,14 @@ HalfPlan half_plan(int M, int V) {
   p.per = (granules + p.slices - 1) / p.slices;
   return p;
 }
-template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* ws, hipStream_t st) {
+template <class T> int launch_half(const cube_sample_args& a, HalfSlice* ws, hipStream_t st) {
   constexpr size_t bytes = 4 * MAGS;
   const HalfPlan p = half_plan(a.M, a.V);
   if (p.slices == 1) {
     static CubeLdsReservation lds;
     constexpr size_t all = bytes + sizeof(HalfScratch);
     if (!lds.ensure((const void*)half_row_kernel<T>, all)) CUBE_FAIL(CUBE_ERR_LAUNCH, "cube_sample_rows: LDS reservation failed");
-    return in_parts<T>(a, [&](const cube_sample_args& part) { hipLaunchKernelGGL((half_row_kernel<T>), dim3(part.M), dim3(HWG), all, st, part, S); });
+    return in_parts<T>(a, [&](const cube_sample_args& part) { hipLaunchKernelGGL((half_row_kernel<T>), dim3(part.M), dim3(HWG), all, st, part); });
   }
   static CubeLdsReservation lds, lds2;
   constexpr size_t kept = KEPT_BYTES;
@@ -1694,7 +1839,7 @@ template <class T> int launch_half(const cube_sample_args& a, int S, HalfSlice* 
   for (int r0 = 0; r0 < a.M; r0 += p.rows) {
     const int n = a.M - r0 < p.rows ? a.M - r0 : p.rows;
     hipLaunchKernelGGL((half_count_kernel<T>), dim3(p.slices, n), dim3(HWG), bytes, st, a, r0, ws, p.per);
-    hipLaunchKernelGGL((half_choose_kernel<T>), dim3(n), dim3(HWG), kept, st, a, r0, ws, p.slices, p.per, S);
+    hipLaunchKernelGGL((half_choose_kernel<T>), dim3(n), dim3(HWG), kept, st, a, r0, ws, p.slices, p.per);
     CUBE_CHECK_LAUNCH("cube_sample_rows");
   }
   return CUBE_OK;
@@ -1712,16 +1857,16 @@ bool sliced(int type, int M, int V) {
   return V > MID_V && (type == CUBE_T_F32 || (type == CUBE_T_F16 && M <= 32 && (long long)M * V <= 1 << 23));
 }
 
-template <class T> int launch(const cube_sample_args& a, int S, void* ws, hipStream_t st) {
-  if (a.V <= SHORT_V) return launch_short<T>(a, S, st);
+template <class T> int launch(const cube_sample_args& a, void* ws, hipStream_t st) {
+  if (a.V <= SHORT_V) return launch_short<T>(a, st);
   if constexpr (!std::is_same<T, bf16_t>::value) {
-    if (sliced(a.type, a.M, a.V)) return launch_long<T>(a, S, (LongRow*)ws, st);
+    if (sliced(a.type, a.M, a.V)) return launch_long<T>(a, (LongRow*)ws, st);
   }
   if constexpr (sizeof(T) == 2) {
-    if (a.V > half_v<T>()) return launch_half<T>(a, S, (HalfSlice*)ws, st);
+    if (a.V > half_v<T>()) return launch_half<T>(a, (HalfSlice*)ws, st);
   }
   // 256 threads keep several rows on a CU; above 4096 logits a row's own passes are what takes time
-  return a.V <= 4096 ? launch_mid<T, 256>(a, S, st) : launch_mid<T, 1024>(a, S, st);
+  return a.V <= 4096 ? launch_mid<T, 256>(a, st) : launch_mid<T, 1024>(a, st);
 }
 
 }  // namespace
@@ -1748,11 +1893,8 @@ extern "C" int cube_sample_rows(const cube_sample_args* a, void* ws, size_t ws_b
   const size_t need = cube_sample_workspace_bytes(a->type, a->M, a->V);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: workspace of %zu bytes (need %zu, 16-byte aligned)", ws_bytes, need);
-  int bits = 0;
-  while ((1 << bits) < a->V) ++bits;
-  const int S = 62 - bits < 46 ? 62 - bits : 46;  // V weights of at most 2^S stay below 2^63
   hipStream_t st = (hipStream_t)stream;
-  if (a->type == CUBE_T_F32) return launch<float>(*a, S, ws, st);
-  if (a->type == CUBE_T_BF16) return launch<bf16_t>(*a, S, ws, st);
-  return launch<_Float16>(*a, S, ws, st);
+  if (a->type == CUBE_T_F32) return launch<float>(*a, ws, st);
+  if (a->type == CUBE_T_BF16) return launch<bf16_t>(*a, ws, st);
+  return launch<_Float16>(*a, ws, st);
 }
