@@ -1253,8 +1253,8 @@ template <class T, class C> __device__ bool decide_half(HalfScratch& s, const C&
         }
       }
     });
-    __syncthreads();
   }
+  __syncthreads();  // of a greedy row too: every wave has read the counts that become running sums now
   if (wave == 0) {
     prefix_half<T>(s);
     Spot at;
