@@ -426,8 +426,8 @@ int cube_quant_fp8(const void* x, int x_type, long long ld_x, int M, int K, void
  * of quantised rows <= 2^24.  Sums beyond fp32's range become infinities.
  * 16-bit outputs come from the 8-bit matrix instructions, which keep 13 bits below the largest of 8 neighbouring products (about
  * 1.5e-5 of the result's 2-norm).  fp32 outputs have exact products: operand values from 2^-133 to below 2^128 are taken as they are,
- * smaller ones rounded to a multiple of 2^-133, 2^128 as infinity.  Scale byte 255 (E8M0's NaN) does not occur in quantised rows.
- * Calls on one stream need no synchronisation between them.                                                              */
+ * smaller ones rounded to a multiple of 2^-133, 2^128 as infinity.  tanh is within 2^-22 of itself before the output's rounding.
+ * Scale byte 255 (E8M0's NaN) does not occur in quantised rows.  Calls on one stream need no synchronisation between them.  */
 typedef struct cube_fp8_args {
   const void* A; int a_type; long long lda; const uint32_t* A_scale; int lds_a; int M;
   const void* W; long long ldw; const uint32_t* W_scale; int lds_w; int N; int K;
