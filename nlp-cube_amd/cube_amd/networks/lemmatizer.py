@@ -381,13 +381,15 @@ class Lemmatizer:
     def decode_batch(self, X, sampling=None):
         """-> (chars int32 [B, n], cases int32 [B, n]) arg-max (or, with `sampling`, drawn) sequences (NumPy), no logits kept."""
         self._require_gpu()
-        oc, ok, _, _ = self._decode(self._encode(X), max_steps=self.max_steps, sampling=sampling)
+        oc, ok, _, _ = self._decode(self._encode(X), max_steps=self.max_steps, sampling=None if sampling is None else sampling.begin())
         return oc, ok
 
     @hip.on_device
     def _decode_batches(self, batches, collate, sampling=None):
         """batches: iterable of lists of items for `collate`.  Yields (index, lemma strings) per batch, in order, with the
         host work of neighbouring batches (collate of the next, strings of the previous) under the device's decode."""
+        sampling = None if sampling is None else sampling.begin()
+
         def finish(k, h):
             oc, ok, _, _ = self._decode_finish(h)
             return k, self._strings(oc, ok)
@@ -504,7 +506,7 @@ class Lemmatizer:
     def process(self, doc, collate, batch_size=4, num_workers=4, merge=True, max_words=8192, sampling=None):
         """reference: lemmatizer.py:185-231.  `num_workers` is accepted and ignored.
         sampling (no counterpart in the reference): a `networks.sampling.Sampling`; the lemmas are drawn instead of decoded
-        greedily -- alternatives for an ambiguous word, one call each.
+        greedily -- alternatives for an ambiguous word, one call each (with a seed: one seed each).
         merge (no counterpart in the reference, results unchanged): the reference's in-order batches of
         `batch_size` words whose longest word has the same length (same S, hence the same pad positions
         for every word in them) run together as one device batch of up to `max_words` words; words do not

@@ -1,12 +1,14 @@
 """Sampled decoding: the settings of `cube_sample_rows` as a decoder takes them (no counterpart in the reference, whose decoder
 is greedy, cube/networks/lemmatizer.py:160-167)."""
+import copy
+
 import torch
 
 
 class Sampling:
     """temperature, top_k, top_p, min_p of a decoder's draws (numbers; include/cube_hip.h says what each keeps) and where their random
-    numbers come from: `seed` (the same draws every time for the same batches) or, where it is None, torch's own generator of the
-    device."""
+    numbers come from: `seed` (every call of process / decode_batch starts from it: the same draws every time for the same batches)
+    or, where it is None, torch's own generator of the device."""
 
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=None):
         if not temperature >= 0:
@@ -18,6 +20,12 @@ class Sampling:
         self.temperature, self.top_k, self.top_p, self.min_p = float(temperature), int(top_k), float(top_p), float(min_p)
         self.seed = seed
         self._generators = {}
+
+    def begin(self):
+        """The same settings at the start of their random numbers: what one call of a decoder draws from."""
+        s = copy.copy(self)
+        s._generators = {}
+        return s
 
     def uniforms(self, steps, rows, device):
         """float64 [steps, rows] in [0, 1) on the device."""
