@@ -5,6 +5,34 @@ import torch
 from cube_amd import hip
 
 
+class Fp8Weight(torch.Tensor):
+    """What an Fp8Linear answers with for `weight`: shape, type and device as of a Linear's weight; whatever computes with it gets the
+    values that the 8-bit rows stand for.  Read only.  (torch's encoder layers look at the weights of their Linear layers, and call the
+    layers only where one of them is of a class of its own, as this is.)"""
+
+    @staticmethod
+    def __new__(cls, rows, dtype):
+        return torch.Tensor._make_wrapper_subclass(cls, (rows.rows, rows.columns), dtype=dtype, device=rows.q.device)
+
+    def __init__(self, rows, dtype):
+        self._rows = rows
+
+    def __repr__(self):
+        return "Fp8Weight(%d, %d, dtype=%s, device=%s)" % (*self.shape, self.dtype, self.device)
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):   # its being here is what the layers look for
+        with torch._C.DisableTorchFunctionSubclass():
+            return func(*args, **(kwargs or {}))
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        if func._schema.is_mutable:
+            raise ValueError("an Fp8Linear's weight cannot be written: %s" % func)
+        args, kwargs = torch.utils._pytree.tree_map(lambda t: t._rows.float().to(t.dtype) if isinstance(t, cls) else t, (args, kwargs or {}))
+        return func(*args, **kwargs)
+
+
 class Fp8Linear(torch.nn.Module):
     """Stands for `linear` (same call, same shapes, the input's type out): e4m3 weights with one power-of-two scale per row and 128
     columns, activations quantised the same way per call, fp32 sums.  Made on the device of `linear`'s weight, an MI355X."""
@@ -16,6 +44,7 @@ class Fp8Linear(torch.nn.Module):
         self.register_buffer("q", rows.q)
         self.register_buffer("scale", rows.scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float())
+        self.register_buffer("kind", torch.empty(0, dtype=linear.weight.dtype, device=rows.q.device), persistent=False)   # the type that .half() and the like change
         self._rows = rows
 
     def _apply(self, fn, *args, **kwargs):
@@ -29,6 +58,10 @@ class Fp8Linear(torch.nn.Module):
     def _load_from_state_dict(self, *args, **kwargs):
         super()._load_from_state_dict(*args, **kwargs)
         self._rows = hip.Fp8Rows(self.q, self.scale, self.in_features)
+
+    @property
+    def weight(self):
+        return Fp8Weight(self._rows, self.kind.dtype)
 
     def forward(self, x):
         rows = x.reshape(-1, self.in_features)
