@@ -45,29 +45,28 @@ class Fp8Linear(torch.nn.Module):
         self.register_buffer("scale", rows.scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float())
         self.register_buffer("kind", torch.empty(0, dtype=linear.weight.dtype, device=rows.q.device), persistent=False)   # the type that .half() and the like change
-        self._rows = rows
+
+    @property
+    def rows(self):
+        """The weight as the kernels take it, from the buffers as they are now."""
+        return hip.Fp8Rows(self.q, self.scale, self.in_features)
 
     def _apply(self, fn, *args, **kwargs):
         bias = self.bias
         super()._apply(fn, *args, **kwargs)
         if bias is not None:
             self.bias = bias.to(self.q.device)   # .half() and the like round it: what is added to the sums stays fp32
-        self._rows = hip.Fp8Rows(self.q, self.scale, self.in_features)
         return self
-
-    def _load_from_state_dict(self, *args, **kwargs):
-        super()._load_from_state_dict(*args, **kwargs)
-        self._rows = hip.Fp8Rows(self.q, self.scale, self.in_features)
 
     @property
     def weight(self):
-        return Fp8Weight(self._rows, self.kind.dtype)
+        return Fp8Weight(self.rows, self.kind.dtype)
 
     def forward(self, x):
         rows = x.reshape(-1, self.in_features)
         if rows.stride(1) != 1 or rows.stride(0) < self.in_features:   # transposed or broadcast rows
             rows = rows.contiguous()
-        y = hip.linear_fp8(rows, self._rows, self.bias)
+        y = hip.linear_fp8(rows, self.rows, self.bias)
         return y.reshape(x.shape[:-1] + (self.out_features,))
 
     def extra_repr(self):

@@ -91,3 +91,20 @@ def test_the_weight_stands_for_the_rows(dev):
     y = torch.randn(5, 200, device=dev)
     with torch.no_grad():
         assert torch.equal(g(y), f.to(dev)(y))
+
+
+def test_the_buffers_are_what_counts(dev):
+    """Buffers set by assignment, by a state dict that replaces them, and for one call by torch.func.functional_call."""
+    from cube_amd.networks.fp8 import Fp8Linear
+    torch.manual_seed(6)
+    a, b = (Fp8Linear(torch.nn.Linear(200, 30).to(dev)) for _ in range(2))
+    x = torch.randn(5, 200, device=dev)
+    with torch.no_grad():
+        ya, yb = a(x), b(x)
+        assert not torch.equal(ya, yb)
+        assert torch.equal(torch.func.functional_call(a, dict(b.named_buffers()), (x,)), yb) and torch.equal(a(x), ya)
+        a.load_state_dict(b.state_dict(), assign=True)
+        assert torch.equal(a(x), yb)
+        c = Fp8Linear(torch.nn.Linear(200, 30).to(dev))
+        c.q, c.scale, c.bias = b.q.clone(), b.scale.clone(), b.bias.clone()
+        assert torch.equal(c(x), yb) and torch.equal(c.weight + 0, b.weight + 0)
