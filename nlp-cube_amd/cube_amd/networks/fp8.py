@@ -74,11 +74,13 @@ class Fp8Linear(torch.nn.Module):
 
 
 def quantise_linears(module):
-    """Every nn.Linear below `module` (itself excepted) -> Fp8Linear, in place.  -> how many."""
-    n = 0
+    """Every nn.Linear below `module` (itself excepted) -> Fp8Linear, in place; one that stands in several places is one layer in all of
+    them afterwards too.  -> how many layers."""
+    made = {}
     for parent in list(module.modules()):
-        for name, child in list(parent.named_children()):
+        for name, child in list(parent._modules.items()):   # (named_children leaves out a second name of the same child)
             if type(child) is torch.nn.Linear:
-                setattr(parent, name, Fp8Linear(child))
-                n += 1
-    return n
+                if child not in made:
+                    made[child] = Fp8Linear(child).train(child.training)
+                setattr(parent, name, made[child])
+    return len(made)

@@ -108,3 +108,21 @@ def test_the_buffers_are_what_counts(dev):
         c = Fp8Linear(torch.nn.Linear(200, 30).to(dev))
         c.q, c.scale, c.bias = b.q.clone(), b.scale.clone(), b.bias.clone()
         assert torch.equal(c(x), yb) and torch.equal(c.weight + 0, b.weight + 0)
+
+
+def test_a_layer_in_several_places_stays_one(dev):
+    """Under a second name of the same parent, and in another parent: one 8-bit layer, counted once; evaluation stays evaluation."""
+    from cube_amd.networks.fp8 import Fp8Linear, quantise_linears
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = torch.nn.Linear(16, 16)
+            self.b = self.a
+            self.c = torch.nn.Sequential(self.a, torch.nn.Linear(16, 4))
+
+    net = Net().to(dev).eval()
+    assert quantise_linears(net) == 2
+    assert type(net.a) is Fp8Linear and net.b is net.a and net.c[0] is net.a and type(net.c[1]) is Fp8Linear
+    assert not any(type(m) is torch.nn.Linear for m in net.modules()) and not any(m.training for m in net.modules())
+    assert quantise_linears(net) == 0
