@@ -321,11 +321,15 @@ def masked_mean(layers, weights, ld_x, word_len, N, W, C, out, ld_out, word_rows
 FP8_BLOCK = 128  # columns that share one scale
 FP8_ACTS = {None: 0, "none": 0, "tanh": 1, "relu": 2}
 _T = {}          # torch dtype -> CUBE_T_*, filled when torch is there
+_forward_ad = None   # torch.autograd.forward_ad, likewise
 
 
 def _types():
+    global _forward_ad
     if not _T:
         import torch
+        from torch.autograd import forward_ad
+        _forward_ad = forward_ad
         _T.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
     return _T
 
@@ -333,6 +337,8 @@ def _types():
 def _matrix(who, name, t):
     """A 2-D f32 / bf16 / f16 tensor on a GPU with neighbouring columns -> (type code, row stride)."""
     code = (_T or _types()).get(t.dtype)
+    if _forward_ad._current_level >= 0:
+        _no_tangent(who, t)
     if code is None or t.dim() != 2:
         raise ValueError("%s: %s must be a 2-D float32, bfloat16 or float16 tensor, got %s %s" % (who, name, t.dtype, tuple(t.shape)))
     if not t.is_cuda:
@@ -352,6 +358,8 @@ def _vector(who, name, t, n, dtype, device):
     if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
         raise ValueError("%s: %s must be a contiguous %s tensor of %d values on %s, got %s %s on %s"
                          % (who, name, dtype, n, device, t.dtype, tuple(t.shape), t.device))
+    if _forward_ad._current_level >= 0:
+        _no_tangent(who, t)
     return t.data_ptr()
 
 
@@ -359,6 +367,12 @@ def _no_grad(who):
     import torch
     if torch.is_grad_enabled():
         raise ValueError("%s has no gradient: call it under torch.no_grad() or on detached tensors" % who)
+
+
+def _no_tangent(who, t):
+    """Refuses a dual tensor of forward-mode differentiation (torch.no_grad() does not turn that off, and requires_grad does not show it)."""
+    if _forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError("%s has no gradient: call it on tensors without a tangent (torch.autograd.forward_ad.unpack_dual)" % who)
 
 
 class Fp8Rows:

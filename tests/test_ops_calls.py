@@ -1,0 +1,31 @@
+"""CPU: what the calls on tensors of the 8-bit Linear operators and the sampler (cube_amd/hip.py) refuse before anything is launched."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from cube_amd import hip
+
+
+def rows(n=4, columns=200):
+    return hip.Fp8Rows(torch.zeros(n, 256, dtype=torch.uint8), torch.zeros(1, n, dtype=torch.int32), columns)
+
+
+def f64(n=4):
+    return torch.full((n,), 0.5, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(grad):
+    """A dual tensor does not require a gradient, and no_grad() does not turn its tangent off: it would be lost without a word."""
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        x = forward_ad.make_dual(torch.randn(4, 200), torch.randn(4, 200))
+        for call in (lambda: hip.quant_fp8(x), lambda: hip.linear_fp8(x, rows()), lambda: hip.sample_rows(x, f64())):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        v = forward_ad.make_dual(torch.randn(4), torch.randn(4))
+        with pytest.raises(ValueError, match="tangent"):
+            hip._vector("linear_fp8", "bias", v, 4, torch.float32, v.device)
+        with pytest.raises(hip.CubeHipError, match="no CPU fallback"):    # without a tangent: the next refusal
+            hip.quant_fp8(torch.randn(4, 200))
+    with pytest.raises(hip.CubeHipError, match="no CPU fallback"):
+        hip.quant_fp8(torch.randn(4, 200))
