@@ -358,6 +358,8 @@ def _vector(who, name, t, n, dtype, device):
     if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
         raise ValueError("%s: %s must be a contiguous %s tensor of %d values on %s, got %s %s on %s"
                          % (who, name, dtype, n, device, t.dtype, tuple(t.shape), t.device))
+    if t.requires_grad:
+        _no_grad(who)
     if _forward_ad._current_level >= 0:
         _no_tangent(who, t)
     return t.data_ptr()
@@ -452,8 +454,6 @@ def _fp8_output(who, M, K, device, w, bias, act, out, out_dtype):
             _no_grad(who)
         code, ldo = _matrix(who, "out", out)
     if bias is not None:
-        if bias.requires_grad:
-            _no_grad(who)
         bias = _vector(who, "bias", bias, N, torch.float32, device)
     return out, (q.data_ptr(), q.shape[1], w.scale.data_ptr(), N, N, K, bias, FP8_ACTS[act], out.data_ptr(), code, ldo)
 

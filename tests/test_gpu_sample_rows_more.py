@@ -31,3 +31,16 @@ def test_greedy_rows_of_every_long_form(dev, M, V, t):
         tok, prob = hip.sample_rows(z.to(dev), u, temperature=0.0)
         np.testing.assert_array_equal(tok.cpu().numpy(), want)
         assert bool((prob == 1).all())
+
+
+def test_settings_that_ask_for_a_gradient(dev):
+    z, u = torch.randn(4, 60, device=dev), torch.full((4,), 0.5, dtype=torch.float64, device=dev)
+    for name in ("temperature", "top_p", "min_p"):
+        v = torch.full((4,), 0.7, device=dev, requires_grad=True)
+        with pytest.raises(ValueError, match="gradient"):
+            hip.sample_rows(z, u, **{name: v})
+        with torch.no_grad():
+            got = hip.sample_rows(z, u, **{name: v})
+        assert torch.equal(got[0], hip.sample_rows(z, u, **{name: v.detach()})[0])
+    with pytest.raises(ValueError, match="gradient"):
+        hip.sample_rows(z, u.clone().requires_grad_())

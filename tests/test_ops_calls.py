@@ -29,3 +29,14 @@ def test_forward_mode_tangents_are_refused(grad):
             hip.quant_fp8(torch.randn(4, 200))
     with pytest.raises(hip.CubeHipError, match="no CPU fallback"):
         hip.quant_fp8(torch.randn(4, 200))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_vectors_that_ask_for_a_gradient_are_refused(dtype):
+    """bias, u, and the settings of a draw (a temperature that is learnt): refused unless gradients are off."""
+    v = torch.full((4,), 0.7, dtype=dtype, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        hip._vector("sample_rows", "temperature", v, 4, dtype, v.device)
+    with torch.no_grad():
+        assert hip._vector("sample_rows", "temperature", v, 4, dtype, v.device) == v.data_ptr()
+    assert hip._vector("sample_rows", "temperature", v.detach(), 4, dtype, v.device) == v.data_ptr()
