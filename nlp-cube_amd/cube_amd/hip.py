@@ -341,6 +341,8 @@ def _matrix(who, name, t):
         _no_tangent(who, t)
     if code is None or t.dim() != 2:
         raise ValueError("%s: %s must be a 2-D float32, bfloat16 or float16 tensor, got %s %s" % (who, name, t.dtype, tuple(t.shape)))
+    if t.is_neg():
+        _negated(who, name)
     if not t.is_cuda:
         raise CubeHipError("%s: %s is on %s; it must be on an MI355X (there is no CPU fallback)" % (who, name, t.device))
     rows, cols = t.shape
@@ -358,11 +360,17 @@ def _vector(who, name, t, n, dtype, device):
     if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
         raise ValueError("%s: %s must be a contiguous %s tensor of %d values on %s, got %s %s on %s"
                          % (who, name, dtype, n, device, t.dtype, tuple(t.shape), t.device))
+    if t.is_neg():
+        _negated(who, name)
     if t.requires_grad:
         _no_grad(who)
     if _forward_ad._current_level >= 0:
         _no_tangent(who, t)
     return t.data_ptr()
+
+
+def _negated(who, name):
+    raise ValueError("%s: %s is a view that stands for its memory with the sign changed; call resolve_neg() on it" % (who, name))
 
 
 def _no_grad(who):

@@ -40,3 +40,14 @@ def test_vectors_that_ask_for_a_gradient_are_refused(dtype):
     with torch.no_grad():
         assert hip._vector("sample_rows", "temperature", v, 4, dtype, v.device) == v.data_ptr()
     assert hip._vector("sample_rows", "temperature", v.detach(), 4, dtype, v.device) == v.data_ptr()
+
+
+def test_negated_views_are_refused():
+    """The imaginary part of a conjugate is its memory with the sign changed: one column (or value) of it passes as neighbouring ones."""
+    x = torch.zeros(4, 1, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    for call in (lambda: hip.quant_fp8(x), lambda: hip.sample_rows(x, f64()), lambda: hip._vector("linear_fp8", "bias", x[:1, 0], 1, torch.float32, x.device)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    with pytest.raises(hip.CubeHipError, match="no CPU fallback"):
+        hip.quant_fp8(x.resolve_neg())
