@@ -343,9 +343,11 @@ def _matrix(who, name, t):
         raise ValueError("%s: %s must be a 2-D float32, bfloat16 or float16 tensor, got %s %s" % (who, name, t.dtype, tuple(t.shape)))
     if t.is_neg():
         _negated(who, name)
+    rows, cols = t.shape
+    if rows > 0x7fffffff or cols > 0x7fffffff:   # (ctypes would drop the upper bits without a word)
+        raise ValueError("%s: %s has more than 2^31 - 1 rows or columns: %s" % (who, name, tuple(t.shape)))
     if not t.is_cuda:
         raise CubeHipError("%s: %s is on %s; it must be on an MI355X (there is no CPU fallback)" % (who, name, t.device))
-    rows, cols = t.shape
     ld, one = t.stride()
     if one != 1 and cols > 1:
         raise ValueError("%s: the columns of %s must be neighbours (stride 1), got stride %d" % (who, name, one))
@@ -393,6 +395,8 @@ class Fp8Rows:
     def __init__(self, q, scale, columns):
         import torch
         kb = (columns + FP8_BLOCK - 1) // FP8_BLOCK
+        if q.dim() == 2 and q.shape[0] > 0x7fffffff or columns > 0x7fffffff:
+            raise ValueError("Fp8Rows: more than 2^31 - 1 rows or columns: %s" % (tuple(q.shape),))
         if columns < 1 or q.dtype != torch.uint8 or q.dim() != 2 or q.shape[1] != kb * FP8_BLOCK or not q.is_contiguous():
             raise ValueError("Fp8Rows: q must be a contiguous uint8 [rows, %d] tensor for %d columns, got %s %s"
                              % (kb * FP8_BLOCK, columns, q.dtype, tuple(q.shape)))

@@ -51,3 +51,18 @@ def test_negated_views_are_refused():
             call()
     with pytest.raises(hip.CubeHipError, match="no CPU fallback"):
         hip.quant_fp8(x.resolve_neg())
+
+
+@pytest.mark.parametrize("shape", [(1 << 31, 2), ((1 << 32) + 4, 2), (1, 1 << 31), (2, (1 << 32) + 100)])
+def test_sizes_beyond_31_bits_are_refused(shape):
+    """The C functions take 32-bit counts, and ctypes drops what is above them: 2^32 + 100 columns were 100."""
+    x = torch.zeros(1, 1).expand(shape)
+    for call in (lambda: hip.quant_fp8(x), lambda: hip.linear_fp8(x, rows()), lambda: hip.sample_rows(x, f64())):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
+    if shape[1] == 2:
+        with pytest.raises(ValueError, match="2\\^31"):
+            hip.Fp8Rows(torch.zeros(1, 1, dtype=torch.uint8).expand(shape[0], 128), torch.zeros(1, 1, dtype=torch.int32).expand(1, shape[0]), 100)
+    else:
+        with pytest.raises(ValueError, match="2\\^31"):
+            hip.Fp8Rows(torch.zeros(1, 128, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.int32), shape[1])
