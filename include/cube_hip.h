@@ -416,14 +416,14 @@ enum { CUBE_T_F32 = 0, CUBE_T_BF16 = 1, CUBE_T_F16 = 2, CUBE_T_E4M3 = 3 };
 enum { CUBE_FP8_NONE = 0, CUBE_FP8_TANH = 1, CUBE_FP8_RELU = 2 };
 
 /* x [M, ld_x] (f32, bf16 or f16) -> q, scale.  Per row and block: e = the smallest integer >= -127 with max|x| <= 448 * 2^e over
- * the finite values, q = e4m3(x * 2^-e), nearest, ties to even; an infinity or NaN becomes e4m3's NaN.  q: 16-byte aligned rows,
- * apart from x; K <= 2^24, M <= 2^30.                                                                                    */
+ * the finite values, q = e4m3(x * 2^-e), nearest, ties to even; an infinity or NaN becomes e4m3's NaN.  q: 16-byte aligned rows.
+ * x, q and scale share no byte (refused); K <= 2^24, M <= 2^30.                                                          */
 int cube_quant_fp8(const void* x, int x_type, long long ld_x, int M, int K, void* q, long long ld_q, uint32_t* scale, int ld_s,
                    void* stream);
 
 /* out[m, n] = act(bias[n] + sum_k a[m, k] * w[n, k]), rounded once to out_type; sums in fp32.  Leading dimensions in elements;
- * bias may be NULL; out may be any matrix aligned to its type that shares no byte with an input.  M, N <= 2^30, K, ldw and the lda
- * of quantised rows <= 2^24.  Sums beyond fp32's range become infinities.
+ * bias may be NULL; out may be any matrix aligned to its type; it and ws share no byte with an input (refused).  M, N <= 2^30,
+ * K, ldw and the lda of quantised rows <= 2^24.  Sums beyond fp32's range become infinities.
  * 16-bit outputs come from the 8-bit matrix instructions, which keep 13 bits below the largest of 8 neighbouring products (about
  * 1.5e-5 of the result's 2-norm).  fp32 outputs have exact products: operand values from 2^-133 to below 2^128 are taken as they are,
  * smaller ones rounded to a multiple of 2^-133, 2^128 as infinity.  tanh is within 2^-22 of itself before the output's rounding.
@@ -452,7 +452,7 @@ int cube_linear_fp8(const cube_fp8_args* args, void* ws, size_t ws_bytes, void* 
  * temperature / top_k / top_p / min_p: device arrays of M, or NULL for the scalar beside each.  Weights are added as integers: the
  * token does not depend on how the row is split.  They are exponentials to 2^-50 of themselves, cut to a whole 2^-62 of the largest
  * (V <= 256: rounded to 2^-46), so a border lies within 2^-48 + V * 2^-62 (2^-39) of the total from where it would exactly.
- * V <= CUBE_SAMPLE_MAX_V; token and prob share no byte with an input.                                                      */
+ * V <= CUBE_SAMPLE_MAX_V; token, prob and ws share no byte with an input or each other (refused); ld <= 2^40. */
 #define CUBE_SAMPLE_MAX_V (1 << 22)
 typedef struct cube_sample_args {
   const void* logits; int type; long long ld; int M; int V;

@@ -75,3 +75,29 @@ struct CubeLdsReservation {
     return true;
   }
 };
+
+// Memory that an entry point reads or writes: rows of `width` bytes, `pitch` apart.
+struct CubeArea {
+  const void* at; long long pitch, width, rows;
+  CubeArea(const void* p, long long pitch_, long long width_, long long rows_) : at(p), pitch(pitch_), width(width_), rows(rows_) {
+    if (pitch == width) { width *= rows; rows = rows > 0; }  // one run
+  }
+  CubeArea(const void* p, long long bytes) : at(p), pitch(bytes), width(bytes), rows(1) {}
+};
+// Whether two areas share bytes: exactly, but for rows of two distances that lie in one another's range (taken to).  Windows of one buffer
+// side by side do not, nor does a vector between a matrix's rows.
+inline bool cube_overlap(const CubeArea& a, const CubeArea& b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const __int128 x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+  const __int128 x1 = x + (__int128)a.pitch * (a.rows - 1) + a.width, y1 = y + (__int128)b.pitch * (b.rows - 1) + b.width;
+  if (x >= y1 || y >= x1) return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.rows == 1) return cube_overlap(b, a);
+  if (b.rows == 1) {  // the first row of a that ends behind b's first byte
+    const __int128 i = y < x + a.width ? 0 : (y - x - a.width) / a.pitch + 1;
+    return i < a.rows && x + i * a.pitch < y1;
+  }
+  if (a.pitch != b.pitch) return true;
+  const long long d = y >= x ? (long long)((y - x) % a.pitch) : (long long)((a.pitch - (x - y) % a.pitch) % a.pitch);
+  return d < a.width || d + b.width > a.pitch;
+}

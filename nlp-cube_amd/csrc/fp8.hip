@@ -814,14 +814,19 @@ size_t quant_bytes(int M, int K) {
   return q + (size_t)((kblocks(K) + 3) / 4) * M * 4;
 }
 
-// whether two matrices share bytes: address, bytes from row to row, bytes of a row, rows (windows of one buffer side by side do not)
-bool overlap(const void* a, long long pa, long long wa, int na, const void* b, long long pb, long long wb, int nb) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  const __int128 x1 = (__int128)pa * (na - 1) + wa + x, y1 = (__int128)pb * (nb - 1) + wb + y;
-  if (x >= y1 || y >= x1) return false;
-  if (pa != pb) return true;
-  const long long d = y >= x ? (long long)((y - x) % (uintptr_t)pa) : (pa - (long long)((x - y) % (uintptr_t)pa)) % pa;
-  return d < wa || d + wb > pa;
+CubeArea code_area(const void* q, long long ld, int rows, int K) { return {q, ld, (long long)kblocks(K) * BLK, rows}; }
+CubeArea scale_area(const uint32_t* s, int ld, int rows, int K) { return {s, 4LL * ld, 4LL * rows, (kblocks(K) + 3) / 4}; }
+CubeArea plain_area(const void* x, int type, long long ld, int rows, int columns) {
+  return {x, ld * type_size(type), (long long)columns * type_size(type), rows};
+}
+// what neither the output nor the workspace may touch; A_scale: NULL where A is plain
+const char* touches(const CubeArea& to, const cube_fp8_args* a, const uint32_t* A_scale, const CubeArea& A) {
+  if (cube_overlap(A, to)) return "A";
+  if (A_scale && cube_overlap(scale_area(A_scale, a->lds_a, a->M, a->K), to)) return "A_scale";
+  if (cube_overlap(code_area(a->W, a->ldw, a->N, a->K), to)) return "W";
+  if (cube_overlap(scale_area(a->W_scale, a->lds_w, a->N, a->K), to)) return "W_scale";
+  if (cube_overlap({a->bias, 4LL * a->N}, to)) return "bias";
+  return nullptr;
 }
 
 // what cube_gemm_fp8 and cube_linear_fp8 check alike
@@ -866,6 +871,9 @@ extern "C" int cube_quant_fp8(const void* x, int x_type, long long ld_x, int M, 
               (long long)kblocks(K) * BLK, ld_s, M);
   if (((uintptr_t)q & 15) || ld_q % 16) CUBE_FAIL(CUBE_ERR_ALIGN, "cube_quant_fp8: rows of q are not 16-byte aligned");
   if ((uintptr_t)x % type_size(x_type) || ((uintptr_t)scale & 3)) CUBE_FAIL(CUBE_ERR_ALIGN, "cube_quant_fp8: x / scale not aligned to their types");
+  const CubeArea from = plain_area(x, x_type, ld_x, M, K), codes = code_area(q, ld_q, M, K), words = scale_area(scale, ld_s, M, K);
+  if (cube_overlap(from, codes) || cube_overlap(from, words) || cube_overlap(codes, words))
+    CUBE_FAIL(CUBE_ERR_ARG, "cube_quant_fp8: x, q and scale overlap");
   return quant_any(x, x_type, ld_x, M, K, q, ld_q, scale, ld_s, (hipStream_t)stream);
 }
 
@@ -881,8 +889,8 @@ extern "C" int cube_gemm_fp8(const cube_fp8_args* a, void* stream) {
               a->lds_a, a->M);
   if (((uintptr_t)a->A & 15) || a->lda % 16 || ((uintptr_t)a->A_scale & 3))
     CUBE_FAIL(CUBE_ERR_ALIGN, "cube_gemm_fp8: rows of A are not 16-byte aligned, or A_scale not 4-byte aligned");
-  if (overlap(a->A, a->lda, (long long)kblocks(a->K) * BLK, a->M, a->out, a->ldo * type_size(a->out_type), (long long)a->N * type_size(a->out_type), a->M))
-    CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: out overlaps A");
+  const char* met = touches(plain_area(a->out, a->out_type, a->ldo, a->M, a->N), a, a->A_scale, code_area(a->A, a->lda, a->M, a->K));
+  if (met) CUBE_FAIL(CUBE_ERR_ARG, "cube_gemm_fp8: out overlaps %s", met);
   Fp8Params p = params(a);
   return launch_gemm(p, (hipStream_t)stream);
 }
@@ -904,8 +912,14 @@ extern "C" int cube_linear_fp8(const cube_fp8_args* a, void* ws, size_t ws_bytes
   const size_t need = cube_linear_fp8_workspace_bytes(a->M, a->N, a->K);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: workspace of %zu bytes (need %zu, 16-byte aligned)", ws_bytes, need);
-  const long long es = type_size(a->a_type), eo = type_size(a->out_type);
-  if (overlap(a->A, a->lda * es, a->K * es, a->M, a->out, a->ldo * eo, a->N * eo, a->M)) CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: out overlaps A");
+  const CubeArea from = plain_area(a->A, a->a_type, a->lda, a->M, a->K), out = plain_area(a->out, a->out_type, a->ldo, a->M, a->N);
+  const char* met = touches(out, a, nullptr, from);
+  if (met) CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: out overlaps %s", met);
+  if (need) {
+    const CubeArea work = {ws, (long long)need};
+    met = cube_overlap(out, work) ? "out" : touches(work, a, nullptr, from);
+    if (met) CUBE_FAIL(CUBE_ERR_ARG, "cube_linear_fp8: the workspace overlaps %s", met);
+  }
   Fp8Params p = params(a);
   hipStream_t st = (hipStream_t)stream;
   if (!need) {

@@ -1886,13 +1886,21 @@ extern "C" int cube_sample_rows(const cube_sample_args* a, void* ws, size_t ws_b
   if (a->M == 0) return CUBE_OK;
   if (!a->logits || !a->u || !a->token) CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: null logits / u / token");
   if (a->type < CUBE_T_F32 || a->type > CUBE_T_F16) CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: type=%d", a->type);
-  if (a->ld < a->V) CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: ld=%lld < V=%d", a->ld, a->V);
+  if (a->ld < a->V || a->ld > 1LL << 40) CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: ld=%lld outside V=%d..2^40", a->ld, a->V);
   if ((uintptr_t)a->logits % (a->type == CUBE_T_F32 ? 4 : 2) || ((uintptr_t)a->u & 7) ||
       (((uintptr_t)a->token | (uintptr_t)a->prob | (uintptr_t)a->temperature | (uintptr_t)a->top_k | (uintptr_t)a->top_p | (uintptr_t)a->min_p) & 3))
     CUBE_FAIL(CUBE_ERR_ALIGN, "cube_sample_rows: a pointer is not aligned to its type");
   const size_t need = cube_sample_workspace_bytes(a->type, a->M, a->V);
   if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15)))
     CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: workspace of %zu bytes (need %zu, 16-byte aligned)", ws_bytes, need);
+  const long long es = a->type == CUBE_T_F32 ? 4 : 2, M4 = 4LL * a->M;
+  const CubeArea in[] = {{a->logits, a->ld * es, a->V * es, a->M}, {a->u, 2 * M4}, {a->temperature, M4}, {a->top_k, M4}, {a->top_p, M4}, {a->min_p, M4}};
+  const CubeArea out[] = {{a->token, M4}, {a->prob, M4}, {need ? ws : nullptr, (long long)need}};
+  for (const CubeArea& o : out)
+    for (const CubeArea& i : in)
+      if (cube_overlap(i, o)) CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: an input overlaps token, prob or the workspace");
+  if (cube_overlap(out[0], out[1]) || cube_overlap(out[0], out[2]) || cube_overlap(out[1], out[2]))
+    CUBE_FAIL(CUBE_ERR_ARG, "cube_sample_rows: token, prob and the workspace overlap");
   hipStream_t st = (hipStream_t)stream;
   if (a->type == CUBE_T_F32) return launch<float>(*a, ws, st);
   if (a->type == CUBE_T_BF16) return launch<bf16_t>(*a, ws, st);

@@ -56,3 +56,58 @@ def test_tanh_at_its_ends(dev):
         np.testing.assert_allclose(np_(got[0]), want, rtol=2.0 ** -22, atol=2.0 ** -149)
     x[1, 5] = float("nan")
     assert bool(torch.isnan(hip.linear_fp8(x, w, bias, act="tanh")[1]).all())
+
+
+# ---- memory beside memory ---------------------------------------------------------------------------------------------------
+
+def test_arrays_beside_one_another_are_taken(dev):
+    """Random layouts of cube_quant_fp8 within one buffer that share no byte: the call is taken and writes what it does elsewhere, and
+    nothing else.  (Rows of two distances within one another's range are refused whether or not they meet.)"""
+    import random
+    rng = random.Random(2)
+    size = 1 << 16
+    buf = torch.zeros(size, dtype=torch.uint8, device=dev)
+    lib, base, taken = hip.load(), buf.data_ptr(), 0
+    for _ in range(400):
+        M, K = rng.randint(1, 6), rng.randint(1, 140)
+        kb = -(-K // 128)
+        pitch = 16 * rng.randint(64, 90)                         # x and q as windows of one matrix, or lying one behind the other
+        ld_x, ld_q, ld_s = (pitch // 4, pitch, M) if rng.random() < 0.6 else (K + rng.choice([0, 5]), kb * 128 + 16 * rng.choice([0, 9]), M + rng.choice([0, 3]))
+        x, q, s = 4 * rng.randint(0, 2000), 16 * rng.randint(0, 600), 4 * rng.randint(0, 3000)
+        bx = {x + 4 * ld_x * r + i for r in range(M) for i in range(4 * K)}
+        bq = {q + ld_q * r + i for r in range(M) for i in range(kb * 128)}
+        bs = {s + i for i in range(4 * M)}
+        within = x < q + ld_q * (M - 1) + kb * 128 and q < x + 4 * (ld_x * (M - 1) + K)
+        two = M > 1 and 4 * ld_x != ld_q and 4 * K != 4 * ld_x and kb * 128 != ld_q and within
+        if bx & bq or bx & bs or bq & bs or two:
+            continue
+        taken += 1
+        v = torch.randn(M, K)
+        host = np.full(size, 0xA5, dtype=np.uint8)
+        for r in range(M):
+            host[x + 4 * ld_x * r: x + 4 * (ld_x * r + K)] = v[r].numpy().view(np.uint8)
+        buf.copy_(torch.from_numpy(host))
+        assert lib.cube_quant_fp8(base + x, 0, ld_x, M, K, base + q, ld_q, base + s, ld_s, hip.stream_handle()) == 0, lib.cube_last_error()
+        want = hip.quant_fp8(v.to(dev))
+        for r in range(M):
+            host[q + ld_q * r: q + ld_q * r + kb * 128] = want.q[r].cpu().numpy()
+        host[s: s + 4 * M] = want.scale[0].cpu().numpy().view(np.uint8)
+        np.testing.assert_array_equal(buf.cpu().numpy(), host)
+    assert taken > 60
+
+
+def test_an_output_between_its_inputs(dev):
+    """out, bias and weights in one allocation without a gap, and a token vector behind its logits: taken."""
+    M, N, K = 70, 64, 256
+    buf = torch.zeros(1 << 18, dtype=torch.uint8, device=dev)
+    w = hip.quant_fp8(torch.randn(N, K, device=dev))
+    q = buf[:N * K].view(N, K)
+    s = buf[N * K:N * K + 4 * N].view(torch.int32).view(1, N)
+    out = buf[N * K + 4 * N:N * K + 4 * N + 2 * M * N].view(torch.bfloat16).view(M, N)
+    bias = buf[N * K + 4 * N + 2 * M * N:][:4 * N].view(torch.float32)
+    q.copy_(w.q), s.copy_(w.scale), bias.copy_(torch.randn(N, device=dev))
+    x = torch.randn(M, K, device=dev).bfloat16()
+    want = hip.linear_fp8(x, w, bias.clone())
+    assert torch.equal(hip.linear_fp8(x, hip.Fp8Rows(q, s, K), bias, out=out), want)
+    with pytest.raises(hip.CubeHipError, match="overlaps bias"):
+        hip.linear_fp8(x, hip.Fp8Rows(q, s, K), buf[N * K + 4 * N:][:4 * N].view(torch.float32), out=out)
