@@ -111,3 +111,94 @@ def test_an_output_between_its_inputs(dev):
     assert torch.equal(hip.linear_fp8(x, hip.Fp8Rows(q, s, K), bias, out=out), want)
     with pytest.raises(hip.CubeHipError, match="overlaps bias"):
         hip.linear_fp8(x, hip.Fp8Rows(q, s, K), buf[N * K + 4 * N:][:4 * N].view(torch.float32), out=out)
+
+
+# ---- every tile and both of its loops, with 16-bit outputs --------------------------------------------------------------------
+
+def scaled_integers(rng, rows, K, dev):
+    """Codes of magnitude up to 3 at scales 1, 2, 4, another for every block of every row: sums of up to 2^15 products (at most 9 * 16
+    each) are integers below 2^23, exact in fp32 whatever their order, and lose nothing in the 8-bit instructions (one block, one scale)."""
+    kb = -(-K // 128)
+    v = rng.integers(-3, 4, (rows, kb * 128)).astype(np.float64)
+    v[:, K:] = 0
+    return rows_from(v, rng.integers(127, 130, (rows, kb)), K, dev)
+
+
+# 256x256 tiles by blocks of K (one, more than its two stages, over a change of the scale word, around two); 128x128; 128x64; 64x64 with
+# four stages and with wave groups along K
+TILES = [(4000, 4050, K) for K in (100, 300, 512, 600, 768, 1100)] + [(5000, 3900, 260), (8192, 768, 768), (8000, 520, 1000), (8192, 768, 100), (2100, 1100, 700),
+                                                                      (2100, 1100, 130), (512, 768, 768), (65, 1000, 2500), (300, 260, 1500)]
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_every_tile_in_16_bits(dev, M, N, K):
+    rng = np.random.default_rng(M + N + K)
+    a, w = scaled_integers(rng, M, K, dev), scaled_integers(rng, N, K, dev)
+    bias = rng.integers(-50, 50, N).astype(np.float32)
+    y = (a.float().double() @ w.float().double().t()).cpu() + torch.from_numpy(bias).double()
+    for t in (torch.bfloat16, torch.float16, torch.float32):
+        got = hip.gemm_fp8(a, w, torch.from_numpy(bias).to(dev), out_dtype=t)
+        assert torch.equal(got.cpu(), y.float().to(t)), t
+
+
+@pytest.mark.parametrize("M,N,K", [(4000, 4050, 600), (8192, 768, 300), (2100, 1100, 300)])
+def test_large_tiles_into_strided_rows(dev, M, N, K):
+    rng = np.random.default_rng(7)
+    a, w = scaled_integers(rng, M, K, dev), scaled_integers(rng, N, K, dev)
+    for t in (torch.bfloat16, torch.float16):
+        want = hip.gemm_fp8(a, w, out_dtype=t)
+        for col, pad in ((1, 2), (8, 8), (0, 1)):
+            base = torch.full((M + 2, col + N + pad), -7.0, dtype=t, device=dev)
+            hip.gemm_fp8(a, w, out=base[1:M + 1, col:col + N])
+            assert torch.equal(base[1:M + 1, col:col + N], want)
+            base[1:M + 1, col:col + N] = -7.0
+            assert bool((base == -7.0).all())
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("M", [1, 16, 20, 33, 48, 60, 130])
+def test_a_vocabulary_in_16_bits(dev, M, t):
+    """As the fp32 test of a vocabulary: few rows (a tile of columns a wave) and many."""
+    rng = np.random.default_rng(M)
+    N, K = 131072 + 77, 260
+    w = integer_rows(rng, 1000, K, dev)
+    few = w.float().double()
+    w = hip.Fp8Rows(w.q.repeat(132, 1)[:N].contiguous(), w.scale.repeat(1, 132)[:, :N].contiguous(), K)
+    x = torch.randint(-3, 4, (M, K), generator=torch.Generator().manual_seed(M)).float()
+    x[:, ::128] = 448.0                                      # the scale of every block is 1: the small integers stay what they are
+    # 448 times at most 3 beside products of at most 9: fewer than 13 bits, nothing is lost
+    want = (x.to(dev).double() @ few.t()).repeat(1, 132)[:, :N].float().to(TYPES[t])
+    for got in (hip.linear_fp8(x.to(dev).to(TYPES[t]), w), hip.gemm_fp8(hip.quant_fp8(x.to(dev)), w, out_dtype=TYPES[t])):
+        assert torch.equal(got, want)
+
+
+# ---- streams ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("M", [1, 33, 200, 3000])
+def test_quantiser_and_product_on_a_side_stream(dev, M, t):
+    """The two calls one behind the other on another stream than the tensors were made on: the same bits as on their own, in new memory
+    each time; and as one call, where that runs the same product."""
+    x = torch.randn(M, 1000, device=dev).to(TYPES[t])
+    w = hip.quant_fp8(torch.randn(300, 1000, device=dev))
+    first = hip.gemm_fp8(hip.quant_fp8(x), w, out_dtype=TYPES[t])
+    v, e = oo.quant(np_(x))
+    want, mag = oo.gemm(oo.rows_value(v, e), values(w))
+    close(np_(first), want, mag, 1000, t)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            got = hip.gemm_fp8(hip.quant_fp8(x), w, out_dtype=TYPES[t])
+        side.synchronize()
+        assert torch.equal(got, first)
+    if M >= 200:
+        assert torch.equal(hip.linear_fp8(x, w), first)
+
+
+@pytest.mark.parametrize("M,N,K,t", [(1001, 500, 300, "f32"), (8192, 768, 768, "bf16"), (4000, 4050, 1100, "bf16"), (1, 4096, 4096, "bf16"), (8192, 500, 768, "f32")])
+def test_the_same_bits_every_time(dev, M, N, K, t):
+    x, w = torch.randn(M, K, device=dev).to(TYPES[t]), hip.quant_fp8(torch.randn(N, K, device=dev))
+    first = hip.linear_fp8(x, w, act="tanh")
+    for _ in range(4):
+        assert torch.equal(hip.linear_fp8(x, w, act="tanh"), first)
