@@ -302,8 +302,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS) void gemm_fp8_kernel(const Fp8Pa
   constexpr int ROWS = (BM + BN) * BLK, STAGE = ROWS + (BM + BN) * 4;
   constexpr int LOADS = PA + PB + PS;                    // a wave's loads per stage
   // EARLY: a step's barrier and first fragment reads come under the last products of the step before it.  With 8 row tiles a wave, where
-  // a workgroup has the CU for itself, that takes 2 to 4 % off (8192x4096x4096 131 -> 128 us, 8192x8192x8192 425 -> 415); with fewer,
-  // where another workgroup covers them, it costs 2 % (2048x2048x2048 15.0 -> 15.9 us, 8192x500x768 f32 13.8 -> 14.2).
+  // a workgroup has the CU for itself, that takes up to 1 % off (8192x8192x8192 427 -> 424 us, 8192x4096x4096 109 either way); with fewer,
+  // where another workgroup covers them, nothing (2048x2048x2048 13.7 -> 13.8 us, 8192x500x768 f32 13.3 -> 13.4).
   constexpr bool EARLY = TM >= 8;
   constexpr int SLOTS = EARLY ? TM / 2 + 1 : TM;         // row tiles whose products loads go out with
   constexpr int PER = (LOADS + SLOTS - 1) / SLOTS;
@@ -791,15 +791,17 @@ int launch_gemm(Fp8Params& p, hipStream_t st) {
   const bool exact = p.out_type == CUBE_T_F32;
   if (p.M <= 16) return launch_few<uint8_t, true, 1>(p, st);
   if (p.M <= FEW_ROWS) return launch_few<uint8_t, true, 2>(p, st);
-  // The largest tile that still gives every CU work, by the number of tiles (times of one launch, 16-bit output unless said):
-  //   256x256: 8192x4096x4096 110 us (128x128: 125 us), where their last round fills 4 of 5 CUs:  5000x4000x2000, 320 of them,
-  //     63 us (54 us), 8192x3000x1024, 384, 42 us (39 us)
-  //   128x128 (two workgroups a CU): 8192x768x768 11.7 us (128x64 13.2, 64x64 15.1), 8000x520x8000 54 us (64, 67);
-  //     256 of them, one a CU, lose: 2048x2048x2048 18.3 us (128x64 15.3)
-  //   128x64: 4096x1024x1024 9.7 us (64x64 12.1), 8192x500x768 f32 14.9 us (18.4)
-  //   64x64 with four stages: 512x768x768 4.8 us (128x64 5.9), 1001x500x300 f32 6.5 us (7.5)
-  //   the same with four wave groups along K: 65x4096x4096 10.3 us (one group 12.8), 65x64x8000 f32 21.4 us (32.5); with a K of
-  //     1024 and less it loses: 65x4096x1024 6.1 us (5.7)
+  // The largest tile that still gives every CU work, by the number of tiles (launches one behind the other from a graph, 16-bit
+  // output and no activation unless said):
+  //   256x256: 8192x4096x4096 111 us (128x128: 139 us), where their last round fills 4 of 5 CUs:  5000x4000x2000, 320 of them,
+  //     60 us (54 us), 8192x3000x1024, 384, 43 us (39 us).  A narrow output fills no such tile, and the count does not see it:
+  //     65536x16x768 23 us (128x64 13)
+  //   128x128 (two workgroups a CU): 8192x768x768 10.8 us (128x64 12.8, 64x64 14.8), 8000x520x8000 53 us (67, 68);
+  //     256 of them, one a CU, lose: 2048x2048x2048 16.2 us (128x64 14.4)
+  //   128x64: 4096x1024x1024 9.3 us (64x64 11.4), 8192x500x768 f32 13.4 us (15.7)
+  //   64x64 with four stages: 512x768x768 4.6 us (128x64 5.7), 1001x500x300 f32 5.1 us (6.5)
+  //   the same with four wave groups along K: 65x4096x4096 9.8 us (one group 12.2), 65x64x8000 f32 20.5 us (28.4); with a K of
+  //     1024 and less it loses: 65x4096x1024 5.6 us (5.1)
   auto tiles = [&](int bm, int bn) { return (long long)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
   const long long big = tiles(256, 256), rounds = (big + 255) / 256;
   if (!exact && 5 * big >= 4 * 256 * rounds) return launch_tiles<256, 256, 2, 4, 2, 1, false>(p, st);

@@ -902,7 +902,7 @@ __global__ __launch_bounds__(WG) void sample_mid_kernel(cube_sample_args a) {
 // ---- half: 16-bit logits by the counts of their values ----------------------------------------------------------------------
 // A slice's counts: one 32-bit word per magnitude (the 15 bits without the sign), the number of its logits in the low half and
 // of its negative ones in the high half; a slice has at most 65528 logits, so neither runs over.  Groups of 64 * E magnitudes, E
-// to a lane: an octave of bf16, half an octave of f16 (quarters of that, 128 x 250002: 88 us, these 60:
+// to a lane: an octave of bf16, half an octave of f16 (quarters of that, 128 x 250002: 88 us, these 61:
 // a row then has 130 groups).
 // In the candidates' order group g comes GROUPS - 1 - g-th for positive values, falling inside, and GROUPS + g-th for negative
 // ones, rising.
@@ -935,7 +935,7 @@ __device__ __forceinline__ Words<8> load_words(const uint32_t* p, Words<8>) {
 
 // The granules lo .. hi - 1 of a row: f(word) for the two logits of each 32-bit word of the whole ones, g(raw) for the logits of the
 // row's first and last granule where those are not whole.  Four loads of a thread are on their way together (with each followed by
-// its use 128 x 250002 took 40 us in all, 37 here).
+// its use 128 x 250002 took 3 us more in all).
 template <class T, class F, class G> __device__ __forceinline__ void half_words(const Row<T>& row, int lo, int hi, F f, G g) {
   const uint16_t* at = (const uint16_t*)row.at - row.lead;
   const int whole = (row.V + row.lead) / 8;
@@ -1814,7 +1814,7 @@ HalfPlan half_plan(int M, int V) {
   p.rows = HALF_AT_ONCE / p.slices < M ? HALF_AT_ONCE / p.slices : M;  // V <= 2^22: at most 65 slices
   if (p.slices > 1 || M < 64) {
     // few rows: more and shorter slices, up to one workgroup a CU, but eight of four granules a thread at most: the second launch
-    // has one workgroup to add the slices' counts (1 x 250002: 31 slices 64 us, 8 slices 23 us)
+    // has one workgroup to add the slices' counts (1 x 250002: 31 slices took 64 us where 8 took 23)
     const int most = (granules + 4 * HWG - 1) / (4 * HWG), want = 256 / p.rows < 8 ? 256 / p.rows : 8;
     const int more = most < want ? most : want;
     p.slices = more > p.slices ? more : p.slices;
@@ -1845,14 +1845,14 @@ template <class T> int launch_half(const cube_sample_args& a, HalfSlice* ws, hip
   return CUBE_OK;
 }
 
-// 16-bit rows longer than this are counted by value (us: bf16 64 x 16000, top-p 16 against 19; bf16 256 x 32000 19 against 33).  f16
-// has eight times as many values to an octave: 256 x 32000, top-p 31 against 33, but top-k 33 against 17 and 1 x 20000 24 against 16.
+// 16-bit rows longer than this are counted by value (us, top-p: bf16 64 x 16000 17 against 18; 256 x 32000 20 against 30).  f16
+// has eight times as many values to an octave: 256 x 32000 33 against 29, top-k 35 against 16, and 1 x 20000 28 against 17.
 template <class T> constexpr int half_v() { return std::is_same<T, bf16_t>::value ? 16000 : MID_V; }
 
 // Rows that go through slices, histogram and list: f32 beyond what a workgroup holds; of f16 up to 32 rows of 2^23 logits in all, while
-// counting by value costs more (us, plain and top-p: 1 x 250002 20 and 25 against 36 and 39;  32 x 40000 25 and 29 against 34 and 36;
-// 32 x 250002 49 and 52 against 48 and 51;  64 x 40000 33 and 39 against 28 and 30).  bf16 has too many equal values for the list
-// (1 x 250002, top-p 30 against 22).
+// counting by value costs more (us, plain, top-p, top-k: 1 x 250002 22 and 30 against 40 and 45;  32 x 40000 27 and 33 against 36 and 39;
+// 8 x 500000 40, 54, 33 against 48, 52, 55;  24 x 250002 52, 60, 40 against 48, 52, 56;  64 x 40000 35 and 41 against 30 and 33).  bf16
+// has too many equal values for the list (1 x 250002, top-p 33 against 24).
 bool sliced(int type, int M, int V) {
   return V > MID_V && (type == CUBE_T_F32 || (type == CUBE_T_F16 && M <= 32 && (long long)M * V <= 1 << 23));
 }
